@@ -63,6 +63,23 @@ class G4qPhasePrologue(ctypes.Structure):
                 ("residual_out", ctypes.c_void_p), ("ld_residual_out", ctypes.c_int64), ("eps", ctypes.c_float)]
 
 
+class G4qHeadRows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("n_heads", ctypes.c_int32)]
+
+
+class G4qPagedCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("n_pages", ctypes.c_int64),
+                ("page_size", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("slot_stride", ctypes.c_int64)]
+
+
+class G4qPagedBatch(ctypes.Structure):
+    _fields_ = [("q_offsets", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("n_seqs", ctypes.c_int32), ("max_pages", ctypes.c_int32),
+                ("max_q", ctypes.c_int32)]
+
+
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
 PHASE_ARGMAX = 0x4
@@ -73,6 +90,13 @@ PATH_GEMV_CLUSTER = 2
 PATH_GEMM = 3
 PATH_GENERIC = 4
 IPC_HANDLE_BYTES = 64
+APPEND_RAW_VALUES = 0x1
+ERR_PAGE = 60       # g4q_device_error: a page id outside the cache
+ERR_TABLE = 61      # a sequence longer than its row of the block table
+ERR_LENS = 62       # offsets or lengths that do not fit together
+_HR = ctypes.POINTER(G4qHeadRows)
+_PC = ctypes.POINTER(G4qPagedCache)
+_PB = ctypes.POINTER(G4qPagedBatch)
 
 SIGNATURES = {
     "g4q_runtime_version": [ctypes.POINTER(G4qVersionInfo)],
@@ -99,6 +123,13 @@ SIGNATURES = {
     "g4q_geglu": [_P, _I64, _P, _I64, _I64, _I64, _P, _I64, _P],
     "g4q_rms_norm": [_P, _I64, _P, _I64, _I64, _F, _P, _I64, _P],
     "g4q_rms_norm_residual": [_P, _I64, _P, _I64, _I64, _F, _P, _I64, _P, _P, _I64, _P],
+    "g4q_rope_create": [_I32, _I32, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_P)],
+    "g4q_rope_free": [_P],
+    "g4q_qk_norm_rope": [_P, _HR, _HR, _I64, _P, _P, _P, _F, _HR, _HR, _P],
+    "g4q_kv_append": [_P, _HR, _HR, _HR, _I64, _P, _P, _F, _U32, _HR, _PC, _PB, _P],
+    "g4q_attn_create": [_I32, _I32, _I32, ctypes.POINTER(_P)],
+    "g4q_paged_attention": [_P, _HR, _I64, _PC, _PB, _F, _I32, _HR, _P],
+    "g4q_attn_free": [_P],
     "g4q_device_error": [ctypes.POINTER(_I32), _I32],
     "g4q_decode_plan_create": [ctypes.POINTER(G4qDecodePhase), _I32, _I32, ctypes.POINTER(_P)],
     "g4q_decode_plan_run": [_P, _I64, _F, _F, _I64, _P, _P, _P, _P, _I64, _P],

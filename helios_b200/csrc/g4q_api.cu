@@ -6,6 +6,7 @@
 // (runtime.cc:41-45, 841-846, 900-912), and no C++ exception crossing the boundary.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -14,6 +15,7 @@
 #include <string>
 
 #include "g4q.h"
+#include "g4q_attn.cuh"
 #include "g4q_internal.h"
 
 namespace g4q {
@@ -73,13 +75,13 @@ DeviceScratch& device_scratch() {
     DeviceScratch& s = g_per_dev[d & 63];
     if (s.err == nullptr) {
         constexpr int64_t kRows = 65536, kQuads = 65536;
-        int* err = nullptr;
+        int* err = nullptr;   // the error word, then the input-error word
         float* rms = nullptr;
         int* counters = nullptr;
-        check_cuda(cudaMalloc(&err, sizeof(int)), "cudaMalloc(device error word)");
+        check_cuda(cudaMalloc(&err, 2 * sizeof(int)), "cudaMalloc(device error word)");
         cudaError_t e = cudaMalloc(&rms, kRows * sizeof(float));
         if (e == cudaSuccess) e = cudaMalloc(&counters, kQuads * sizeof(int));
-        if (e == cudaSuccess) e = cudaMemset(err, 0, sizeof(int));
+        if (e == cudaSuccess) e = cudaMemset(err, 0, 2 * sizeof(int));
         if (e == cudaSuccess) e = cudaMemset(counters, 0, kQuads * sizeof(int));
         if (e == cudaSuccess) e = cudaDeviceSynchronize();
         if (e != cudaSuccess) {
@@ -92,6 +94,7 @@ DeviceScratch& device_scratch() {
         s.rms_rows = kRows;
         s.counters = counters;
         s.counters_n = kQuads;
+        s.input_err = err + 1;
         s.err = err;
     }
     return s;
@@ -967,18 +970,293 @@ G4qStatus g4q_rms_norm_residual(const uint16_t* x, int64_t ldx, const uint16_t* 
     });
 }
 
+static Rope* checked_rope(const G4qRope* h, const char* what) {
+    auto* r = reinterpret_cast<Rope*>(const_cast<G4qRope*>(h));
+    require(r != nullptr, G4Q_ERR_INVALID_ARGUMENT, std::string(what) + " requires a non-null rope handle");
+    require(r->magic == kRopeMagic, G4Q_ERR_INVALID_ARGUMENT, std::string(what) + " received an invalid rope handle");
+    require(r->device == current_device(), G4Q_ERR_INVALID_ARGUMENT,
+            std::string(what) + ": the current CUDA device is not the handle's device");
+    return r;
+}
+
+// One tensor of head rows: element strides in multiples of 8, 16-byte aligned data, heads that do not overlap.
+static void check_heads(const G4qHeadRows* t, int64_t head_dim, const char* name) {
+    const std::string n(name);
+    require(t != nullptr && t->data != nullptr, G4Q_ERR_INVALID_ARGUMENT, n + " must be non-null");
+    require(t->n_heads >= 1 && t->n_heads <= 65536, G4Q_ERR_INVALID_ARGUMENT, n + ".n_heads must be in [1, 65536]");
+    require(t->token_stride % 8 == 0 && t->head_stride % 8 == 0 && t->token_stride >= 0, G4Q_ERR_INVALID_ARGUMENT,
+            n + ": strides must be multiples of 8 elements");
+    require(t->n_heads == 1 || t->head_stride >= head_dim, G4Q_ERR_INVALID_ARGUMENT, n + ".head_stride must be >= head_dim");
+    require_aligned16(t->data, name);
+}
+
+static void check_weight(const uint16_t* w, const char* name) {
+    if (w != nullptr) require_aligned16(w, name);
+}
+
+// The checks that every paged call shares; fills the strides and the batch's view.
+static PagedView checked_batch(const G4qPagedCache* c, const G4qPagedBatch* b, int64_t rows) {
+    require(c != nullptr && c->k != nullptr && c->v != nullptr, G4Q_ERR_INVALID_ARGUMENT, "cache: k and v must be non-null");
+    require_aligned16(c->k, "cache.k");
+    require_aligned16(c->v, "cache.v");
+    require(c->page_size >= 16 && c->page_size <= 65536 && (c->page_size & (c->page_size - 1)) == 0, G4Q_ERR_UNSUPPORTED_CONFIG,
+            "cache.page_size must be a power of two in [16, 65536]");
+    require(c->n_pages >= 1 && c->n_pages < 0x7FFFFFFF, G4Q_ERR_INVALID_ARGUMENT, "cache.n_pages must be in [1, 2^31 - 1)");
+    require(c->n_kv_heads >= 1 && c->n_kv_heads <= 65535, G4Q_ERR_INVALID_ARGUMENT, "cache.n_kv_heads must be in [1, 65535]");
+    for (int64_t s : {c->page_stride, c->head_stride, c->slot_stride})
+        require(s >= c->head_dim && s % 8 == 0 && s < ((int64_t)1 << 38), G4Q_ERR_INVALID_ARGUMENT,
+                "cache strides must be >= head_dim, multiples of 8 elements and below 2^38");
+    require(b != nullptr && b->q_offsets != nullptr && b->kv_lens != nullptr && b->block_table != nullptr,
+            G4Q_ERR_INVALID_ARGUMENT, "batch: q_offsets, kv_lens and block_table must be non-null");
+    for (const void* p : {(const void*)b->q_offsets, (const void*)b->kv_lens, (const void*)b->block_table})
+        require((reinterpret_cast<uintptr_t>(p) & 3u) == 0, G4Q_ERR_INVALID_ARGUMENT, "batch arrays must be 4-byte aligned");
+    require(b->n_seqs >= 1 && b->n_seqs <= 65535, G4Q_ERR_INVALID_ARGUMENT, "batch.n_seqs must be in [1, 65535]");
+    require(b->max_pages >= 1 && b->table_stride >= b->max_pages, G4Q_ERR_INVALID_ARGUMENT,
+            "batch.max_pages must be >= 1 and table_stride >= max_pages");
+    require((int64_t)b->max_pages * c->page_size <= 0x7FFFFFFF - 65536, G4Q_ERR_INVALID_ARGUMENT,
+            "batch.max_pages x page_size must stay below 2^31 - 2^16");
+    require(b->max_q >= 1, G4Q_ERR_INVALID_ARGUMENT, "batch.max_q must be >= 1");
+    require(rows >= 0 && rows <= 0x7FFFFFFF - 65536, G4Q_ERR_INVALID_ARGUMENT, "rows must be in [0, 2^31 - 2^16)");
+    PagedView v;
+    v.q_offsets = b->q_offsets;
+    v.kv_lens = b->kv_lens;
+    v.table = b->block_table;
+    v.table_ld = b->table_stride;
+    v.n_seqs = b->n_seqs;
+    v.max_pages = b->max_pages;
+    v.n_pages = (int)c->n_pages;
+    v.page_shift = __builtin_ctz((unsigned)c->page_size);
+    v.rows = (int)rows;
+    v.max_q = (int)std::min<int64_t>(b->max_q, std::max<int64_t>(rows, 1));
+    v.err = device_scratch().input_err;
+    return v;
+}
+
+G4qStatus g4q_rope_create(int32_t head_dim, int32_t rotary_dim, const double* inv_freq, G4qRope** out) {
+    return guarded("g4q_rope_create", [&] {
+        require(out != nullptr, G4Q_ERR_INVALID_ARGUMENT, "out must be non-null");
+        *out = nullptr;
+        require(head_dim == 64 || head_dim == 128 || head_dim == 256 || head_dim == 512, G4Q_ERR_UNSUPPORTED_CONFIG,
+                "head_dim must be 64, 128, 256 or 512");
+        require(rotary_dim >= 16 && rotary_dim <= head_dim && rotary_dim % 16 == 0, G4Q_ERR_UNSUPPORTED_CONFIG,
+                "rotary_dim must be a multiple of 16 in [16, head_dim]");
+        require(inv_freq != nullptr, G4Q_ERR_INVALID_ARGUMENT, "inv_freq must be non-null");
+        uint64_t turns[256];
+        for (int i = 0; i < rotary_dim / 2; ++i) {
+            require(std::isfinite(inv_freq[i]), G4Q_ERR_INVALID_ARGUMENT, "inv_freq must be finite");
+            // the fraction of a turn per position; whole turns drop out, positions being integers
+            const long double t = (long double)inv_freq[i] / 6.283185307179586476925286766559005768L;
+            const long double f = std::ldexp(t - std::floor(t), 64);
+            turns[i] = f >= 18446744073709551615.0L ? 0 : (uint64_t)(f + 0.5L);
+        }
+        device_scratch();   // holds the input-error word; created here, as no call inside a capture may allocate
+        auto* r = new (std::nothrow) Rope();
+        require(r != nullptr, G4Q_ERR_MEMORY_GUARD, "host allocation failed");
+        r->head_dim = head_dim;
+        r->rotary = rotary_dim;
+        const size_t bytes = (size_t)rotary_dim / 2 * sizeof(uint64_t);
+        cudaError_t e = cudaGetDevice(&r->device);
+        if (e == cudaSuccess) e = cudaMalloc(&r->turns, bytes);
+        if (e == cudaSuccess) e = cudaMemcpy(r->turns, turns, bytes, cudaMemcpyHostToDevice);
+        if (e == cudaSuccess) e = cudaDeviceSynchronize();
+        if (e != cudaSuccess) {
+            cudaFree(r->turns);
+            delete r;
+            check_cuda(e, "rope table");
+        }
+        r->magic = kRopeMagic;
+        *out = reinterpret_cast<G4qRope*>(r);
+    });
+}
+
+G4qStatus g4q_rope_free(G4qRope* h) {
+    return guarded("g4q_rope_free", [&] {
+        auto* r = reinterpret_cast<Rope*>(h);
+        require(r != nullptr, G4Q_ERR_INVALID_ARGUMENT, "requires a non-null rope handle");
+        require(r->magic == kRopeMagic, G4Q_ERR_INVALID_ARGUMENT, "received an invalid rope handle");
+        r->magic = 0;
+        int prev = 0;
+        cudaGetDevice(&prev);
+        cudaSetDevice(r->device);
+        cudaFree(r->turns);
+        cudaSetDevice(prev);
+        delete r;
+    });
+}
+
+static HeadRowsCall head_rows_call(const Rope& r, const G4qHeadRows* q, const G4qHeadRows* q_out, const G4qHeadRows* k,
+                                   int64_t M, const uint16_t* q_weight, const uint16_t* k_weight, float eps) {
+    require(eps >= 0.0f && std::isfinite(eps), G4Q_ERR_INVALID_ARGUMENT, "eps must be finite and >= 0");
+    check_weight(q_weight, "q_weight");
+    check_weight(k_weight, "k_weight");
+    HeadRowsCall c = {};
+    c.rows = M;
+    c.rotary = r.rotary;
+    c.turns = r.turns;
+    c.eps = eps;
+    c.q_weight = q_weight;
+    c.k_weight = k_weight;
+    if (q != nullptr) {
+        check_heads(q, r.head_dim, "q");
+        check_heads(q_out, r.head_dim, "q_out");
+        require(q_out->n_heads == q->n_heads, G4Q_ERR_INVALID_ARGUMENT, "q_out must have q's heads");
+        c.q = q->data, c.q_t = q->token_stride, c.q_h = q->head_stride, c.hq = q->n_heads;
+        c.q_out = q_out->data, c.qo_t = q_out->token_stride, c.qo_h = q_out->head_stride;
+    }
+    if (k != nullptr) {
+        check_heads(k, r.head_dim, "k");
+        c.k = k->data, c.k_t = k->token_stride, c.k_h = k->head_stride, c.hk = k->n_heads;
+    }
+    return c;
+}
+
+G4qStatus g4q_qk_norm_rope(const G4qRope* rope, const G4qHeadRows* q, const G4qHeadRows* k, int64_t M,
+                           const int32_t* positions, const uint16_t* q_weight, const uint16_t* k_weight, float eps,
+                           const G4qHeadRows* q_out, const G4qHeadRows* k_out, void* stream) {
+    return guarded("g4q_qk_norm_rope", [&] {
+        Rope* r = checked_rope(rope, "g4q_qk_norm_rope");
+        require(M >= 0 && M < 0x7FFFFFFF, G4Q_ERR_INVALID_ARGUMENT, "M must be in [0, 2^31 - 1)");
+        if (M == 0) return;
+        require(q != nullptr || k != nullptr, G4Q_ERR_INVALID_ARGUMENT, "one of q and k must be non-null");
+        require(positions != nullptr && (reinterpret_cast<uintptr_t>(positions) & 3u) == 0, G4Q_ERR_INVALID_ARGUMENT,
+                "positions must be non-null and 4-byte aligned");
+        HeadRowsCall c = head_rows_call(*r, q, q_out, k, M, q_weight, k_weight, eps);
+        c.positions = positions;
+        if (k != nullptr) {
+            check_heads(k_out, r->head_dim, "k_out");
+            require(k_out->n_heads == k->n_heads, G4Q_ERR_INVALID_ARGUMENT, "k_out must have k's heads");
+            c.k_out = k_out->data, c.ko_t = k_out->token_stride, c.ko_h = k_out->head_stride;
+        }
+        launch_head_rows(c, r->head_dim, false, reinterpret_cast<cudaStream_t>(stream));
+    });
+}
+
+G4qStatus g4q_kv_append(const G4qRope* rope, const G4qHeadRows* q, const G4qHeadRows* k, const G4qHeadRows* v, int64_t M,
+                        const uint16_t* q_weight, const uint16_t* k_weight, float eps, uint32_t flags,
+                        const G4qHeadRows* q_out, const G4qPagedCache* cache, const G4qPagedBatch* batch, void* stream) {
+    return guarded("g4q_kv_append", [&] {
+        Rope* r = checked_rope(rope, "g4q_kv_append");
+        require((flags & ~G4Q_APPEND_RAW_VALUES) == 0, G4Q_ERR_INVALID_ARGUMENT, "unknown flag bits");
+        const PagedView pv = checked_batch(cache, batch, M);
+        require(cache->head_dim == r->head_dim, G4Q_ERR_INVALID_ARGUMENT, "the cache's head_dim is not the rope's");
+        if (M == 0) return;
+        require(k != nullptr && v != nullptr, G4Q_ERR_INVALID_ARGUMENT, "k and v must be non-null");
+        HeadRowsCall c = head_rows_call(*r, q, q_out, k, M, q_weight, k_weight, eps);
+        check_heads(v, r->head_dim, "v");
+        require(k->n_heads == cache->n_kv_heads && v->n_heads == cache->n_kv_heads, G4Q_ERR_INVALID_ARGUMENT,
+                "k and v must have the cache's heads");
+        c.v = v->data, c.v_t = v->token_stride, c.v_h = v->head_stride, c.hv = v->n_heads;
+        c.raw_v = (flags & G4Q_APPEND_RAW_VALUES) ? 1 : 0;
+        c.k_out = cache->k, c.v_out = cache->v;
+        c.ko_h = cache->head_stride, c.page_stride = cache->page_stride, c.slot_stride = cache->slot_stride;
+        c.pv = pv;
+        launch_head_rows(c, r->head_dim, true, reinterpret_cast<cudaStream_t>(stream));
+    });
+}
+
+static Attn* checked_attn(const G4qAttn* h, const char* what) {
+    auto* a = reinterpret_cast<Attn*>(const_cast<G4qAttn*>(h));
+    require(a != nullptr, G4Q_ERR_INVALID_ARGUMENT, std::string(what) + " requires a non-null attention handle");
+    require(a->magic == kAttnMagic, G4Q_ERR_INVALID_ARGUMENT, std::string(what) + " received an invalid attention handle");
+    require(a->device == current_device(), G4Q_ERR_INVALID_ARGUMENT,
+            std::string(what) + ": the current CUDA device is not the handle's device");
+    return a;
+}
+
+G4qStatus g4q_attn_create(int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, G4qAttn** out) {
+    return guarded("g4q_attn_create", [&] {
+        require(out != nullptr, G4Q_ERR_INVALID_ARGUMENT, "out must be non-null");
+        *out = nullptr;
+        require(head_dim == 64 || head_dim == 128 || head_dim == 256 || head_dim == 512, G4Q_ERR_UNSUPPORTED_CONFIG,
+                "head_dim must be 64, 128, 256 or 512");
+        require(n_kv_heads >= 1 && n_q_heads >= n_kv_heads && n_q_heads % n_kv_heads == 0, G4Q_ERR_INVALID_ARGUMENT,
+                "n_q_heads must be a positive multiple of n_kv_heads");
+        require(n_q_heads / n_kv_heads <= 64 && n_kv_heads <= 65535, G4Q_ERR_UNSUPPORTED_CONFIG,
+                "at most 64 query heads per key head and 65535 key heads");
+        device_scratch();
+        auto* a = new (std::nothrow) Attn();
+        require(a != nullptr, G4Q_ERR_MEMORY_GUARD, "host allocation failed");
+        a->hq = n_q_heads;
+        a->hk = n_kv_heads;
+        a->head_dim = head_dim;
+        cudaError_t e = cudaGetDevice(&a->device);
+        size_t rows = 0;
+        if (e == cudaSuccess) {
+            try {
+                rows = attn_part_rows(head_dim);
+            } catch (const Error&) {
+                e = cudaErrorUnknown;
+            }
+        }
+        if (e == cudaSuccess) e = cudaMalloc(&a->part_o, rows * head_dim * sizeof(float));
+        if (e == cudaSuccess) e = cudaMalloc(&a->part_ml, rows * 2 * sizeof(float));
+        if (e != cudaSuccess) {
+            cudaFree(a->part_o);
+            cudaFree(a->part_ml);
+            delete a;
+            check_cuda(e, "attention scratch");
+        }
+        a->magic = kAttnMagic;
+        *out = reinterpret_cast<G4qAttn*>(a);
+    });
+}
+
+G4qStatus g4q_attn_free(G4qAttn* h) {
+    return guarded("g4q_attn_free", [&] {
+        auto* a = reinterpret_cast<Attn*>(h);
+        require(a != nullptr, G4Q_ERR_INVALID_ARGUMENT, "requires a non-null attention handle");
+        require(a->magic == kAttnMagic, G4Q_ERR_INVALID_ARGUMENT, "received an invalid attention handle");
+        a->magic = 0;
+        int prev = 0;
+        cudaGetDevice(&prev);
+        cudaSetDevice(a->device);
+        cudaFree(a->part_o);
+        cudaFree(a->part_ml);
+        cudaSetDevice(prev);
+        delete a;
+    });
+}
+
+G4qStatus g4q_paged_attention(const G4qAttn* attn, const G4qHeadRows* q, int64_t M, const G4qPagedCache* cache,
+                              const G4qPagedBatch* batch, float scale, int32_t window, const G4qHeadRows* out,
+                              void* stream) {
+    return guarded("g4q_paged_attention", [&] {
+        Attn* a = checked_attn(attn, "g4q_paged_attention");
+        const PagedView pv = checked_batch(cache, batch, M);
+        require(cache->head_dim == a->head_dim && cache->n_kv_heads == a->hk, G4Q_ERR_INVALID_ARGUMENT,
+                "the cache's head_dim and heads are not the handle's");
+        require(std::isfinite(scale) && scale > 0.0f, G4Q_ERR_INVALID_ARGUMENT, "scale must be finite and positive");
+        require(window >= 0, G4Q_ERR_INVALID_ARGUMENT, "window must be >= 0 (0: none)");
+        if (M == 0) return;
+        check_heads(q, a->head_dim, "q");
+        check_heads(out, a->head_dim, "out");
+        require(q->n_heads == a->hq && out->n_heads == a->hq, G4Q_ERR_INVALID_ARGUMENT,
+                "q and out must have the handle's query heads");
+        AttnCall c = {};
+        c.q = q->data, c.q_t = q->token_stride, c.q_h = q->head_stride;
+        c.out = out->data, c.o_t = out->token_stride, c.o_h = out->head_stride;
+        c.k = cache->k, c.v = cache->v;
+        c.page_stride = cache->page_stride, c.head_stride = cache->head_stride, c.slot_stride = cache->slot_stride;
+        c.hq = a->hq, c.hk = a->hk;
+        c.scale = scale;
+        c.window = window;
+        c.pv = pv;
+        launch_attention(*a, c, reinterpret_cast<cudaStream_t>(stream));
+    });
+}
+
 G4qStatus g4q_device_error(int32_t* code, int32_t reset) {
     return guarded("g4q_device_error", [&] {
         require(code != nullptr, G4Q_ERR_INVALID_ARGUMENT, "requires a non-null code pointer");
         // nothing is allocated here: a device on which only the allocation-free entry point ran
         // has no library scratch yet, and its error word is the entry point's static one
-        int v = 0;
+        int v[2] = {0, 0};
         if (DeviceScratch* ds = device_scratch_if_created()) {
-            check_cuda(cudaMemcpy(&v, ds->err, sizeof(int), cudaMemcpyDeviceToHost), "read device error word");
-            if (reset && v != 0) check_cuda(cudaMemset(ds->err, 0, sizeof(int)), "reset device error word");
+            check_cuda(cudaMemcpy(v, ds->err, sizeof(v), cudaMemcpyDeviceToHost), "read device error word");
+            if (reset && (v[0] != 0 || v[1] != 0)) check_cuda(cudaMemset(ds->err, 0, sizeof(v)), "reset device error word");
         }
         const int v2 = noalloc_error(reset != 0);
-        *code = v != 0 ? v : v2;
+        *code = v[0] != 0 ? v[0] : v2 != 0 ? v2 : v[1];
     });
 }
 

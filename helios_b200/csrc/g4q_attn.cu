@@ -1,0 +1,639 @@
+// g4q_attn.cu -- attention of a few new tokens per sequence over a paged cache (sm_100a): one decoded token
+// each, or a block of drafted ones, up to 64 query rows (tokens x query heads of a key head) per key head.
+//
+//   out = softmax(scale * q k^T + mask) v, masked to the positions j <= t (and j > t - window)
+//
+// Bound by HBM: K and V are read once, for all the query heads of the group, and everything else is small.
+// The work is a list of (sequence, key head, 64-key tile), cut into equal contiguous ranges of tiles, one per
+// CTA: every SM streams the same number of bytes whatever the lengths are, and the TMA ring runs on from one
+// sequence to the next without a pause. A range that ends inside a sequence leaves its fp32 partial
+// (unnormalized output, running maximum and sum per row) in the handle's scratch, at most two per CTA, and the
+// combine kernel joins a sequence's partials in CTA order, so results do not depend on timing.
+//
+// In a CTA one warp feeds the ring (SWIZZLE_128B boxes of one page x 64 elements) and eight compute warps
+// share each tile: for the scores, warp w takes keys 8w..8w+7 against all query rows (mma.sync, rows padded
+// to 16); the running softmax is in fp32 over 16-key slices per thread; for the output, warp w takes head_dim/8
+// columns over the 64 keys. mma.sync is enough here: at 64 rows a tile's products take less time than its bytes.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "g4q_attn.cuh"
+#include "g4q_common.cuh"
+#include "g4q_internal.h"
+
+namespace g4q {
+namespace {
+
+constexpr int kKeys = 64;            // keys per tile
+constexpr int kComputeWarps = 8;
+constexpr int kThreads = (kComputeWarps + 1) * 32;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int D, int MT>
+struct FewCfg {
+    static constexpr int kRows = 16 * MT;
+    static constexpr int kCols = D < 256 ? D : 256;          // elements of a ring stage's rows
+    static constexpr int kParts = D / kCols;                 // stages of one K (or V) tile
+    static constexpr int kStageBytes = kKeys * kCols * 2;
+    static constexpr int kQBytes = kRows * D * 2;
+    static constexpr int kSLd = kKeys + 8;                   // fp32 row stride of the scores: conflict free
+    static constexpr int kSBytes = kRows * kSLd * 4;
+    static constexpr int kPBytes = kRows * kKeys * 2;
+    static constexpr int kFixed = kQBytes + kSBytes + kPBytes + kRows * 12 + 256 + 1024;
+    // two CTAs per SM where three stages each fit (one CTA's prologue and combine then hide behind the other);
+    // else one CTA with the ring as deep as fits
+    static constexpr bool kTwo = kFixed + 3 * kParts * kStageBytes <= 113 * 1024 && kParts == 1;
+    static constexpr int kFit = ((kTwo ? 113 : 226) * 1024 - kFixed) / kStageBytes;
+    static constexpr int kStages = kFit > 8 ? 8 : kFit;
+    static constexpr int kSmem = kFixed + kStages * kStageBytes;
+    static_assert(kStages >= 2 * kParts && kSmem <= 227 * 1024, "ring does not fit");
+};
+
+struct FewCall {
+    AttnCall a;
+    int group;          // query heads per key head
+    int max_rows;       // sequences of more rows (tokens x group) belong to the chunk kernel
+    int box;            // keys per TMA box: min(page_size, 64)
+    int ctas;
+    int part_rows;      // rows of a partial
+    float* part_o;      // [2 * ctas][part_rows][D]
+    float* part_ml;     // [2 * ctas][part_rows][2]
+    int* err;           // wait-error word
+};
+
+struct SeqWork {
+    SeqGeom g;
+    int lo;             // first key of the first tile
+    int nt;             // 64-key tiles, 0: nothing for this kernel
+};
+
+__device__ __forceinline__ SeqWork seq_work(const FewCall& c, int b) {
+    SeqWork w;
+    w.g = seq_geom(c.a.pv, b);
+    w.lo = 0;
+    w.nt = 0;
+    if (w.g.q_len == 0 || w.g.q_len * c.group > c.max_rows) return w;
+    if (c.a.window > 0) w.lo = min(max(0, w.g.first - c.a.window + 1), w.g.kv_len) & ~(c.box - 1);
+    w.nt = max(1, (w.g.kv_len - w.lo + kKeys - 1) / kKeys);   // a sequence without keys still writes zeros
+    return w;
+}
+
+__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+
+// Tiles of sequences [0, end), summed by one warp.
+__device__ __forceinline__ int64_t tiles_before(const FewCall& c, int end, int lane) {
+    int64_t t = 0;
+    for (int b = lane; b < end; b += 32) t += seq_work(c, b).nt;
+    return warp_sum64(t) * c.a.hk;
+}
+
+// A position in the list of tiles.
+struct Cursor {
+    int b, h, t;        // sequence, key head, tile
+    SeqWork w;
+    __device__ __forceinline__ void next_unit(const FewCall& c) {
+        t = 0;
+        if (++h < c.a.hk) return;
+        h = 0;
+        do {
+            ++b;
+            if (b < c.a.pv.n_seqs) w = seq_work(c, b);
+        } while (b < c.a.pv.n_seqs && w.nt == 0);
+    }
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix4t(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+template <int D, int MT>
+__global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
+    attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                    const __grid_constant__ FewCall c) {
+    using C = FewCfg<D, MT>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int start[4];                 // b, h, t and the number of tiles of this CTA
+    const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_addr(smem_raw));
+    const uint32_t s_ring = base;
+    const uint32_t s_q = s_ring + C::kStages * C::kStageBytes;
+    const uint32_t s_p = s_q + C::kQBytes;
+    const uint32_t s_bar = s_p + C::kPBytes;
+    float* s_s = reinterpret_cast<float*>(gen + (s_bar - base) + 256);
+    float* s_alpha = s_s + C::kRows * C::kSLd;       // rescaling factor of a row's output
+    float* s_sum = s_alpha + C::kRows;
+    float* s_max = s_sum + C::kRows;
+    auto full = [&](int s) { return s_bar + 8u * s; };
+    auto empty = [&](int s) { return s_bar + 8u * (C::kStages + s); };
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    wait_for_predecessor();
+    release_successor();
+    if (warp == kComputeWarps) {
+        // this CTA's range of tiles and the place of its first one
+        const int64_t total = tiles_before(c, c.a.pv.n_seqs, lane);
+        const int64_t t0 = total * blockIdx.x / c.ctas, t1 = total * (blockIdx.x + 1) / c.ctas;
+        int64_t before = 0;
+        int found = -1;
+        int64_t rest = 0;
+        for (int b0 = 0; b0 < c.a.pv.n_seqs && found < 0 && t1 > t0; b0 += 32) {
+            const int nt = b0 + lane < c.a.pv.n_seqs ? seq_work(c, b0 + lane).nt : 0;
+            int64_t inc = (int64_t)nt * c.a.hk;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+                if (lane >= o) inc += v;
+            }
+            const unsigned past = __ballot_sync(0xFFFFFFFFu, before + inc > t0);
+            if (past != 0) {
+                const int at = __ffs(past) - 1;
+                const int64_t end = __shfl_sync(0xFFFFFFFFu, inc, at);
+                const int n = __shfl_sync(0xFFFFFFFFu, nt, at);
+                found = b0 + at;
+                rest = t0 - (before + end - (int64_t)n * c.a.hk);
+                if (lane == 0) {
+                    start[0] = found;
+                    start[1] = (int)(rest / n);
+                    start[2] = (int)(rest % n);
+                }
+            }
+            before += __shfl_sync(0xFFFFFFFFu, inc, 31);
+        }
+        if (lane == 0) {
+            start[3] = found < 0 ? 0 : (int)(t1 - t0);
+            for (int s = 0; s < C::kStages; ++s) {
+                bar_init(full(s), 1);
+                bar_init(empty(s), 1);
+            }
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+    }
+    __syncthreads();
+    int left = start[3];
+    Cursor cur;
+    cur.b = start[0];
+    cur.h = start[1];
+    cur.t = start[2];
+    if (left > 0) {
+        cur.w = seq_work(c, cur.b);
+
+        if (warp == kComputeWarps) {
+            // ---------------- producer: K then V of every tile, in ring order
+            int stage = 0;
+            uint32_t round = 0;
+            const int boxes = kKeys / c.box;
+            const PagedView& pv = c.a.pv;
+            const int page_mask = (1 << pv.page_shift) - 1;
+            const uint32_t box_bytes = (uint32_t)c.box * 128u;
+            while (left > 0) {
+                const int k0 = cur.w.lo + cur.t * kKeys;
+                // the boxes that hold a key of the sequence; the others are zeroed (V) or masked (K)
+                const int nb = min(boxes, (cur.w.g.kv_len - k0 + c.box - 1) / c.box);
+#pragma unroll 1
+                for (int part = 0; part < 2 * C::kParts; ++part) {
+                    if (round > 0) bar_wait(empty(stage), (round - 1) & 1, c.err, 70);
+                    const CUtensorMap* map = part < C::kParts ? &tm_k : &tm_v;
+                    const int col0 = (part % C::kParts) * C::kCols;
+                    if (lane == 0) bar_expect_tx(full(stage), (uint32_t)max(nb, 0) * box_bytes * (C::kCols / 64));
+                    __syncwarp();
+                    for (int i = lane; i < nb * (C::kCols / 64); i += 32) {
+                        const int box = i / (C::kCols / 64), cb = i % (C::kCols / 64);
+                        const int key = k0 + box * c.box;
+                        int page = pv.table[cur.b * pv.table_ld + (key >> pv.page_shift)];
+                        if (page < 0 || page >= pv.n_pages) {
+                            record_input_error(pv.err, kErrPage);
+                            page = pv.n_pages;                 // outside the map: reads zeros
+                        }
+                        tma_load_page(s_ring + stage * C::kStageBytes + cb * (kKeys * 128) + box * box_bytes, map,
+                                      col0 + cb * 64, key & page_mask, cur.h, page, full(stage));
+                    }
+                    if (++stage == C::kStages) stage = 0, ++round;
+                }
+                --left;
+                if (++cur.t == cur.w.nt && left > 0) cur.next_unit(c);
+            }
+        } else {
+            // ---------------- compute
+            constexpr int kTpr = 256 / C::kRows;             // threads per row in the softmax
+            constexpr int kKpt = kKeys / kTpr;               // keys per thread
+            constexpr int kNt = D / 64;                      // 8-column tiles per warp in the output
+            const int gi = lane >> 2, t4 = lane & 3;
+            const int srow = threadIdx.x / kTpr, sj = threadIdx.x % kTpr;
+            const float scale2 = c.a.scale * kLog2e;
+            int stage = 0, v_held = -1;      // v_held: V stage(s) not handed back yet
+            uint32_t round = 0;
+            while (left > 0) {
+                // one unit: the tiles of (b, h) in this CTA's range
+                const SeqGeom g = cur.w.g;
+                const int rows = g.q_len * c.group;
+                const int n = min(left, cur.w.nt - cur.t);
+                const bool whole = n == cur.w.nt, first_part = cur.t > 0;
+                for (int i = threadIdx.x; i < C::kRows * (D / 8); i += 256) {
+                    const int r = i / (D / 8), ch = i % (D / 8);
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (r < rows) {
+                        const int tok = r / c.group, hd = cur.h * c.group + r % c.group;
+                        v = *reinterpret_cast<const uint4*>(c.a.q + (int64_t)(g.q0 + tok) * c.a.q_t + (int64_t)hd * c.a.q_h + ch * 8);
+                    }
+                    *reinterpret_cast<uint4*>(gen + (s_q - base) + (ch >> 3) * (C::kRows * 128) + r * 128 +
+                                              (((ch & 7) ^ (r & 7)) << 4)) = v;
+                }
+                // keys a row sees: [vis_lo, vis_hi)
+                int vis_lo = 0, vis_hi = 0;
+                if (srow < rows) {
+                    const int pos = g.first + srow / c.group;
+                    vis_hi = min(max(0, pos + 1), g.kv_len);
+                    if (c.a.window > 0) vis_lo = max(0, pos - c.a.window + 1);
+                }
+                // keys some row of the unit sees: V outside of them is not looked at (it may hold anything)
+                const int any_lo = c.a.window > 0 ? max(0, g.first - c.a.window + 1) : 0;
+                float m = -INFINITY, l = 0.0f;
+                float o[MT][kNt][4];
+#pragma unroll
+                for (int a = 0; a < MT; ++a)
+#pragma unroll
+                    for (int b = 0; b < kNt; ++b)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[a][b][e] = 0.0f;
+                compute_sync();
+                for (int it = 0; it < n; ++it) {
+                    const int k0 = cur.w.lo + (cur.t + it) * kKeys;
+                    // ---- scores of keys 8w..8w+7
+                    float s[MT][4];
+#pragma unroll
+                    for (int a = 0; a < MT; ++a)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[a][e] = 0.0f;
+                    int st = stage;
+                    uint32_t rd = round;
+#pragma unroll
+                    for (int part = 0; part < C::kParts; ++part) {
+                        bar_wait(full(st), rd & 1, c.err, 71);
+                        const uint32_t kb = s_ring + st * C::kStageBytes + (8 * warp + (lane & 7)) * 128;
+#pragma unroll(MT == 1 ? 8 : 2)
+                        for (int kk = 0; kk < C::kCols / 32; ++kk) {
+                            const int dc = kk * 4 + (lane >> 3);             // 16-byte chunk of this lane's row
+                            uint32_t b0, b1, b2, b3;
+                            ldmatrix4(kb + (dc >> 3) * (kKeys * 128) + (((dc & 7) ^ (lane & 7)) << 4), b0, b1, b2, b3);
+#pragma unroll
+                            for (int a = 0; a < MT; ++a) {
+#pragma unroll
+                                for (int half = 0; half < 2; ++half) {
+                                    const int qc = part * (C::kCols / 8) + kk * 4 + half * 2 + (lane >> 4);
+                                    const int qr = 16 * a + (lane & 15);
+                                    uint32_t a0, a1, a2, a3;
+                                    ldmatrix4(s_q + (qc >> 3) * (C::kRows * 128) + qr * 128 + (((qc & 7) ^ (qr & 7)) << 4),
+                                              a0, a1, a2, a3);
+                                    mma_bf16_16816(s[a], a0, a1, a2, a3, half ? b2 : b0, half ? b3 : b1);
+                                }
+                            }
+                        }
+                        if (++st == C::kStages) st = 0, ++rd;
+                    }
+#pragma unroll
+                    for (int a = 0; a < MT; ++a) {
+                        float* sr = s_s + (16 * a + gi) * C::kSLd + 8 * warp + 2 * t4;
+                        *reinterpret_cast<float2*>(sr) = make_float2(s[a][0], s[a][1]);
+                        *reinterpret_cast<float2*>(sr + 8 * C::kSLd) = make_float2(s[a][2], s[a][3]);
+                    }
+                    compute_sync();
+                    // every warp is past this tile's K and the previous tile's V
+                    if (threadIdx.x == 0) {
+#pragma unroll
+                        for (int part = 0; part < C::kParts; ++part) {
+                            bar_arrive(empty((stage + part) % C::kStages));
+                            if (v_held >= 0) bar_arrive(empty((v_held + part) % C::kStages));
+                        }
+                    }
+                    stage = st;
+                    round = rd;
+                    v_held = st;
+                    // ---- running softmax: thread (srow, sj) has keys sj * kKpt ..
+                    {
+                        float x[kKpt];
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < kKpt; i += 4) {
+                            const float4 v = *reinterpret_cast<const float4*>(s_s + srow * C::kSLd + sj * kKpt + i);
+                            x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
+                        }
+#pragma unroll
+                        for (int i = 0; i < kKpt; ++i) {
+                            const int key = k0 + sj * kKpt + i;
+                            x[i] = key >= vis_lo && key < vis_hi ? x[i] * scale2 : -INFINITY;
+                            top = fmaxf(top, x[i]);
+                        }
+#pragma unroll
+                        for (int w = kTpr / 2; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, w));
+                        const float m_new = fmaxf(m, top);
+                        const float ref = m_new == -INFINITY ? 0.0f : m_new;      // a row that sees nothing yet
+                        const float alpha = fast_exp2(m - ref);
+                        m = m_new;
+                        float sum = 0.0f;
+                        uint32_t pk[kKpt / 2];
+#pragma unroll
+                        for (int i = 0; i < kKpt; i += 2) {
+                            const float e0 = fast_exp2(x[i] - ref), e1 = fast_exp2(x[i + 1] - ref);
+                            pk[i / 2] = pack_bf16(e0, e1);
+                            // the sum takes the weights as the product will: their bf16 rounding cancels in part
+                            sum += bf16_bits_to_f32(pk[i / 2] & 0xFFFFu) + __uint_as_float(pk[i / 2] & 0xFFFF0000u);
+                        }
+#pragma unroll
+                        for (int w = kTpr / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, w);
+                        l = l * alpha + sum;
+                        if (sj == 0) s_alpha[srow] = alpha;
+                        uint8_t* pr = gen + (s_p - base) + srow * 128;
+#pragma unroll
+                        for (int i = 0; i < kKpt / 2; i += 2) {
+                            const int byte = sj * kKpt * 2 + i * 4;
+                            *reinterpret_cast<uint2*>(pr + (((byte >> 4) ^ (srow & 7)) << 4) + (byte & 15)) =
+                                make_uint2(pk[i], pk[i + 1]);
+                        }
+                    }
+                    // ---- V rows that no row of the unit sees become zeros (a zero weight times NaN is NaN)
+                    if (k0 < any_lo || k0 + kKeys > g.kv_len) {
+                        int vs = stage;
+                        uint32_t vr = round;
+#pragma unroll
+                        for (int part = 0; part < C::kParts; ++part) {
+                            bar_wait(full(vs), vr & 1, c.err, 72);
+                            uint8_t* vb = gen + (s_ring - base) + vs * C::kStageBytes;
+                            for (int i = threadIdx.x; i < kKeys * (C::kCols / 8); i += 256) {
+                                const int key = (i >> 3) & (kKeys - 1);
+                                if (k0 + key < any_lo || k0 + key >= g.kv_len)
+                                    *reinterpret_cast<uint4*>(vb + i * 16) = make_uint4(0, 0, 0, 0);
+                            }
+                            if (++vs == C::kStages) vs = 0, ++vr;
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the stage's next copy
+                    }
+                    compute_sync();
+                    // ---- output columns of this warp
+                    {
+                        constexpr int kWarpCols = D / kComputeWarps;
+                        const int col = warp * kWarpCols;                     // first column of this warp
+                        const int part = col / C::kCols, pc = col % C::kCols;
+                        int vs = stage + part;
+                        uint32_t vr = round;
+                        if (vs >= C::kStages) vs -= C::kStages, ++vr;
+                        bar_wait(full(vs), vr & 1, c.err, 73);
+                        const uint32_t vb = s_ring + vs * C::kStageBytes;
+#pragma unroll
+                        for (int a = 0; a < MT; ++a) {
+                            const float f0 = s_alpha[16 * a + gi], f1 = s_alpha[16 * a + gi + 8];
+#pragma unroll
+                            for (int b = 0; b < kNt; ++b) {
+                                o[a][b][0] *= f0, o[a][b][1] *= f0;
+                                o[a][b][2] *= f1, o[a][b][3] *= f1;
+                            }
+                        }
+#pragma unroll(MT == 1 ? 4 : 1)
+                        for (int kk = 0; kk < kKeys / 16; ++kk) {
+                            uint32_t pa[MT][4];
+#pragma unroll
+                            for (int a = 0; a < MT; ++a) {
+                                const int pr = 16 * a + (lane & 15), ch = kk * 2 + (lane >> 4);
+                                ldmatrix4(s_p + pr * 128 + ((ch ^ (pr & 7)) << 4), pa[a][0], pa[a][1], pa[a][2], pa[a][3]);
+                            }
+                            const int key = kk * 16 + (lane & 15);
+#pragma unroll
+                            for (int b = 0; b < kNt; b += 2) {
+                                uint32_t v0, v1, v2 = 0, v3 = 0;
+                                // D = 64 has one 8-column tile per warp: the upper half re-reads the same chunk
+                                const int ch = (pc >> 3) + b + (kNt > 1 ? (lane >> 4) : 0);
+                                ldmatrix4t(vb + (ch >> 3) * (kKeys * 128) + key * 128 + (((ch & 7) ^ (key & 7)) << 4), v0, v1,
+                                           v2, v3);
+#pragma unroll
+                                for (int a = 0; a < MT; ++a) {
+                                    mma_bf16_16816(o[a][b], pa[a][0], pa[a][1], pa[a][2], pa[a][3], v0, v1);
+                                    if constexpr (kNt > 1)
+                                        mma_bf16_16816(o[a][b + 1], pa[a][0], pa[a][1], pa[a][2], pa[a][3], v2, v3);
+                                }
+                            }
+                        }
+                    }
+                    stage += C::kParts;
+                    if (stage >= C::kStages) stage -= C::kStages, ++round;
+                }
+                // ---- the unit's rows: final, or this CTA's partial
+                if (sj == 0) {
+                    s_sum[srow] = l;
+                    s_max[srow] = m;
+                }
+                compute_sync();
+                const int64_t slot = (int64_t)blockIdx.x * 2 + (first_part ? 0 : 1);
+#pragma unroll
+                for (int a = 0; a < MT; ++a) {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const int r = 16 * a + gi + 8 * half;
+                        if (r >= rows) continue;
+                        const float sum = s_sum[r];
+                        const int col = warp * (D / kComputeWarps) + 2 * t4;
+                        if (whole) {
+                            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // a row that sees nothing is zero
+                            const int tok = r / c.group, hd = cur.h * c.group + r % c.group;
+                            uint16_t* dst = c.a.out + (int64_t)(g.q0 + tok) * c.a.o_t + (int64_t)hd * c.a.o_h + col;
+#pragma unroll
+                            for (int b = 0; b < kNt; ++b)
+                                *reinterpret_cast<uint32_t*>(dst + 8 * b) =
+                                    pack_bf16(o[a][b][2 * half] * inv, o[a][b][2 * half + 1] * inv);
+                        } else {
+                            float* dst = c.part_o + (slot * c.part_rows + r) * D + col;
+#pragma unroll
+                            for (int b = 0; b < kNt; ++b)
+                                *reinterpret_cast<float2*>(dst + 8 * b) = make_float2(o[a][b][2 * half], o[a][b][2 * half + 1]);
+                            if (warp == 0 && t4 == 0)
+                                *reinterpret_cast<float2*>(c.part_ml + (slot * c.part_rows + r) * 2) = make_float2(s_max[r], sum);
+                        }
+                    }
+                }
+                left -= n;
+                cur.t += n;
+                if (left > 0) cur.next_unit(c);
+            }
+        }
+    }
+}
+
+// Joins the partials of the units that CTA ranges cut. One CTA per (token row, query head, 128 columns); its
+// warps take the unit's partials in turn, in CTA order, and their sums are added in warp order.
+constexpr int kJoinWarps = 8;
+
+template <int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const __grid_constant__ FewCall c) {
+    constexpr int kW = D < 128 ? D : 128;        // columns per CTA
+    constexpr int kV = kW / 32;                  // per lane
+    __shared__ float s_ml[kJoinWarps][2];
+    __shared__ float s_o[kJoinWarps][kW];
+    wait_for_predecessor();
+    release_successor();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = blockIdx.y, h = blockIdx.x / c.part_rows, r = blockIdx.x % c.part_rows;
+    const SeqWork w = seq_work(c, b);
+    if (w.nt == 0 || r >= w.g.q_len * c.group) return;
+    // the unit's tiles in the list, and the CTAs whose ranges hold its first and its last one
+    const int64_t total = tiles_before(c, c.a.pv.n_seqs, lane);
+    const int64_t u0 = tiles_before(c, b, lane) + (int64_t)h * w.nt, u1 = u0 + w.nt;
+    const int c0 = (int)(((u0 + 1) * c.ctas - 1) / total), c1 = (int)((u1 * c.ctas - 1) / total);
+    if (c0 == c1) return;                         // one CTA had all of it and wrote the result
+    const int col = blockIdx.z * kW + lane * kV;
+    // A CTA whose range starts with a tile of this unit after its first has it in slot 0; the CTA that has the
+    // unit's first tile, in slot 1.
+    float top = -INFINITY;
+    for (int i = c0 + lane; i <= c1; i += 32) {
+        const int64_t slot = (int64_t)i * 2 + (i == c0 ? 1 : 0);
+        if (total * (i + 1) / c.ctas > total * i / c.ctas) top = fmaxf(top, c.part_ml[(slot * c.part_rows + r) * 2]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float acc[kV];
+#pragma unroll
+    for (int e = 0; e < kV; ++e) acc[e] = 0.0f;
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int i = c0 + warp; i <= c1; i += kJoinWarps) {
+        if (total * (i + 1) / c.ctas <= total * i / c.ctas) continue;
+        const int64_t at = ((int64_t)i * 2 + (i == c0 ? 1 : 0)) * c.part_rows + r;
+        const float f = fast_exp2(c.part_ml[at * 2] - ref);
+        sum += f * c.part_ml[at * 2 + 1];
+        if constexpr (kV == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(c.part_o + at * D + col);
+            acc[0] += f * v.x, acc[1] += f * v.y, acc[2] += f * v.z, acc[3] += f * v.w;
+        } else {
+            const float2 v = *reinterpret_cast<const float2*>(c.part_o + at * D + col);
+            acc[0] += f * v.x, acc[1] += f * v.y;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < kV; ++e) s_o[warp][lane * kV + e] = acc[e];
+    if (lane == 0) s_ml[warp][0] = sum;
+    __syncthreads();
+    if (threadIdx.x < kW / 2) {
+        float lsum = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kJoinWarps; ++i) {
+            lsum += s_ml[i][0];
+            x += s_o[i][2 * threadIdx.x];
+            y += s_o[i][2 * threadIdx.x + 1];
+        }
+        const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+        const int tok = r / c.group, hd = h * c.group + r % c.group;
+        *reinterpret_cast<uint32_t*>(c.a.out + (int64_t)(w.g.q0 + tok) * c.a.o_t + (int64_t)hd * c.a.o_h +
+                                     blockIdx.z * kW + 2 * threadIdx.x) = pack_bf16(x * inv, y * inv);
+    }
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+template <int D, int MT>
+int few_ctas() { return device_sm_count() * (FewCfg<D, MT>::kTwo ? 2 : 1); }
+
+template <int D, int MT>
+void launch_few(const Attn& h, const AttnCall& a, cudaStream_t st) {
+    using C = FewCfg<D, MT>;
+    static bool attr_set[64] = {false};
+    const int dev = current_device();
+    if (!attr_set[dev & 63]) {
+        check_cuda(cudaFuncSetAttribute(attn_few_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
+                   "cudaFuncSetAttribute(attn_few)");
+        attr_set[dev & 63] = true;
+    }
+    const int page_size = 1 << a.pv.page_shift;
+    FewCall c;
+    c.a = a;
+    c.group = a.hq / a.hk;
+    c.max_rows = C::kRows;
+    c.box = std::min(page_size, kKeys);
+    c.part_rows = std::min<int64_t>((int64_t)a.pv.max_q * c.group, C::kRows);
+    c.part_o = h.part_o;
+    c.part_ml = h.part_ml;
+    c.err = device_scratch().err;
+    // no more CTAs than there can be tiles: by the table's capacity, or the window
+    int64_t cap = (int64_t)a.pv.max_pages << a.pv.page_shift;
+    if (a.window > 0) cap = std::min<int64_t>(cap, (int64_t)a.window + c.max_rows / c.group + c.box);
+    const int64_t per_unit = std::max<int64_t>(1, (cap + kKeys - 1) / kKeys);
+    c.ctas = (int)std::min<int64_t>(few_ctas<D, MT>(), per_unit * a.hk * a.pv.n_seqs);
+    const CUtensorMap tk = paged_map(a, a.k, D, c.box), tv = paged_map(a, a.v, D, c.box);
+    launch_dependent(attn_few_kernel<D, MT>, dim3((unsigned)c.ctas), dim3(kThreads), C::kSmem, st, tk, tv, c);
+    if (per_unit > 1) {   // a unit of one tile is never cut
+        const dim3 grid((unsigned)(c.part_rows * a.hk), (unsigned)a.pv.n_seqs, D < 128 ? 1 : D / 128);
+        launch_dependent(attn_join_kernel<D>, grid, dim3(kJoinWarps * 32), 0, st, c);
+    }
+}
+
+template <int D>
+void launch_few_rows(const Attn& h, const AttnCall& a, cudaStream_t st) {
+    const int64_t rows = (int64_t)a.pv.max_q * (a.hq / a.hk);
+    if (rows > 64) throw Error(G4Q_ERR_UNSUPPORTED_CONFIG, "more than 64 query rows per key head");
+    if (rows <= 16)
+        launch_few<D, 1>(h, a, st);
+    else if (rows <= 32)
+        launch_few<D, 2>(h, a, st);
+    else
+        launch_few<D, 4>(h, a, st);
+}
+
+template <int D>
+size_t few_part_rows() {
+    return 2 * std::max({(size_t)few_ctas<D, 1>() * 16, (size_t)few_ctas<D, 2>() * 32, (size_t)few_ctas<D, 4>() * 64});
+}
+
+}  // namespace
+
+CUtensorMap paged_map(const AttnCall& a, const uint16_t* base, int D, int box) {
+    static const EncodeTiledFn encode = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(p);
+    }();
+    if (encode == nullptr) throw Error(G4Q_ERR_RUNTIME, "cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)1 << a.pv.page_shift, (cuuint64_t)a.hk, (cuuint64_t)a.pv.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)a.slot_stride * 2, (cuuint64_t)a.head_stride * 2, (cuuint64_t)a.page_stride * 2};
+    const cuuint32_t shape[4] = {64, (cuuint32_t)box, 1, 1}, es[4] = {1, 1, 1, 1};
+    CUtensorMap m;
+    const CUresult r = encode(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<uint16_t*>(base), dims, strides, shape, es,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw Error(G4Q_ERR_RUNTIME, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+    return m;
+}
+
+size_t attn_part_rows(int head_dim) {
+    switch (head_dim) {
+        case 64: return few_part_rows<64>();
+        case 128: return few_part_rows<128>();
+        case 256: return few_part_rows<256>();
+        default: return few_part_rows<512>();
+    }
+}
+
+void launch_attention(const Attn& h, const AttnCall& a, cudaStream_t st) {
+    switch (h.head_dim) {
+        case 64: return launch_few_rows<64>(h, a, st);
+        case 128: return launch_few_rows<128>(h, a, st);
+        case 256: return launch_few_rows<256>(h, a, st);
+        case 512: return launch_few_rows<512>(h, a, st);
+    }
+}
+
+}  // namespace g4q

@@ -58,6 +58,26 @@ void launch_lora_transpose(const float* b, int64_t N, int rank, float* bt, cudaS
 void launch_lora_apply(const Lora& l, const uint16_t* x, int64_t M, int64_t ldx, uint16_t* y, int64_t ldy,
                        cudaStream_t st);
 
+constexpr uint64_t kRopeMagic = 0x4734515F524F5045ull;    // "G4Q_ROPE"
+constexpr uint64_t kAttnMagic = 0x4734515F4154544Eull;    // "G4Q_ATTN"
+
+// Rotation frequencies: inv_freq / 2 pi in units of 2^-64 turn, [rotary / 2] on the device.
+struct Rope {
+    uint64_t magic = 0;
+    int head_dim = 0, rotary = 0;
+    int device = -1;
+    uint64_t* turns = nullptr;
+};
+
+// Paged attention of one head layout, with the scratch of the partial results.
+struct Attn {
+    uint64_t magic = 0;
+    int hq = 0, hk = 0, head_dim = 0;
+    int device = -1;
+    float* part_o = nullptr;
+    float* part_ml = nullptr;
+};
+
 // round-to-nearest-even of a float to bf16, as a float (host side)
 float bf16_round_host(float f);
 
@@ -98,6 +118,7 @@ size_t max_dynamic_smem(const void* kernel);
 // per-row RMS scales of the prefill GEMM.
 struct DeviceScratch {
     int* err = nullptr;
+    int* input_err = nullptr;    // codes 60-62: what a paged batch's device arrays held (no wait gives up on it)
     float* rms = nullptr;
     int64_t rms_rows = 0;
     float* slots = nullptr;      // stream-K GEMV partial sums

@@ -21,8 +21,8 @@
  *     arrival counters, the prefill GEMM's row scales and split-K partials. Calls that overlap on
  *     the GPU race on it, even on different streams or handles, so issue a device's compute calls
  *     on one stream or order them with events (as the reference's single scheduler thread issues
- *     its matmuls one after another). Decode plans, LoRA handles and the allreduce communicator own
- *     their scratch; the LM head's lives in its weight handle.
+ *     its matmuls one after another). Decode plans, LoRA and attention handles and the allreduce
+ *     communicator own their scratch; the LM head's lives in its weight handle.
  *   - That scratch is never freed while the process runs: it grows at g4q_weight_create (GEMV
  *     slots) or at the first GEMM launch outside a stream capture that needs more (split-K
  *     partials), and a grown buffer replaces the old one without freeing it. A CUDA graph captured
@@ -276,6 +276,94 @@ G4qStatus g4q_rms_norm_residual(const uint16_t* x, int64_t ldx, const uint16_t* 
                                 float eps, const uint16_t* residual, int64_t ld_res, const uint16_t* layer_scalar,
                                 uint16_t* out, int64_t ld_out, void* stream);
 
+/* ---- attention between the q|k|v and the o matmul ---------------------------------------------------
+ * What attention_forward and its decode twins (native_model.cc:788-897, 976-1129, 1131-1282) do to the
+ * q/k/v projections: RMSNorm of every query and key head (:820-860), the values norm without a weight
+ * (:844), fast::rope, the KV cache update and fast::scaled_dot_product_attention with its causal or
+ * sliding-window mask. head_dim is 64, 128, 256 or 512; activations and cache are bf16.
+ *
+ * Head rows: M tokens of n_heads heads of head_dim elements, element strides per token and per head
+ * (multiples of 8, data 16-byte aligned; [M, heads, head_dim] views of a q|k|v matmul's output qualify). */
+typedef struct G4qHeadRows {
+    uint16_t* data;
+    int64_t token_stride;
+    int64_t head_stride;
+    int32_t n_heads;
+} G4qHeadRows;
+
+/* A paged cache of one layer: k and v hold n_pages pages of page_size slots (a power of two, 16 or more) of
+ * n_kv_heads heads; strides in elements, the same for k and v: [pages, heads, slots, head_dim] and
+ * [pages, slots, heads, head_dim] both qualify. */
+typedef struct G4qPagedCache {
+    uint16_t* k;
+    uint16_t* v;
+    int64_t n_pages;
+    int32_t page_size;
+    int32_t n_kv_heads;
+    int32_t head_dim;
+    int64_t page_stride;
+    int64_t head_stride;
+    int64_t slot_stride;
+} G4qPagedCache;
+
+/* The sequences of one step (device arrays of int32, read by the kernels, so a captured graph replays with
+ * what they hold then): sequence b owns the rows [q_offsets[b], q_offsets[b+1]) of the step's M new tokens,
+ * which are the last ones of its kv_lens[b] tokens (the new ones included); its position j is in page
+ * block_table[b * table_stride + j / page_size] at slot j % page_size. Table entries of pages without a token
+ * to read or write are not looked at. max_q: at least the longest q_offsets[b+1] - q_offsets[b]. Rows before
+ * q_offsets[0] or behind q_offsets[n_seqs] belong to no sequence and are left as they were. What the arrays
+ * hold is checked on the device: nothing outside of the cache, the table or the rows is touched, and
+ * g4q_device_error reports 60 (a page id outside the cache: not stored; read as zeros), 61 (a sequence
+ * longer than its table row: its later keys are dropped), 62 (bad offsets, a negative length or more than
+ * max_q new tokens: the sequence is skipped; more new tokens than kv_lens[b]: those before position 0 are
+ * neither stored nor see a key). */
+typedef struct G4qPagedBatch {
+    const int32_t* q_offsets;
+    const int32_t* kv_lens;
+    const int32_t* block_table;
+    int64_t table_stride;
+    int32_t n_seqs;
+    int32_t max_pages;      /* columns of the block table */
+    int32_t max_q;
+} G4qPagedBatch;
+
+/* Rotation frequencies (inv_freq: host array of rotary_dim / 2, in radians per position; the first rotary_dim
+ * elements of a head are rotated in pairs (i, i + rotary_dim / 2), rotary_dim a multiple of 16). The angle
+ * position * inv_freq is reduced in 64-bit integers, so it is exact to 1e-7 at every int32 position. */
+typedef struct G4qRope G4qRope;
+G4qStatus g4q_rope_create(int32_t head_dim, int32_t rotary_dim, const double* inv_freq, G4qRope** out);
+G4qStatus g4q_rope_free(G4qRope* rope);
+
+/* q_out = rope(rms_norm(q) * q_weight), k_out = rope(rms_norm(k) * k_weight) for M tokens at `positions`
+ * (device int32 [M]), in one launch, fp32 inside with one rounding at the end. Weights: bf16 [head_dim] or
+ * NULL (none). q (with q_out) or k (with k_out) may be NULL. An output may be its input (same data and
+ * strides); otherwise they must not overlap. */
+G4qStatus g4q_qk_norm_rope(const G4qRope* rope, const G4qHeadRows* q, const G4qHeadRows* k, int64_t M,
+                           const int32_t* positions, const uint16_t* q_weight, const uint16_t* k_weight, float eps,
+                           const G4qHeadRows* q_out, const G4qHeadRows* k_out, void* stream);
+
+/* The same on the new tokens of a paged batch, at their positions in it: the keys are stored in the cache's
+ * pages, the values beside them (rms_norm without a weight; with G4Q_APPEND_RAW_VALUES as they are). v may be
+ * k (full-attention layers, whose key projection is the value too: :820-822). q (with q_out) may be NULL. */
+#define G4Q_APPEND_RAW_VALUES 0x1u
+G4qStatus g4q_kv_append(const G4qRope* rope, const G4qHeadRows* q, const G4qHeadRows* k, const G4qHeadRows* v, int64_t M,
+                        const uint16_t* q_weight, const uint16_t* k_weight, float eps, uint32_t flags,
+                        const G4qHeadRows* q_out, const G4qPagedCache* cache, const G4qPagedBatch* batch, void* stream);
+
+/* out = softmax(scale * q . k^T) v over the cache, query head h against key head h / (n_q_heads / n_kv_heads);
+ * the query at position t sees the keys j <= t, and j > t - window when window > 0. Single tokens, drafted
+ * blocks and prompt chunks may be mixed in one call. A row that sees no key is zero. What the cache holds at
+ * slots that no query of a sequence's step sees does not matter (NaN included); a non-finite value that some
+ * query of the step sees may reach the step's other queries of that sequence. The handle owns the scratch of
+ * partial results: calls on one handle must not overlap on the GPU (one stream, or events), replays of graphs
+ * that captured it included. Allocates nothing. */
+typedef struct G4qAttn G4qAttn;
+G4qStatus g4q_attn_create(int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, G4qAttn** out);
+G4qStatus g4q_paged_attention(const G4qAttn* attn, const G4qHeadRows* q, int64_t M, const G4qPagedCache* cache,
+                              const G4qPagedBatch* batch, float scale, int32_t window, const G4qHeadRows* out,
+                              void* stream);
+G4qStatus g4q_attn_free(G4qAttn* attn);
+
 /* ---- decode plan: every quantized matmul of one decode step in one persistent kernel ----------
  * Replaces the per-token chain of quantized_linear calls of the decode drivers
  * (native_model.cc:1843-1911 decode_last_logits -> 48 x target_layer_decode_forward :1284-1328 ->
@@ -404,7 +492,8 @@ G4qStatus g4q_comm_free(G4qComm* comm);
  * Every wait inside a libg4q kernel is bounded; a wait that gives up records a nonzero code in a
  * per-device error word and the kernel runs to its end (its results are then invalid). This
  * reads the word for the current device (synchronising it) and optionally clears it; it also
- * reports (and clears) code 50 of g4q_lm_head_argmax_noalloc, and allocates nothing. No
+ * reports (and clears) code 50 of g4q_lm_head_argmax_noalloc and the codes 60-62 of a paged batch
+ * (G4qPagedBatch), and allocates nothing. No
  * reference counterpart: the reference's MLX graph has no device-side waits. */
 G4qStatus g4q_device_error(int32_t* code, int32_t reset);
 
