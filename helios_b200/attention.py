@@ -22,41 +22,59 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from .quantized import _ptr, _stream
 
 __all__ = ["Rope", "PagedKVCache", "PagedBatch", "PagedAttention", "qk_norm_rope", "kv_append"]
 
 
-def _head_rows(t: torch.Tensor, head_dim: int, name: str, out: bool = False) -> _lib.G4qHeadRows:
-    """The C view of a [tokens, heads, head_dim] tensor (any strides that keep 16-byte chunks whole)."""
-    if t.dtype != torch.bfloat16 or not t.is_cuda:
-        raise ValueError(f"{name} must be a bfloat16 CUDA tensor")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is not on the current CUDA device")
-    if t.dim() != 3 or t.shape[2] != head_dim:
-        raise ValueError(f"{name} must be [tokens, heads, {head_dim}] (got {tuple(t.shape)})")
+_BF16 = torch.bfloat16
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _head_rows(t: torch.Tensor, head_dim: int, device: int, name: str, out: bool = False) -> _lib.G4qHeadRows:
+    """The C view of a [tokens, heads, head_dim] tensor (any strides that keep 16-byte chunks whole). These
+    checks run on every call of a decode step, so they stay a few attribute reads per tensor."""
+    if t.dtype is not _BF16 or t.get_device() != device:
+        raise ValueError(f"{name} must be a bfloat16 CUDA tensor on cuda:{device} (got {t.dtype} on {t.device})")
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != head_dim:
+        raise ValueError(f"{name} must be [tokens, heads, {head_dim}] (got {tuple(shape)})")
     st, sh, sd = t.stride()
-    if sd != 1 or st % 8 or sh % 8 or t.data_ptr() % 16:
+    data = t.data_ptr()
+    if sd != 1 or (st | sh) & 7 or data & 15:
         raise ValueError(f"{name}: the last dimension must be contiguous, strides multiples of 8 and data 16-byte aligned")
-    if out and ((t.shape[0] > 1 and st < head_dim) or (t.shape[1] > 1 and sh < head_dim)):
+    if shape[1] == 1:
+        sh = max(sh, head_dim)
+    if out and (sh < head_dim or (shape[0] > 1 and st < head_dim)):
         raise ValueError(f"{name}: its rows overlap")
-    return _lib.G4qHeadRows(t.data_ptr(), st, sh if t.shape[1] > 1 else max(sh, head_dim), t.shape[1])
+    return _lib.G4qHeadRows(data, st, sh, shape[1])
 
 
-def _norm_weight(w: Optional[torch.Tensor], head_dim: int, like: torch.Tensor, name: str) -> Optional[torch.Tensor]:
+def _norm_weight(w: Optional[torch.Tensor], head_dim: int, device: int, name: str) -> Optional[int]:
     if w is None:
         return None
-    if w.dtype != torch.bfloat16 or w.shape != (head_dim,) or w.device != like.device or not w.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous bf16 tensor of shape ({head_dim},) on {like.device}")
-    return w
+    if w.dtype is not _BF16 or w.get_device() != device or w.shape != (head_dim,) or not w.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous bf16 tensor of shape ({head_dim},) on cuda:{device}")
+    return w.data_ptr()
 
 
 def _int32(t: torch.Tensor, dims: int, name: str) -> torch.Tensor:
-    if t.dtype != torch.int32 or not t.is_cuda or t.dim() != dims or (t.numel() and t.stride(-1) != 1):
+    if t.dtype is not torch.int32 or not t.is_cuda or t.dim() != dims or (t.numel() and t.stride(-1) != 1):
         raise ValueError(f"{name} must be a {dims}-D int32 CUDA tensor with contiguous rows")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is not on the current CUDA device")
     return t
+
+
+def _same_device(device: int, **what) -> None:
+    for name, x in what.items():
+        if x.device != device:
+            raise ValueError(f"{name} is on cuda:{x.device}, not on cuda:{device}")
+
+
+def _like(t: torch.Tensor, out: Optional[torch.Tensor], name: str) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
+    if out.shape != t.shape:
+        raise ValueError(f"{name} must be shaped {tuple(t.shape)}")
+    return out
 
 
 class Rope:
@@ -116,7 +134,7 @@ class PagedKVCache:
                 raise ValueError(f"{name}: head_dim must be contiguous")
         if k.shape != v.shape or k.stride() != v.stride() or k.device != v.device:
             raise ValueError("k and v must have the same shape, strides and device")
-        self.k, self.v = k, v
+        self.k, self.v, self.device = k, v, k.get_device()
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         sp, sh, ss, _ = k.stride()
         # the stride of a dimension of one is never used, but has to be a legal one
@@ -151,11 +169,22 @@ class PagedBatch:
         n = kv_lens.shape[0]
         if n < 1 or q_offsets.shape[0] != n + 1 or block_table.shape[0] != n:
             raise ValueError(f"q_offsets must hold {n + 1} and block_table {n} rows for {n} sequences (at least one)")
+        self.device = kv_lens.get_device()
+        if q_offsets.get_device() != self.device or block_table.get_device() != self.device:
+            raise ValueError("q_offsets, kv_lens and block_table must be on one device")
         if max_q < 1 or (max_kv is not None and max_kv < 1):
             raise ValueError("max_q and max_kv must be >= 1")
         self.max_q, self.max_kv = max_q, max_kv
+        self._views = {}
 
     def view(self, page_size: int) -> _lib.G4qPagedBatch:
+        """The C view for a cache of this page size."""
+        v = self._views.get(page_size)
+        if v is None:
+            v = self._views[page_size] = self._view(page_size)
+        return v
+
+    def _view(self, page_size: int) -> _lib.G4qPagedBatch:
         t = self.block_table
         pages = t.shape[1]
         if self.max_kv is not None:
@@ -165,14 +194,6 @@ class PagedBatch:
                                   self.max_q)
 
 
-def _like(t: torch.Tensor, out: Optional[torch.Tensor], name: str) -> torch.Tensor:
-    if out is None:
-        return torch.empty(t.shape, dtype=torch.bfloat16, device=t.device)
-    if out.shape != t.shape:
-        raise ValueError(f"{name} must be shaped {tuple(t.shape)}")
-    return out
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rope: Rope,
                  q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, *, eps: float = 1e-6,
                  q_out: Optional[torch.Tensor] = None,
@@ -180,17 +201,18 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rope
     """``rope(rms_norm(q) * q_weight)`` and the same for k, in one launch: q [tokens, q_heads, head_dim],
     k [tokens, kv_heads, head_dim] (views of the q|k|v matmul's output qualify), ``positions`` int32 [tokens].
     fp32 inside, one rounding at the end. The outputs may be the inputs (in place)."""
-    d = rope.head_dim
-    cq, ck = _head_rows(q, d, "q"), _head_rows(k, d, "k")
-    if k.shape[0] != q.shape[0]:
+    d, dev = rope.head_dim, rope.device
+    cq, ck = _head_rows(q, d, dev, "q"), _head_rows(k, d, dev, "k")
+    n = q.shape[0]
+    if k.shape[0] != n:
         raise ValueError("q and k must have the same number of tokens")
-    _int32(positions, 1, "positions")
-    if positions.shape[0] != q.shape[0]:
-        raise ValueError("positions must hold one entry per token")
+    if positions.dtype is not torch.int32 or positions.get_device() != dev or positions.shape != (n,) or (
+            n > 1 and positions.stride(0) != 1):
+        raise ValueError(f"positions must be a contiguous int32 tensor on cuda:{dev} with one entry per token")
     q_out, k_out = _like(q, q_out, "q_out"), _like(k, k_out, "k_out")
-    _lib.call("g4q_qk_norm_rope", rope.handle, cq, ck, q.shape[0], _ptr(positions),
-              _ptr(_norm_weight(q_weight, d, q, "q_weight")), _ptr(_norm_weight(k_weight, d, q, "k_weight")), eps,
-              _head_rows(q_out, d, "q_out", True), _head_rows(k_out, d, "k_out", True), _stream())
+    _lib.call("g4q_qk_norm_rope", rope.handle, cq, ck, n, positions.data_ptr(),
+              _norm_weight(q_weight, d, dev, "q_weight"), _norm_weight(k_weight, d, dev, "k_weight"), eps,
+              _head_rows(q_out, d, dev, "q_out", True), _head_rows(k_out, d, dev, "k_out", True), _raw_stream(dev))
     return q_out, k_out
 
 
@@ -201,20 +223,23 @@ def kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cache
     pages, values normalized (without a weight; ``norm_values=False`` stores them as they are) beside them,
     and the queries, treated like the keys with ``q_weight``, returned (None for q None). One launch. ``v``
     may be ``k``. Rows that belong to no sequence are left as they were (in ``q_out`` too)."""
-    d = rope.head_dim
-    ck, cv = _head_rows(k, d, "k"), _head_rows(v, d, "v")
-    if v.shape[0] != k.shape[0] or (q is not None and q.shape[0] != k.shape[0]):
+    d, dev = rope.head_dim, rope.device
+    _same_device(dev, cache=cache, batch=batch)
+    ck = _head_rows(k, d, dev, "k")
+    cv = ck if v is k else _head_rows(v, d, dev, "v")
+    n = k.shape[0]
+    if v.shape[0] != n or (q is not None and q.shape[0] != n):
         raise ValueError("q, k and v must have the same number of tokens")
     cq = co = None
     if q is not None:
-        cq = _head_rows(q, d, "q")
+        cq = _head_rows(q, d, dev, "q")
         q_out = _like(q, q_out, "q_out")
-        co = _head_rows(q_out, d, "q_out", True)
+        co = _head_rows(q_out, d, dev, "q_out", True)
     elif q_out is not None:
         raise ValueError("q_out without q")
-    _lib.call("g4q_kv_append", rope.handle, cq, ck, cv, k.shape[0], _ptr(_norm_weight(q_weight, d, k, "q_weight")),
-              _ptr(_norm_weight(k_weight, d, k, "k_weight")), eps, 0 if norm_values else _lib.APPEND_RAW_VALUES, co,
-              cache.c, batch.view(cache.page_size), _stream())
+    _lib.call("g4q_kv_append", rope.handle, cq, ck, cv, n, _norm_weight(q_weight, d, dev, "q_weight"),
+              _norm_weight(k_weight, d, dev, "k_weight"), eps, 0 if norm_values else _lib.APPEND_RAW_VALUES, co,
+              cache.c, batch.view(cache.page_size), _raw_stream(dev))
     return q_out
 
 
@@ -242,11 +267,12 @@ class PagedAttention:
         the query at position t sees the keys j <= t, and j > t - window when window > 0. ``scale`` defaults
         to ``head_dim ** -0.5``. Single tokens, drafted blocks and prompt chunks may be mixed. A row that sees
         no key is zero; rows that belong to no sequence are left as they were (in ``out``)."""
-        cq = _head_rows(q, self.head_dim, "q")
+        d, dev = self.head_dim, self.device
+        _same_device(dev, cache=cache, batch=batch)
+        cq = _head_rows(q, d, dev, "q")
         out = _like(q, out, "out")
         _lib.call("g4q_paged_attention", self.handle, cq, q.shape[0], cache.c, batch.view(cache.page_size),
-                  self.head_dim ** -0.5 if scale is None else scale, window,
-                  _head_rows(out, self.head_dim, "out", True), _stream())
+                  d ** -0.5 if scale is None else scale, window, _head_rows(out, d, dev, "out", True), _raw_stream(dev))
         return out
 
     def free(self) -> None:

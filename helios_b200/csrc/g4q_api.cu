@@ -135,6 +135,11 @@ static void require(bool cond, G4qStatus s, const std::string& msg) {
     if (!cond) throw Error(s, msg);
 }
 
+// A literal's message is not made into a string unless it is needed (a decode step's calls are a few us).
+static void require(bool cond, G4qStatus s, const char* msg) {
+    if (!cond) throw Error(s, msg);
+}
+
 static Weight* checked(const G4qWeight* h, const char* what) {
     auto* w = reinterpret_cast<Weight*>(const_cast<G4qWeight*>(h));
     require(w != nullptr, G4Q_ERR_INVALID_ARGUMENT, std::string(what) + " requires a non-null weight handle");
@@ -970,35 +975,39 @@ G4qStatus g4q_rms_norm_residual(const uint16_t* x, int64_t ldx, const uint16_t* 
     });
 }
 
-static Rope* checked_rope(const G4qRope* h, const char* what) {
+static Rope* checked_rope(const G4qRope* h) {
     auto* r = reinterpret_cast<Rope*>(const_cast<G4qRope*>(h));
-    require(r != nullptr, G4Q_ERR_INVALID_ARGUMENT, std::string(what) + " requires a non-null rope handle");
-    require(r->magic == kRopeMagic, G4Q_ERR_INVALID_ARGUMENT, std::string(what) + " received an invalid rope handle");
-    require(r->device == current_device(), G4Q_ERR_INVALID_ARGUMENT,
-            std::string(what) + ": the current CUDA device is not the handle's device");
+    require(r != nullptr, G4Q_ERR_INVALID_ARGUMENT, "requires a non-null rope handle");
+    require(r->magic == kRopeMagic, G4Q_ERR_INVALID_ARGUMENT, "received an invalid rope handle");
+    require(r->device == current_device(), G4Q_ERR_INVALID_ARGUMENT, "the current CUDA device is not the handle's device");
     return r;
 }
 
 // One tensor of head rows: element strides in multiples of 8, 16-byte aligned data, heads that do not overlap.
 static void check_heads(const G4qHeadRows* t, int64_t head_dim, const char* name) {
-    const std::string n(name);
-    require(t != nullptr && t->data != nullptr, G4Q_ERR_INVALID_ARGUMENT, n + " must be non-null");
-    require(t->n_heads >= 1 && t->n_heads <= 65536, G4Q_ERR_INVALID_ARGUMENT, n + ".n_heads must be in [1, 65536]");
-    require(t->token_stride % 8 == 0 && t->head_stride % 8 == 0 && t->token_stride >= 0, G4Q_ERR_INVALID_ARGUMENT,
-            n + ": strides must be multiples of 8 elements");
-    require(t->n_heads == 1 || t->head_stride >= head_dim, G4Q_ERR_INVALID_ARGUMENT, n + ".head_stride must be >= head_dim");
-    require_aligned16(t->data, name);
+    const char* wrong = nullptr;
+    if (t == nullptr || t->data == nullptr)
+        wrong = " must be non-null";
+    else if (t->n_heads < 1 || t->n_heads > 65536)
+        wrong = ".n_heads must be in [1, 65536]";
+    else if (t->token_stride % 8 != 0 || t->head_stride % 8 != 0 || t->token_stride < 0)
+        wrong = ": strides must be multiples of 8 elements";
+    else if (t->n_heads > 1 && t->head_stride < head_dim)
+        wrong = ".head_stride must be >= head_dim";
+    else if ((reinterpret_cast<uintptr_t>(t->data) & 15u) != 0)
+        wrong = " must be 16-byte aligned";
+    if (wrong != nullptr) throw Error(G4Q_ERR_INVALID_ARGUMENT, std::string(name) + wrong);
 }
 
-static void check_weight(const uint16_t* w, const char* name) {
-    if (w != nullptr) require_aligned16(w, name);
+static void check_aligned(const uint16_t* w, const char* name) {
+    if ((reinterpret_cast<uintptr_t>(w) & 15u) != 0) require_aligned16(w, name);
 }
 
 // The checks that every paged call shares; fills the strides and the batch's view.
 static PagedView checked_batch(const G4qPagedCache* c, const G4qPagedBatch* b, int64_t rows) {
     require(c != nullptr && c->k != nullptr && c->v != nullptr, G4Q_ERR_INVALID_ARGUMENT, "cache: k and v must be non-null");
-    require_aligned16(c->k, "cache.k");
-    require_aligned16(c->v, "cache.v");
+    check_aligned(c->k, "cache.k");
+    check_aligned(c->v, "cache.v");
     require(c->page_size >= 16 && c->page_size <= 65536 && (c->page_size & (c->page_size - 1)) == 0, G4Q_ERR_UNSUPPORTED_CONFIG,
             "cache.page_size must be a power of two in [16, 65536]");
     require(c->n_pages >= 1 && c->n_pages < 0x7FFFFFFF, G4Q_ERR_INVALID_ARGUMENT, "cache.n_pages must be in [1, 2^31 - 1)");
@@ -1087,8 +1096,8 @@ G4qStatus g4q_rope_free(G4qRope* h) {
 static HeadRowsCall head_rows_call(const Rope& r, const G4qHeadRows* q, const G4qHeadRows* q_out, const G4qHeadRows* k,
                                    int64_t M, const uint16_t* q_weight, const uint16_t* k_weight, float eps) {
     require(eps >= 0.0f && std::isfinite(eps), G4Q_ERR_INVALID_ARGUMENT, "eps must be finite and >= 0");
-    check_weight(q_weight, "q_weight");
-    check_weight(k_weight, "k_weight");
+    check_aligned(q_weight, "q_weight");
+    check_aligned(k_weight, "k_weight");
     HeadRowsCall c = {};
     c.rows = M;
     c.rotary = r.rotary;
@@ -1114,7 +1123,7 @@ G4qStatus g4q_qk_norm_rope(const G4qRope* rope, const G4qHeadRows* q, const G4qH
                            const int32_t* positions, const uint16_t* q_weight, const uint16_t* k_weight, float eps,
                            const G4qHeadRows* q_out, const G4qHeadRows* k_out, void* stream) {
     return guarded("g4q_qk_norm_rope", [&] {
-        Rope* r = checked_rope(rope, "g4q_qk_norm_rope");
+        Rope* r = checked_rope(rope);
         require(M >= 0 && M < 0x7FFFFFFF, G4Q_ERR_INVALID_ARGUMENT, "M must be in [0, 2^31 - 1)");
         if (M == 0) return;
         require(q != nullptr || k != nullptr, G4Q_ERR_INVALID_ARGUMENT, "one of q and k must be non-null");
@@ -1135,7 +1144,7 @@ G4qStatus g4q_kv_append(const G4qRope* rope, const G4qHeadRows* q, const G4qHead
                         const uint16_t* q_weight, const uint16_t* k_weight, float eps, uint32_t flags,
                         const G4qHeadRows* q_out, const G4qPagedCache* cache, const G4qPagedBatch* batch, void* stream) {
     return guarded("g4q_kv_append", [&] {
-        Rope* r = checked_rope(rope, "g4q_kv_append");
+        Rope* r = checked_rope(rope);
         require((flags & ~G4Q_APPEND_RAW_VALUES) == 0, G4Q_ERR_INVALID_ARGUMENT, "unknown flag bits");
         const PagedView pv = checked_batch(cache, batch, M);
         require(cache->head_dim == r->head_dim, G4Q_ERR_INVALID_ARGUMENT, "the cache's head_dim is not the rope's");
@@ -1154,12 +1163,11 @@ G4qStatus g4q_kv_append(const G4qRope* rope, const G4qHeadRows* q, const G4qHead
     });
 }
 
-static Attn* checked_attn(const G4qAttn* h, const char* what) {
+static Attn* checked_attn(const G4qAttn* h) {
     auto* a = reinterpret_cast<Attn*>(const_cast<G4qAttn*>(h));
-    require(a != nullptr, G4Q_ERR_INVALID_ARGUMENT, std::string(what) + " requires a non-null attention handle");
-    require(a->magic == kAttnMagic, G4Q_ERR_INVALID_ARGUMENT, std::string(what) + " received an invalid attention handle");
-    require(a->device == current_device(), G4Q_ERR_INVALID_ARGUMENT,
-            std::string(what) + ": the current CUDA device is not the handle's device");
+    require(a != nullptr, G4Q_ERR_INVALID_ARGUMENT, "requires a non-null attention handle");
+    require(a->magic == kAttnMagic, G4Q_ERR_INVALID_ARGUMENT, "received an invalid attention handle");
+    require(a->device == current_device(), G4Q_ERR_INVALID_ARGUMENT, "the current CUDA device is not the handle's device");
     return a;
 }
 
@@ -1221,7 +1229,7 @@ G4qStatus g4q_paged_attention(const G4qAttn* attn, const G4qHeadRows* q, int64_t
                               const G4qPagedBatch* batch, float scale, int32_t window, const G4qHeadRows* out,
                               void* stream) {
     return guarded("g4q_paged_attention", [&] {
-        Attn* a = checked_attn(attn, "g4q_paged_attention");
+        Attn* a = checked_attn(attn);
         const PagedView pv = checked_batch(cache, batch, M);
         require(cache->head_dim == a->head_dim && cache->n_kv_heads == a->hk, G4Q_ERR_INVALID_ARGUMENT,
                 "the cache's head_dim and heads are not the handle's");

@@ -61,7 +61,7 @@ def test_python_layer_refuses_before_the_library():
     from helios_b200 import attention as A
     cpu = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="CUDA tensor"):
-        A._head_rows(cpu, 64, "q")
+        A._head_rows(cpu, 64, 0, "q")
     with pytest.raises(ValueError, match="4-D bfloat16 CUDA"):
         A.PagedKVCache(torch.zeros(2, 1, 16, 64, dtype=torch.bfloat16), torch.zeros(2, 1, 16, 64, dtype=torch.bfloat16))
     with pytest.raises(ValueError, match="int32 CUDA"):
