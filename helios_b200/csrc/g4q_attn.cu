@@ -25,6 +25,7 @@
 namespace g4q {
 namespace {
 
+constexpr int kFewRows = 64;         // rows per key head that this kernel takes
 constexpr int kKeys = 64;            // keys per tile
 constexpr int kComputeWarps = 8;
 constexpr int kThreads = (kComputeWarps + 1) * 32;
@@ -581,7 +582,6 @@ void launch_few(const Attn& h, const AttnCall& a, cudaStream_t st) {
 template <int D>
 void launch_few_rows(const Attn& h, const AttnCall& a, cudaStream_t st) {
     const int64_t rows = (int64_t)a.pv.max_q * (a.hq / a.hk);
-    if (rows > 64) throw Error(G4Q_ERR_UNSUPPORTED_CONFIG, "more than 64 query rows per key head");
     if (rows <= 16)
         launch_few<D, 1>(h, a, st);
     else if (rows <= 32)
@@ -597,7 +597,8 @@ size_t few_part_rows() {
 
 }  // namespace
 
-CUtensorMap paged_map(const AttnCall& a, const uint16_t* base, int D, int box) {
+namespace {
+CUtensorMap bf16_map(int rank, const uint16_t* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
     static const EncodeTiledFn encode = [] {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -607,33 +608,56 @@ CUtensorMap paged_map(const AttnCall& a, const uint16_t* base, int D, int box) {
         return reinterpret_cast<EncodeTiledFn>(p);
     }();
     if (encode == nullptr) throw Error(G4Q_ERR_RUNTIME, "cuTensorMapEncodeTiled is unavailable");
-    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)1 << a.pv.page_shift, (cuuint64_t)a.hk, (cuuint64_t)a.pv.n_pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)a.slot_stride * 2, (cuuint64_t)a.head_stride * 2, (cuuint64_t)a.page_stride * 2};
-    const cuuint32_t shape[4] = {64, (cuuint32_t)box, 1, 1}, es[4] = {1, 1, 1, 1};
+    const cuuint32_t es[4] = {1, 1, 1, 1};
     CUtensorMap m;
-    const CUresult r = encode(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<uint16_t*>(base), dims, strides, shape, es,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const CUresult r = encode(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<uint16_t*>(base), dims, strides,
+                              box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) throw Error(G4Q_ERR_RUNTIME, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
     return m;
 }
+}  // namespace
 
-size_t attn_part_rows(int head_dim) {
-    switch (head_dim) {
-        case 64: return few_part_rows<64>();
-        case 128: return few_part_rows<128>();
-        case 256: return few_part_rows<256>();
-        default: return few_part_rows<512>();
-    }
+CUtensorMap paged_map(const AttnCall& a, const uint16_t* base, int D, int box) {
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)1 << a.pv.page_shift, (cuuint64_t)a.hk, (cuuint64_t)a.pv.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)a.slot_stride * 2, (cuuint64_t)a.head_stride * 2, (cuuint64_t)a.page_stride * 2};
+    const cuuint32_t shape[4] = {64, (cuuint32_t)box, 1, 1};
+    return bf16_map(4, base, dims, strides, shape);
 }
 
-void launch_attention(const Attn& h, const AttnCall& a, cudaStream_t st) {
+CUtensorMap rows_map(const uint16_t* base, int64_t token_stride, int64_t head_stride, int heads, int rows, int D, int box_heads,
+                     int box_tokens) {
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
+    const cuuint32_t shape[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+    return bf16_map(3, base, dims, strides, shape);
+}
+
+size_t attn_part_rows(int head_dim) {
+    const size_t few = head_dim == 64 ? few_part_rows<64>() : head_dim == 128 ? few_part_rows<128>()
+                       : head_dim == 256 ? few_part_rows<256>() : few_part_rows<512>();
+    return std::max(few, chunk_part_rows());
+}
+
+void launch_few_any(const Attn& h, const AttnCall& a, cudaStream_t st) {
     switch (h.head_dim) {
         case 64: return launch_few_rows<64>(h, a, st);
         case 128: return launch_few_rows<128>(h, a, st);
         case 256: return launch_few_rows<256>(h, a, st);
         case 512: return launch_few_rows<512>(h, a, st);
     }
+}
+
+void launch_attention(const Attn& h, const AttnCall& a, cudaStream_t st) {
+    // A sequence goes by its own rows (new tokens x group): at most 64 to the kernel above, which shares the keys
+    // evenly over the SMs, more to the chunk kernel. Only the lengths on the device say which are there; where
+    // every row belongs to a sequence of max_q tokens, or there is one sequence only, the host knows.
+    const int group = a.hq / a.hk;
+    const int64_t rows = (int64_t)a.pv.max_q * group;
+    if (rows <= kFewRows) return launch_few_any(h, a, st);
+    if ((int64_t)a.pv.n_seqs * a.pv.max_q == a.pv.rows) return launch_chunk(h, a, 0, st);
+    launch_few_any(h, a, st);
+    launch_chunk(h, a, kFewRows, st);
 }
 
 }  // namespace g4q

@@ -70,7 +70,12 @@ struct AttnCall {
 };
 
 CUtensorMap paged_map(const AttnCall& a, const uint16_t* base, int head_dim, int box);   // box: slots x 64 elements
-size_t attn_part_rows(int head_dim);
+// boxes of 64 elements x box_heads heads x box_tokens tokens of head rows
+CUtensorMap rows_map(const uint16_t* base, int64_t token_stride, int64_t head_stride, int heads, int rows, int head_dim,
+                     int box_heads, int box_tokens);
+size_t attn_part_rows(int head_dim);    // rows of scratch that the two kernels' partials need at most
+size_t chunk_part_rows();
+void launch_chunk(const Attn& h, const AttnCall& a, int few_rows, cudaStream_t st);
 void launch_attention(const Attn& h, const AttnCall& a, cudaStream_t st);
 
 struct SeqGeom {

@@ -1,0 +1,587 @@
+// g4q_attn_chunk.cu -- attention of a prompt's chunk (more than 64 query rows per key head) over a paged
+// cache, on the 5th-generation tensor cores (sm_100a).
+//
+//   out = softmax(scale * q k^T + mask) v, masked to the positions j <= t (and j > t - window)
+//
+// One CTA has a tile of 128 query rows: floor(128 / group) tokens times the query heads of one key head, so
+// every K and V tile serves the whole group. It walks the 128-key tiles that the rows see, warp-specialised:
+//   warp 0      fills a ring of 32 KB stages by TMA (boxes of one page x 64 elements, SWIZZLE_128B): K tiles as
+//               [128 keys x 128 elements], V tiles as [64 keys x 256 elements], in the order they are used.
+//   warp 1      one thread issues the MMAs: S = Q K^T (both operands K-major in shared memory, M = N = 128) into
+//               one of two TMEM buffers, and O += P V (P from TMEM, V as it lies, MN-major) into up to 256 TMEM
+//               columns. S of tile j+1 is computed before P V of tile j, so the tensor cores have work while
+//               the softmax of tile j runs.
+//   warps 2-5   the softmax, one query row per thread: S from TMEM, row maximum, 2^(s - m) rounded to bf16 back
+//               over S. The maximum used, m, is only raised when a row exceeds it by more than 2^8: the weights
+//               stay below 256 (bf16 keeps its relative precision), and the output, which would have to be
+//               rescaled in TMEM, is touched in the first few tiles only. Then O / sum to global memory.
+// head_dim 512: O would take all of TMEM, so a CTA computes half of the output columns and the scores whole
+// (1.5 times the products of a single pass; a row tile of 64 would halve the tensor cores' rate instead).
+// Few tiles for many SMs (a drafted block, a small chunk over a long context): the keys of a tile are split
+// over grid.z and a join kernel adds the fp32 partials in split order.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "g4q_attn.cuh"
+#include "g4q_common.cuh"
+#include "g4q_internal.h"
+
+namespace g4q {
+namespace {
+
+constexpr int kTile = 128;             // query rows and keys of a tile
+constexpr int kThreads = 192;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRaise = 8.0f;         // how far (log2) a score may exceed the maximum in use
+constexpr uint32_t kTmemCols = 512;
+constexpr int kMaxSplits = 16;
+
+template <int D>
+struct ChunkCfg {
+    static constexpr int kDv = D < 256 ? D : 256;            // output columns of a CTA
+    static constexpr int kHalves = D / kDv;
+    static constexpr int kKCols = D < 128 ? D : 128;         // K stage: 128 keys x kKCols
+    static constexpr int kKSt = D / kKCols;                  // stages of a K tile
+    static constexpr int kVKeys = kDv == 256 ? 64 : 128;     // V stage: kVKeys x kDv
+    static constexpr int kVSt = kTile / kVKeys;
+    static constexpr int kStageBytes = kTile * kKCols * 2;
+    static constexpr int kQBytes = kTile * D * 2;
+    static constexpr int kFit = (227 * 1024 - 1024 - 256 - kQBytes) / kStageBytes;
+    static constexpr int kStages = kFit > 8 ? 8 : kFit;
+    static constexpr int kSmem = 1024 + kQBytes + kStages * kStageBytes + 256;
+    static_assert(kVKeys * kDv == kTile * kKCols && kStages >= 3, "stages hold either operand");
+};
+
+struct ChunkCall {
+    AttnCall a;
+    int group;
+    int few_rows;        // sequences of at most so many rows belong to the other kernel
+    int tokens;          // tokens of a tile: 128 / group
+    int box;
+    int splits;
+    int slots;           // tiles the grid has room for
+    float* part_o;       // [splits][slots * hk][128][D]
+    float* part_ml;      // [splits][slots * hk][128][2]
+    int* err;
+};
+
+struct TileWork {
+    SeqGeom g;
+    int t0;              // first token of the tile in its sequence
+    int lo, n;           // first key of the first key tile, and their number
+    int any_lo, any_hi;  // keys that some row of the tile sees
+};
+
+__device__ __forceinline__ int tiles_of(const ChunkCall& c, int b) {
+    const SeqGeom g = seq_geom(c.a.pv, b);
+    return g.q_len * c.group > c.few_rows ? (g.q_len + c.tokens - 1) / c.tokens : 0;
+}
+
+// The sequence and place of row tile `t` of the batch, found by one warp: {b, tile in b}, b < 0 past the end.
+// `reverse`: counted from the end of the batch.
+__device__ __forceinline__ int2 find_tile(const ChunkCall& c, int t, bool reverse, int lane) {
+    if (reverse) {
+        int total = 0;
+        for (int b = lane; b < c.a.pv.n_seqs; b += 32) total += tiles_of(c, b);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+        t = total - 1 - t;
+        if (t < 0) return make_int2(-1, 0);
+    }
+    int before = 0;
+    for (int b0 = 0; b0 < c.a.pv.n_seqs; b0 += 32) {
+        const int nt = b0 + lane < c.a.pv.n_seqs ? tiles_of(c, b0 + lane) : 0;
+        int inc = nt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        const unsigned past = __ballot_sync(0xFFFFFFFFu, before + inc > t);
+        if (past != 0) {
+            const int at = __ffs(past) - 1;
+            const int end = __shfl_sync(0xFFFFFFFFu, inc, at), n = __shfl_sync(0xFFFFFFFFu, nt, at);
+            return make_int2(b0 + at, t - (before + end - n));
+        }
+        before += __shfl_sync(0xFFFFFFFFu, inc, 31);
+    }
+    return make_int2(-1, 0);
+}
+
+__device__ __forceinline__ TileWork tile_work(const ChunkCall& c, int b, int tile) {
+    TileWork w;
+    w.g = seq_geom(c.a.pv, b);
+    w.t0 = tile * c.tokens;
+    const int last = w.g.first + min(w.t0 + c.tokens, w.g.q_len) - 1;
+    w.any_hi = min(max(last + 1, 0), w.g.kv_len);
+    w.any_lo = c.a.window > 0 ? max(0, w.g.first + w.t0 - c.a.window + 1) : 0;
+    w.lo = min(w.any_lo, w.any_hi) & ~(c.box - 1);
+    w.n = max(1, (w.any_hi - w.lo + kTile - 1) / kTile);    // rows that see nothing still become zeros
+    return w;
+}
+
+// Shared-memory descriptor of a SWIZZLE_128B operand. K-major: rows of 128 bytes, 8-row groups 1024 bytes
+// apart (lbo unused). MN-major: 64 elements of the MN dimension per 128-byte row, one row per k, 8 k's 1024
+// bytes apart, the next 64 elements lbo bytes on.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)(lbo >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+// kind::f16 instruction descriptor: D f32, A and B bf16, M = 128; b_mn: B is MN-major.
+constexpr uint32_t instr_desc(int n, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+        "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+        "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
+        : "memory");
+}
+
+// Waits for this thread's TMEM loads. The values are then passed through an empty statement, so that no use of
+// them can be moved before the wait.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t* v, int n) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < n; ++i) asm volatile("" : "+r"(v[i]));
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, int x, int head, int token, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(token), "r"(bar)
+        : "memory");
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ ChunkCall c) {
+    using C = ChunkCfg<D>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int2 found;
+    const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_addr(smem_raw));
+    const uint32_t s_q = base, s_ring = s_q + C::kQBytes, s_bar = s_ring + C::kStages * C::kStageBytes;
+    auto full = [&](int s) { return s_bar + 8u * s; };
+    auto empty = [&](int s) { return s_bar + 8u * (C::kStages + s); };
+    auto s_full = [&](int b) { return s_bar + 8u * (2 * C::kStages + b); };
+    auto p_full = [&](int b) { return s_bar + 8u * (2 * C::kStages + 2 + b); };
+    const uint32_t q_full = s_bar + 8u * (2 * C::kStages + 4);
+    auto o_done = [&](int b) { return q_full + 8u + 8u * b; };    // products of the even and the odd tiles
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (s_bar - base) + 8u * (2 * C::kStages + 7));
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int h = blockIdx.x / C::kHalves, half = blockIdx.x % C::kHalves;
+    wait_for_predecessor();
+    release_successor();
+    if (warp == 0) {
+        const int2 f = find_tile(c, blockIdx.y, true, lane);    // the longest tiles of a causal chunk start first
+        if (lane == 0) found = f;
+    } else if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                     "r"(kTmemCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else if (threadIdx.x == 64) {
+        for (int s = 0; s < C::kStages; ++s) {
+            bar_init(full(s), 1);
+            bar_init(empty(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            bar_init(s_full(b), 1);
+            bar_init(p_full(b), 4);
+            bar_init(o_done(b), 1);
+        }
+        bar_init(q_full, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t t_o = tmem, t_s = tmem + 256;     // output, two score buffers of 128 columns
+    const int2 at = found;
+
+    if (at.x >= 0) {
+        const TileWork w = tile_work(c, at.x, at.y);
+        // this split's key tiles
+        const int j0 = (int)((int64_t)w.n * blockIdx.z / c.splits), n = (int)((int64_t)w.n * (blockIdx.z + 1) / c.splits) - j0;
+        if (warp == 0) {
+            // ---------------- producer
+            if (n > 0 && lane == 0) {
+                bar_expect_tx(q_full, (uint32_t)(c.tokens * c.group) * 128u * (D / 64));
+                for (int x = 0; x < D / 64; ++x)
+                    tma_load_rows(s_q + x * (kTile * 128), &tm_q, x * 64, h * c.group, w.g.q0 + w.t0, q_full);
+            }
+            __syncwarp();
+            int stage = 0;
+            uint32_t round = 0;
+            const PagedView& pv = c.a.pv;
+            const int page_mask = (1 << pv.page_shift) - 1;
+            const uint32_t box_bytes = (uint32_t)c.box * 128u;
+            // one stage: keys [k0, k0 + keys) of columns [col0, col0 + 64 * blocks); boxes without a key that
+            // some row sees are left out
+            auto load = [&](const CUtensorMap* map, int k0, int keys, int col0, int blocks) {
+                if (round > 0) bar_wait(empty(stage), (round - 1) & 1, c.err, 80);
+                const int nb = max(0, min(keys / c.box, (w.any_hi - k0 + c.box - 1) / c.box));
+                if (lane == 0) bar_expect_tx(full(stage), (uint32_t)(nb * blocks) * box_bytes);
+                __syncwarp();
+                for (int i = lane; i < nb * blocks; i += 32) {
+                    const int box = i / blocks, cb = i % blocks, key = k0 + box * c.box;
+                    int page = pv.table[at.x * pv.table_ld + (key >> pv.page_shift)];
+                    if (page < 0 || page >= pv.n_pages) {
+                        record_input_error(pv.err, kErrPage);
+                        page = pv.n_pages;                    // outside the map: reads zeros
+                    }
+                    tma_load_page(s_ring + stage * C::kStageBytes + cb * (keys * 128) + box * box_bytes, map, col0 + cb * 64,
+                                  key & page_mask, h, page, full(stage));
+                }
+                if (++stage == C::kStages) stage = 0, ++round;
+            };
+            auto load_k = [&](int j) {
+                for (int p = 0; p < C::kKSt; ++p)
+                    load(&tm_k, w.lo + (j0 + j) * kTile, kTile, p * C::kKCols, C::kKCols / 64);
+            };
+            if (n > 0) load_k(0);
+            for (int j = 0; j < n; ++j) {
+                if (j + 1 < n) load_k(j + 1);
+                for (int p = 0; p < C::kVSt; ++p)
+                    load(&tm_v, w.lo + (j0 + j) * kTile + p * C::kVKeys, C::kVKeys, half * C::kDv, C::kDv / 64);
+            }
+        } else if (warp == 1) {
+            // ---------------- MMA issuer
+            int stage = 0;
+            uint32_t round = 0;
+            auto scores = [&](int j) {
+                for (int p = 0; p < C::kKSt; ++p) {
+                    bar_wait(full(stage), round & 1, c.err, 81);
+                    tc_fence_after();
+                    if (lane == 0) {
+#pragma unroll
+                        for (int kk = 0; kk < C::kKCols / 16; ++kk) {
+                            const uint32_t off = (kk >> 2) * (kTile * 128) + (kk & 3) * 32;
+                            mma_ss(t_s + (j & 1) * kTile, sw128_desc(s_q + p * C::kStageBytes + off, 16),
+                                   sw128_desc(s_ring + stage * C::kStageBytes + off, 16), instr_desc(kTile, false), (p | kk) != 0);
+                        }
+                        mma_commit(empty(stage));
+                    }
+                    __syncwarp();
+                    if (++stage == C::kStages) stage = 0, ++round;
+                }
+                if (lane == 0) mma_commit(s_full(j & 1));
+                __syncwarp();
+            };
+            if (n > 0) {
+                bar_wait(q_full, 0, c.err, 82);
+                scores(0);
+            }
+            for (int j = 0; j < n; ++j) {
+                if (j + 1 < n) scores(j + 1);
+                bar_wait(p_full(j & 1), (j >> 1) & 1, c.err, 83);
+                tc_fence_after();
+                for (int p = 0; p < C::kVSt; ++p) {
+                    bar_wait(full(stage), round & 1, c.err, 84);
+                    tc_fence_after();
+                    // V rows that no row of the tile sees become zeros: they hold anything, and a zero weight times
+                    // NaN is NaN
+                    const int k0 = w.lo + (j0 + j) * kTile + p * C::kVKeys;
+                    if (k0 < w.any_lo || k0 + C::kVKeys > w.any_hi) {
+                        for (int i = lane; i < C::kVKeys * (C::kDv / 8); i += 32) {
+                            const int key = k0 + (i >> 3) % C::kVKeys;
+                            if (key < w.any_lo || key >= w.any_hi)
+                                *reinterpret_cast<uint4*>(gen + (s_ring - base) + stage * C::kStageBytes + i * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+                    if (lane == 0) {
+#pragma unroll
+                        for (int kk = 0; kk < C::kVKeys / 16; ++kk)
+                            mma_ts(t_o, t_s + (j & 1) * kTile + (p * C::kVKeys + kk * 16) / 2,
+                                   sw128_desc(s_ring + stage * C::kStageBytes + kk * 2048, C::kVKeys * 128),
+                                   instr_desc(C::kDv, true), (j | p | kk) != 0);
+                        mma_commit(empty(stage));
+                    }
+                    __syncwarp();
+                    if (++stage == C::kStages) stage = 0, ++round;
+                }
+                if (lane == 0) mma_commit(o_done(j & 1));
+                __syncwarp();
+            }
+        } else {
+            // ---------------- softmax, one row per thread
+            const int quarter = warp & 3;
+            const int r = quarter * 32 + lane;
+            const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+            const int tok = r / c.group;
+            const bool mine = tok < c.tokens && w.t0 + tok < w.g.q_len;
+            int vis_lo = 0, vis_hi = 0;
+            if (mine) {
+                const int pos = w.g.first + w.t0 + tok;
+                vis_hi = min(max(pos + 1, 0), w.g.kv_len);
+                if (c.a.window > 0) vis_lo = max(0, pos - c.a.window + 1);
+            }
+            // keys that every row of the tile sees (rows beyond the sequence do not matter)
+            const int all_hi = min(max(w.g.first + w.t0 + 1, 0), w.g.kv_len);
+            const int all_lo = c.a.window > 0 ? max(0, w.g.first + min(w.t0 + c.tokens, w.g.q_len) - c.a.window) : 0;
+            const float scale2 = c.a.scale * kLog2e;
+            float m = -INFINITY, l = 0.0f;
+            for (int j = 0; j < n; ++j) {
+                const int k0 = w.lo + (j0 + j) * kTile;
+                const uint32_t ts = t_s + (j & 1) * kTile + lanes;
+                bar_wait(s_full(j & 1), (j >> 1) & 1, c.err, 85);
+                tc_fence_after();
+                uint32_t s[kTile];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, s + 32 * i);
+                tmem_wait_ld(s, kTile);
+                if (k0 < all_lo || k0 + kTile > all_hi) {
+#pragma unroll
+                    for (int i = 0; i < kTile; ++i)
+                        if (k0 + i < vis_lo || k0 + i >= vis_hi) s[i] = 0xFF800000u;   // -inf
+                }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < kTile; i += 4)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], __uint_as_float(s[i + e]));
+                const float tile_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
+                if (__any_sync(0xFFFFFFFFu, tile_max > m + kRaise)) {
+                    const float m_new = fmaxf(m, tile_max);
+                    const float f = fast_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));
+                    if (j > 0) {
+                        bar_wait(o_done((j - 1) & 1), ((j - 1) >> 1) & 1, c.err, 86);
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int x = 0; x < C::kDv; x += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(t_o + lanes + x, o);
+                            tmem_wait_ld(o, 32);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st32(t_o + lanes + x, o);
+                        }
+                    }
+                    l *= f;
+                    m = m_new;
+                }
+                const float ref = m == -INFINITY ? 0.0f : m;           // a row that has seen nothing yet
+                float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float e0 = fast_exp2(fmaf(__uint_as_float(s[64 * x + 2 * i]), scale2, -ref));
+                        const float e1 = fast_exp2(fmaf(__uint_as_float(s[64 * x + 2 * i + 1]), scale2, -ref));
+                        sum[0] += e0;
+                        sum[1] += e1;
+                        pk[i] = pack_bf16(e0, e1);
+                    }
+                    tmem_st32(ts + 32 * x, pk);
+                }
+                l += sum[0] + sum[1];
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(p_full(j & 1));
+            }
+            // ---------------- epilogue
+            if (n > 0) {
+                bar_wait(o_done((n - 1) & 1), ((n - 1) >> 1) & 1, c.err, 87);
+                tc_fence_after();
+            }
+            const int64_t token = w.g.q0 + w.t0 + tok;
+            const int hd = h * c.group + r % c.group;
+            if (c.splits == 1) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                uint16_t* dst = c.a.out + token * c.a.o_t + (int64_t)hd * c.a.o_h + half * C::kDv;
+#pragma unroll 1
+                for (int x = 0; x < C::kDv; x += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(t_o + lanes + x, o);
+                    tmem_wait_ld(o, 32);
+                    if (mine) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            uint32_t pk[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                pk[e] = pack_bf16(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
+                            *reinterpret_cast<uint4*>(dst + x + i) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                        }
+                    }
+                }
+            } else {
+                const int64_t row = (((int64_t)blockIdx.z * c.slots + blockIdx.y) * c.a.hk + h) * kTile + r;
+                if (n > 0) {
+                    float* dst = c.part_o + row * D + half * C::kDv;
+#pragma unroll 1
+                    for (int x = 0; x < C::kDv; x += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(t_o + lanes + x, o);
+                        tmem_wait_ld(o, 32);
+                        if (mine) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4)
+                                *reinterpret_cast<uint4*>(dst + x + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        }
+                    }
+                }
+                if (half == 0) *reinterpret_cast<float2*>(c.part_ml + row * 2) = make_float2(m, l);   // no tile: -inf, 0
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    }
+}
+
+// Joins the splits of every row tile: one warp per row of a tile (blockIdx.x counts 8-row groups), 128 columns
+// at a time, the partials added in split order.
+template <int D>
+__global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_constant__ ChunkCall c) {
+    constexpr int kW = D < 128 ? D : 128, kV = kW / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    wait_for_predecessor();
+    release_successor();
+    const int2 at = find_tile(c, blockIdx.y, true, lane);
+    const int r = blockIdx.x * 8 + warp, h = blockIdx.z;
+    if (at.x < 0 || r >= c.tokens * c.group) return;
+    const TileWork w = tile_work(c, at.x, at.y);
+    const int tok = r / c.group;
+    if (w.t0 + tok >= w.g.q_len) return;
+    const int64_t row0 = ((int64_t)blockIdx.y * c.a.hk + h) * kTile + r, step = (int64_t)c.slots * c.a.hk * kTile;
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (lane < c.splits) ml = *reinterpret_cast<const float2*>(c.part_ml + (row0 + lane * step) * 2);
+    float top = ml.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const float f = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
+    float total = f * ml.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+    const float mine = total == 0.0f ? 0.0f : f / total;
+    uint16_t* dst = c.a.out + (w.g.q0 + w.t0 + tok) * c.a.o_t + (int64_t)(h * c.group + r % c.group) * c.a.o_h;
+#pragma unroll 1
+    for (int x = 0; x < D; x += kW) {
+        float acc[kV];
+#pragma unroll
+        for (int e = 0; e < kV; ++e) acc[e] = 0.0f;
+        for (int z = 0; z < c.splits; ++z) {
+            const float g = __shfl_sync(0xFFFFFFFFu, mine, z);
+            if ((int64_t)w.n * (z + 1) / c.splits == (int64_t)w.n * z / c.splits) continue;   // had no keys
+            const float* src = c.part_o + (row0 + z * step) * D + x + lane * kV;
+#pragma unroll
+            for (int e = 0; e < kV; e += 2) {
+                const float2 v = *reinterpret_cast<const float2*>(src + e);
+                acc[e] += g * v.x;
+                acc[e + 1] += g * v.y;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kV; e += 2)
+            *reinterpret_cast<uint32_t*>(dst + x + lane * kV + e) = pack_bf16(acc[e], acc[e + 1]);
+    }
+}
+
+template <int D>
+void launch_chunk_dim(const Attn& hd, const AttnCall& a, int few_rows, cudaStream_t st) {
+    using C = ChunkCfg<D>;
+    static bool attr_set[64] = {false};
+    const int dev = current_device();
+    if (!attr_set[dev & 63]) {
+        check_cuda(cudaFuncSetAttribute(attn_chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
+                   "cudaFuncSetAttribute(attn_chunk)");
+        attr_set[dev & 63] = true;
+    }
+    ChunkCall c;
+    c.a = a;
+    c.group = a.hq / a.hk;
+    c.few_rows = few_rows;
+    c.tokens = kTile / c.group;
+    c.box = std::min(1 << a.pv.page_shift, 64);
+    // a sequence has at most one tile that is not full
+    const int64_t slots = std::min<int64_t>((int64_t)a.pv.rows / c.tokens + a.pv.n_seqs,
+                                            (int64_t)a.pv.n_seqs * ((a.pv.max_q + c.tokens - 1) / c.tokens));
+    if (slots > 65535) throw Error(G4Q_ERR_INVALID_ARGUMENT, "too many rows for one call");
+    c.slots = (int)slots;
+    const int64_t ctas = slots * a.hk * C::kHalves;
+    c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, device_sm_count() / ctas));
+    c.part_o = hd.part_o;
+    c.part_ml = hd.part_ml;
+    c.err = device_scratch().err;
+    const CUtensorMap tq = rows_map(a.q, a.q_t, a.q_h, a.hq, a.pv.rows, D, c.group, c.tokens);
+    const CUtensorMap tk = paged_map(a, a.k, D, c.box), tv = paged_map(a, a.v, D, c.box);
+    launch_dependent(attn_chunk_kernel<D>, dim3((unsigned)(a.hk * C::kHalves), (unsigned)slots, (unsigned)c.splits), dim3(kThreads),
+                     C::kSmem, st, tq, tk, tv, c);
+    if (c.splits > 1)
+        launch_dependent(attn_chunk_join_kernel<D>, dim3((unsigned)((c.tokens * c.group + 7) / 8), (unsigned)slots, (unsigned)a.hk),
+                         dim3(256), 0, st, c);
+}
+
+}  // namespace
+
+size_t chunk_part_rows() { return (size_t)device_sm_count() * kTile; }   // splits x tiles x key heads <= SMs
+
+void launch_chunk(const Attn& h, const AttnCall& a, int few_rows, cudaStream_t st) {
+    switch (h.head_dim) {
+        case 64: return launch_chunk_dim<64>(h, a, few_rows, st);
+        case 128: return launch_chunk_dim<128>(h, a, few_rows, st);
+        case 256: return launch_chunk_dim<256>(h, a, few_rows, st);
+        case 512: return launch_chunk_dim<512>(h, a, few_rows, st);
+    }
+}
+
+}  // namespace g4q

@@ -248,6 +248,43 @@ def test_attention_many_sequences(cuda):
     check_attention([i % 3 for i in range(n)], [max(i % 3, 5 * i % 211) for i in range(n)], 8, 4, 64, 16, 0)
 
 
+@pytest.mark.parametrize("d,hq,hk", [(64, 12, 4), (128, 8, 8), (256, 4, 2), (256, 3, 1), (512, 16, 1), (512, 2, 1)])
+@pytest.mark.parametrize("n,kv,page,window", [(128, 128, 64, 0), (130, 130, 16, 0), (200, 331, 32, 0), (65, 1000, 128, 0),
+                                              (257, 900, 16, 100), (300, 301, 64, 1), (90, 700, 256, 517)])
+def test_attention_chunk(cuda, d, hq, hk, n, kv, page, window):
+    check_attention([n], [kv], hq, hk, d, page, window)
+
+
+@pytest.mark.parametrize("d,hq,hk,window", [(256, 16, 8, 0), (512, 16, 1, 0), (128, 6, 2, 200), (64, 64, 1, 0)])
+def test_attention_mixed_batch(cuda, d, hq, hk, window):
+    """Prompts of several lengths beside single tokens and drafted blocks, an empty sequence, and padding rows."""
+    check_attention([150, 1, 0, 33, 8, 1, 200], [150, 700, 9, 33, 300, 1, 450], hq, hk, d, 16, window, before=3, behind=5)
+
+
+def test_attention_chunk_split_over_a_long_context(cuda):
+    """Few row tiles: their keys are split over CTAs, some of which have none in the short sequence."""
+    check_attention([100, 100], [2500, 101], 2, 1, 256, 64, 0)
+    check_attention([100, 100], [3000, 101], 2, 1, 512, 64, 150)
+    check_attention([16, 16], [3000, 17], 16, 1, 512, 64, 0)
+
+
+def test_attention_chunk_peaked_scores(cuda):
+    check_attention([150], [500], 16, 1, 512, 64, 0, scale=1.0)
+
+
+def test_attention_chunk_cache_orders_and_strides(cuda):
+    for order in ("shd", "layers"):
+        check_attention([140, 3], [190, 200], 8, 4, 128, 32, 0, order=order)
+    from helios_b200 import attention as A
+    s = Step([100], [150], 2, 128, 16, 21)
+    big = randn(100, 6 + 4, 128, seed=22)
+    q = big[:, :6]
+    out = torch.zeros(6, 100, 128, dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    A.PagedAttention(6, 2, 128)(q, s.cache, s.batch, out=out)
+    no_device_error()
+    close(out, *s.reference(q, 128 ** -0.5, 0))
+
+
 def test_attention_rows_that_see_nothing(cuda):
     """A sequence without keys, and one with more new tokens than keys (refused for the append, reported)."""
     from helios_b200 import _lib
@@ -259,6 +296,12 @@ def test_attention_rows_that_see_nothing(cuda):
     want, bound = s.reference(q, 128 ** -0.5, 0)
     close(out, want, bound)
     assert not out[1:5].any() and out[5].any()
+    s = Step([140, 80, 70], [60, 0, 300], 2, 128, 16, 3)      # the same for the chunk kernel
+    q = randn(290, 4, 128, seed=4)
+    out = A.PagedAttention(4, 2, 128)(q, s.cache, s.batch)
+    assert _lib.device_error() == _lib.ERR_LENS
+    close(out, *s.reference(q, 128 ** -0.5, 0))
+    assert not out[:80].any() and not out[140:220].any() and out[80].any()
 
 
 def test_attention_strided_queries_and_output(cuda):
@@ -297,6 +340,28 @@ def test_page_ids_and_lengths_outside_are_reported_and_touch_nothing(cuda):
         A.kv_append(None, k, k, s.cache, s.batch, rope)
         assert _lib.device_error() == code
         A.PagedAttention(hq, hk, d)(randn(2, hq, d, seed=3), s.cache, s.batch)
+        assert _lib.device_error() == code
+    no_device_error()
+
+
+def test_chunk_bad_pages_and_lengths(cuda):
+    from helios_b200 import _lib
+    from helios_b200 import attention as A
+    attend = A.PagedAttention(2, 1, 64)
+    q = randn(200, 2, 64, seed=3)
+    for bad in (-1, 1 << 30, 15):
+        s = Step([100, 100], [100, 120], 1, 64, 16, 2, spare=0)
+        s.t_table[1, 2] = bad
+        out = attend(q, s.cache, s.batch)
+        assert _lib.device_error() == _lib.ERR_PAGE
+        want, bound = s.reference(q, 0.125, 0)
+        close(out[:100], want[:100], bound[:100])
+    for off, kv, code in (([0, 100, 200], [100, 4000], _lib.ERR_TABLE), ([0, 150, 100], [100, 120], _lib.ERR_LENS),
+                          ([0, 100, 999], [100, 120], _lib.ERR_LENS), ([0, 100, 200], [100, -9], _lib.ERR_LENS)):
+        s = Step([100, 100], [100, 120], 1, 64, 16, 2, spare=0)
+        s.t_off.copy_(torch.tensor(off, dtype=torch.int32))
+        s.t_kv.copy_(torch.tensor(kv, dtype=torch.int32))
+        attend(q, s.cache, s.batch)
         assert _lib.device_error() == code
     no_device_error()
 
