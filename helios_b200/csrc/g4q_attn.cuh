@@ -109,7 +109,7 @@ __device__ __forceinline__ SeqGeom seq_geom(const PagedView& p, int b) {
 }
 
 // Launch as a programmatic dependent of the stream's previous kernel (the kernel waits for it itself).
-template <typename Arg, typename... Rest>
+template <int kCluster = 1, typename Arg, typename... Rest>
 void launch_dependent(void (*kernel)(Arg, Rest...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const Arg& a,
                       const Rest&... rest) {
     cudaLaunchConfig_t cfg = {};
@@ -117,11 +117,14 @@ void launch_dependent(void (*kernel)(Arg, Rest...), dim3 grid, dim3 block, size_
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = kCluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = kCluster > 1 ? 2 : 1;
     check_cuda(cudaLaunchKernelEx(&cfg, kernel, a, rest...), "attention kernel launch");
 }
 

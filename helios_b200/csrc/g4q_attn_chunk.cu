@@ -3,18 +3,23 @@
 //
 //   out = softmax(scale * q k^T + mask) v, masked to the positions j <= t (and j > t - window)
 //
-// One CTA has a tile of 128 query rows: floor(128 / group) tokens times the query heads of one key head, so
-// every K and V tile serves the whole group. It walks the 128-key tiles that the rows see, warp-specialised:
-//   warp 0      fills a ring of 32 KB stages by TMA (boxes of one page x 64 elements, SWIZZLE_128B): K tiles as
-//               [128 keys x 128 elements], V tiles as [64 keys x 256 elements], in the order they are used.
-//   warp 1      one thread issues the MMAs: S = Q K^T (both operands K-major in shared memory, M = N = 128) into
-//               one of two TMEM buffers, and O += P V (P from TMEM, V as it lies, MN-major) into up to 256 TMEM
-//               columns. S of tile j+1 is computed before P V of tile j, so the tensor cores have work while
-//               the softmax of tile j runs.
+// A tile is 256 query rows of a CTA pair (cta_group::2), 128 to a CTA: floor(128 / group) tokens times the query
+// heads of one key head, so every K and V tile serves the whole group. Each CTA fetches half of a K tile's keys
+// and half of a V tile's columns, and the pair's MMAs read both halves: on single CTAs the fetches of 128 rows' K
+// and V (64 bytes per cycle and SM at head_dim 256) outran L2 and took 3000-4000 cycles a tile. The pair walks
+// the 128-key tiles that its rows see, warp-specialised in each CTA:
+//   warp 0      fills a ring of up to 32 KB stages by TMA (boxes of one page x 64 elements, SWIZZLE_128B), K and V
+//               in the order they are used.
+//   warp 1      of the first CTA: one thread issues the MMAs: S = Q K^T (both operands K-major in shared memory,
+//               M = 256, N = 128) into one of two TMEM buffers, and O += P V (P from TMEM, V as it lies, MN-major)
+//               into up to 256 TMEM columns. S of tile j+1 is computed before P V of tile j, so the tensor cores
+//               have work while the softmax of tile j runs.
 //   warps 2-5   the softmax, one query row per thread: S from TMEM, row maximum, 2^(s - m) rounded to bf16 back
 //               over S. The maximum used, m, is only raised when a row exceeds it by more than 2^8: the weights
 //               stay below 256 (bf16 keeps its relative precision), and the output, which would have to be
 //               rescaled in TMEM, is touched in the first few tiles only. Then O / sum to global memory.
+// head_dim 64: a pair would leave each CTA 32 columns of V, less than a swizzle row, and its tiles' bytes are few
+// for the softmax they take: single CTAs (cta_group::1) run the same code.
 // head_dim 512: O would take all of TMEM, so a CTA computes half of the output columns and the scores whole
 // (1.5 times the products of a single pass; a row tile of 64 would halve the tensor cores' rate instead).
 // Few tiles for many SMs (a drafted block, a small chunk over a long context): the keys of a tile are split
@@ -39,30 +44,32 @@ constexpr int kMaxSplits = 16;
 
 template <int D>
 struct ChunkCfg {
-    static constexpr int kDv = D < 256 ? D : 256;            // output columns of a CTA
+    static constexpr int kCtas = D == 64 ? 1 : 2;            // CTAs that share a K / V tile
+    static constexpr int kDv = D < 256 ? D : 256;            // output columns computed
     static constexpr int kHalves = D / kDv;
-    static constexpr int kKCols = D < 128 ? D : 128;         // K stage: 128 keys x kKCols
+    static constexpr int kKeysHeld = kTile / kCtas;          // K stage: kKeysHeld keys x kKCols elements
+    static constexpr int kKCols = D < 256 ? D : 256;
     static constexpr int kKSt = D / kKCols;                  // stages of a K tile
-    static constexpr int kVKeys = kDv == 256 ? 64 : 128;     // V stage: kVKeys x kDv
-    static constexpr int kVSt = kTile / kVKeys;
-    static constexpr int kStageBytes = kTile * kKCols * 2;
+    static constexpr int kVCols = kDv / kCtas;               // V stage: 128 keys x kVCols elements
+    static constexpr int kStageBytes = kTile * kVCols * 2;
     static constexpr int kQBytes = kTile * D * 2;
     static constexpr int kFit = (227 * 1024 - 1024 - 256 - kQBytes) / kStageBytes;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     static constexpr int kSmem = 1024 + kQBytes + kStages * kStageBytes + 256;
-    static_assert(kVKeys * kDv == kTile * kKCols && kStages >= 3, "stages hold either operand");
+    static_assert(kKeysHeld * kKCols == kTile * kVCols && kVCols % 64 == 0 && kStages >= 3, "stages hold either operand");
 };
 
 struct ChunkCall {
     AttnCall a;
     int group;
     int few_rows;        // sequences of at most so many rows belong to the other kernel
-    int tokens;          // tokens of a tile: 128 / group
+    int tokens;          // tokens of a CTA's 128 rows: 128 / group
+    int tile_tokens;     // tokens of a tile: of all the CTAs that share it
     int box;
     int splits;
     int slots;           // tiles the grid has room for
-    float* part_o;       // [splits][slots * hk][128][D]
-    float* part_ml;      // [splits][slots * hk][128][2]
+    float* part_o;       // [splits][slots * hk][CTAs of a tile * 128][D]
+    float* part_ml;      // [splits][slots * hk][CTAs of a tile * 128][2]
     int* err;
 };
 
@@ -75,7 +82,7 @@ struct TileWork {
 
 __device__ __forceinline__ int tiles_of(const ChunkCall& c, int b) {
     const SeqGeom g = seq_geom(c.a.pv, b);
-    return g.q_len * c.group > c.few_rows ? (g.q_len + c.tokens - 1) / c.tokens : 0;
+    return g.q_len * c.group > c.few_rows ? (g.q_len + c.tile_tokens - 1) / c.tile_tokens : 0;
 }
 
 // The sequence and place of row tile `t` of the batch, found by one warp: {b, tile in b}, b < 0 past the end.
@@ -112,8 +119,8 @@ __device__ __forceinline__ int2 find_tile(const ChunkCall& c, int t, bool revers
 __device__ __forceinline__ TileWork tile_work(const ChunkCall& c, int b, int tile) {
     TileWork w;
     w.g = seq_geom(c.a.pv, b);
-    w.t0 = tile * c.tokens;
-    const int last = w.g.first + min(w.t0 + c.tokens, w.g.q_len) - 1;
+    w.t0 = tile * c.tile_tokens;
+    const int last = w.g.first + min(w.t0 + c.tile_tokens, w.g.q_len) - 1;
     w.any_hi = min(max(last + 1, 0), w.g.kv_len);
     w.any_lo = c.a.window > 0 ? max(0, w.g.first + w.t0 - c.a.window + 1) : 0;
     w.lo = min(w.any_lo, w.any_hi) & ~(c.box - 1);
@@ -134,31 +141,81 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo) {
     return d;
 }
 
-// kind::f16 instruction descriptor: D f32, A and B bf16, M = 128; b_mn: B is MN-major.
-constexpr uint32_t instr_desc(int n, bool b_mn) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+// kind::f16 instruction descriptor: D f32, A and B bf16; b_mn: B is MN-major.
+constexpr uint32_t instr_desc(int m, int n, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// D += A B with A in shared memory (mma_ss) or TMEM (mma_ts). On a CTA pair each CTA holds its 128 rows of A and
+// D, and half of B's columns.
+template <int kCtas>
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-        : "memory");
+    if constexpr (kCtas == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+            : "memory");
 }
 
+template <int kCtas>
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-        : "memory");
+    if constexpr (kCtas == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+            "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+            "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+            : "memory");
 }
 
+// Arrives on the barrier (of every CTA of the pair) when the MMAs issued so far are done.
+template <int kCtas>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    if constexpr (kCtas == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                         bar),
+                     "h"((uint16_t)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// The address of the same shared-memory object in the first CTA of the cluster.
+__device__ __forceinline__ uint32_t in_first_cta(uint32_t addr) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
+}
+
+// Arrivals on a barrier of the cluster. They order nothing beyond this CTA (a cluster-wide release costs 900
+// cycles): what they announce are TMA bytes, which the barrier counts itself, or TMEM contents, ordered by the
+// tcgen05 fences on both sides.
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void bar_expect_tx_cluster(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* v) {
@@ -194,11 +251,32 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-__device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, int x, int head, int token, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(token), "r"(bar)
-        : "memory");
+// TMA loads into this CTA's shared memory; on a pair their bytes count on the barrier of the pair's first CTA.
+template <int kCtas>
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int head, int token, uint32_t bar) {
+    if constexpr (kCtas == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(token), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(token), "r"(bar)
+            : "memory");
+}
+
+template <int kCtas>
+__device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page, uint32_t bar) {
+    if constexpr (kCtas == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+                dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(bar)
+            : "memory");
+    else
+        tma_load_page(dst, map, x, slot, head, page, bar);
 }
 
 template <int D>
@@ -206,6 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     attn_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ ChunkCall c) {
     using C = ChunkCfg<D>;
+    constexpr int kCtas = C::kCtas;
     extern __shared__ uint8_t smem_raw[];
     __shared__ int2 found;
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
@@ -220,31 +299,39 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (s_bar - base) + 8u * (2 * C::kStages + 7));
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int h = blockIdx.x / C::kHalves, half = blockIdx.x % C::kHalves;
+    const int rank = blockIdx.x % kCtas;                 // place in the pair (clusters run along x)
+    const int half = blockIdx.x / kCtas % C::kHalves, h = blockIdx.x / (kCtas * C::kHalves);
     wait_for_predecessor();
     release_successor();
     if (warp == 0) {
         const int2 f = find_tile(c, blockIdx.y, true, lane);    // the longest tiles of a causal chunk start first
         if (lane == 0) found = f;
     } else if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
-                     "r"(kTmemCols));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        if constexpr (kCtas == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                         "r"(kTmemCols));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                         "r"(kTmemCols));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
     } else if (threadIdx.x == 64) {
         for (int s = 0; s < C::kStages; ++s) {
-            bar_init(full(s), 1);
+            bar_init(full(s), kCtas);             // one arrival of each producer, with its bytes
             bar_init(empty(s), 1);
         }
         for (int b = 0; b < 2; ++b) {
             bar_init(s_full(b), 1);
-            bar_init(p_full(b), 4);
+            bar_init(p_full(b), 4 * kCtas);       // every softmax warp of the pair
             bar_init(o_done(b), 1);
         }
-        bar_init(q_full, 1);
+        bar_init(q_full, kCtas);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (kCtas == 2) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const uint32_t t_o = tmem, t_s = tmem + 256;     // output, two score buffers of 128 columns
@@ -252,14 +339,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (at.x >= 0) {
         const TileWork w = tile_work(c, at.x, at.y);
+        const int t0 = w.t0 + rank * c.tokens;       // this CTA's first token
         // this split's key tiles
         const int j0 = (int)((int64_t)w.n * blockIdx.z / c.splits), n = (int)((int64_t)w.n * (blockIdx.z + 1) / c.splits) - j0;
         if (warp == 0) {
             // ---------------- producer
             if (n > 0 && lane == 0) {
-                bar_expect_tx(q_full, (uint32_t)(c.tokens * c.group) * 128u * (D / 64));
+                const uint32_t qb = in_first_cta(q_full);
+                bar_expect_tx_cluster(qb, (uint32_t)(c.tokens * c.group) * 128u * (D / 64));
                 for (int x = 0; x < D / 64; ++x)
-                    tma_load_rows(s_q + x * (kTile * 128), &tm_q, x * 64, h * c.group, w.g.q0 + w.t0, q_full);
+                    tma_rows<kCtas>(s_q + x * (kTile * 128), &tm_q, x * 64, h * c.group, w.g.q0 + t0, qb);
             }
             __syncwarp();
             int stage = 0;
@@ -267,94 +356,139 @@ __global__ void __launch_bounds__(kThreads, 1)
             const PagedView& pv = c.a.pv;
             const int page_mask = (1 << pv.page_shift) - 1;
             const uint32_t box_bytes = (uint32_t)c.box * 128u;
-            // one stage: keys [k0, k0 + keys) of columns [col0, col0 + 64 * blocks); boxes without a key that
-            // some row sees are left out
-            auto load = [&](const CUtensorMap* map, int k0, int keys, int col0, int blocks) {
-                if (round > 0) bar_wait(empty(stage), (round - 1) & 1, c.err, 80);
-                const int nb = max(0, min(keys / c.box, (w.any_hi - k0 + c.box - 1) / c.box));
-                if (lane == 0) bar_expect_tx(full(stage), (uint32_t)(nb * blocks) * box_bytes);
-                __syncwarp();
-                for (int i = lane; i < nb * blocks; i += 32) {
-                    const int box = i / blocks, cb = i % blocks, key = k0 + box * c.box;
-                    int page = pv.table[at.x * pv.table_ld + (key >> pv.page_shift)];
+            const int boxes = kTile / c.box;             // of a tile of keys; box i is lane i's
+            // The page of this lane's box of tile j, looked up two tiles ahead of its use (the look-up takes as long
+            // as half a tile's products).
+            auto look_up = [&](int j) {
+                const int key = w.lo + (j0 + j) * kTile + lane * c.box;
+                int page = pv.n_pages;                    // outside the map: reads zeros
+                if (j < n && lane < boxes && key < w.any_hi) {
+                    page = pv.table[at.x * pv.table_ld + (key >> pv.page_shift)];
                     if (page < 0 || page >= pv.n_pages) {
                         record_input_error(pv.err, kErrPage);
-                        page = pv.n_pages;                    // outside the map: reads zeros
+                        page = pv.n_pages;
                     }
-                    tma_load_page(s_ring + stage * C::kStageBytes + cb * (keys * 128) + box * box_bytes, map, col0 + cb * 64,
-                                  key & page_mask, h, page, full(stage));
+                }
+                return page;
+            };
+            // boxes [b0, b1) of the stage's keys k0.. (`keys` of them, the first one box `first` of its tile) by TMA,
+            // columns [col0, col0 + 64 * blocks)
+            auto fill = [&](const CUtensorMap* map, int pages, int k0, int keys, int first, int b0, int b1, int col0, int blocks) {
+                const uint32_t bar = in_first_cta(full(stage));
+                if (lane == 0) bar_expect_tx_cluster(bar, (uint32_t)((b1 - b0) * blocks) * box_bytes);
+                __syncwarp();
+                for (int i0 = 0; i0 < (b1 - b0) * blocks; i0 += 32) {
+                    const int i = i0 + lane, box = b0 + i / blocks, cb = i % blocks;
+                    const int page = __shfl_sync(0xFFFFFFFFu, pages, (first + box) & 31);
+                    if (i < (b1 - b0) * blocks)
+                        tma_page<kCtas>(s_ring + stage * C::kStageBytes + cb * (keys * 128) + box * box_bytes, map, col0 + cb * 64,
+                                        (k0 + box * c.box) & page_mask, h, page, bar);
                 }
                 if (++stage == C::kStages) stage = 0, ++round;
             };
-            auto load_k = [&](int j) {
-                for (int p = 0; p < C::kKSt; ++p)
-                    load(&tm_k, w.lo + (j0 + j) * kTile, kTile, p * C::kKCols, C::kKCols / 64);
+            auto load_k = [&](int j, int pages) {
+                const int k0 = w.lo + (j0 + j) * kTile + rank * C::kKeysHeld;
+                // a box without a key that some row sees is left out: its scores are masked
+                const int nb = max(0, min(C::kKeysHeld / c.box, (w.any_hi - k0 + c.box - 1) / c.box));
+                for (int p = 0; p < C::kKSt; ++p) {
+                    if (round > 0) bar_wait(empty(stage), (round - 1) & 1, c.err, 80);
+                    fill(&tm_k, pages, k0, C::kKeysHeld, rank * C::kKeysHeld / c.box, 0, nb, p * C::kKCols, C::kKCols / 64);
+                }
             };
-            if (n > 0) load_k(0);
+            auto load_v = [&](int j, int pages) {
+                const int k0 = w.lo + (j0 + j) * kTile, col0 = half * C::kDv + rank * C::kVCols;
+                if (round > 0) bar_wait(empty(stage), (round - 1) & 1, c.err, 80);
+                // Keys that no row of the tile sees hold anything, and a zero weight times NaN is NaN: only boxes of
+                // seen keys come by TMA, the others row by row, with zeros for the keys that are not seen.
+                const int b1 = min(kTile, max(0, w.any_hi - k0)) / c.box;
+                const int b0 = min(b1, max(0, (w.any_lo - k0 + c.box - 1) / c.box));
+                if (b1 - b0 < boxes) {
+                    const int head = b0 * c.box, tail = b1 * c.box;      // rows [0, head) and [tail, 128) by hand
+                    const int rows = head + kTile - tail;
+                    constexpr int kChunks = C::kVCols / 8, kBatch = 8;   // loads in flight per lane
+                    for (int i0 = 0; i0 < rows * kChunks; i0 += 32 * kBatch) {
+                        uint4 v[kBatch];
+#pragma unroll
+                        for (int u = 0; u < kBatch; ++u) {
+                            const int i = i0 + u * 32 + lane, ch = i % kChunks;
+                            int row = min(i / kChunks, rows - 1);
+                            if (row >= head) row += tail - head;
+                            const int key = k0 + row;
+                            const int page = __shfl_sync(0xFFFFFFFFu, pages, row / c.box);
+                            v[u] = make_uint4(0, 0, 0, 0);
+                            if (key >= w.any_lo && key < w.any_hi && page < pv.n_pages)
+                                v[u] = *reinterpret_cast<const uint4*>(c.a.v + page * c.a.page_stride + h * c.a.head_stride +
+                                                                       (key & ((1 << pv.page_shift) - 1)) * c.a.slot_stride + col0 + ch * 8);
+                        }
+#pragma unroll
+                        for (int u = 0; u < kBatch; ++u) {
+                            const int i = i0 + u * 32 + lane, ch = i % kChunks;
+                            int row = i / kChunks;
+                            if (row >= rows) continue;
+                            if (row >= head) row += tail - head;
+                            *reinterpret_cast<uint4*>(gen + (s_ring - base) + stage * C::kStageBytes + (ch >> 3) * (kTile * 128) +
+                                                      row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = v[u];
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;\n\tfence.acq_rel.cluster;" ::: "memory");
+                    __syncwarp();
+                }
+                fill(&tm_v, pages, k0, kTile, 0, b0, b1, col0, C::kVCols / 64);
+            };
+            int pages = look_up(0), pages1 = look_up(1);
+            if (n > 0) load_k(0, pages);
             for (int j = 0; j < n; ++j) {
-                if (j + 1 < n) load_k(j + 1);
-                for (int p = 0; p < C::kVSt; ++p)
-                    load(&tm_v, w.lo + (j0 + j) * kTile + p * C::kVKeys, C::kVKeys, half * C::kDv, C::kDv / 64);
+                const int pages2 = look_up(j + 2);
+                if (j + 1 < n) load_k(j + 1, pages1);
+                load_v(j, pages);
+                pages = pages1;
+                pages1 = pages2;
             }
         } else if (warp == 1) {
-            // ---------------- MMA issuer
-            int stage = 0;
-            uint32_t round = 0;
-            auto scores = [&](int j) {
-                for (int p = 0; p < C::kKSt; ++p) {
-                    bar_wait(full(stage), round & 1, c.err, 81);
-                    tc_fence_after();
-                    if (lane == 0) {
+            // ---------------- MMA issuer (of the pair's first CTA)
+            if (rank == 0) {
+                int stage = 0;
+                uint32_t round = 0;
+                auto scores = [&](int j) {
+                    for (int p = 0; p < C::kKSt; ++p) {
+                        bar_wait(full(stage), round & 1, c.err, 81);
+                        tc_fence_after();
+                        if (lane == 0) {
 #pragma unroll
-                        for (int kk = 0; kk < C::kKCols / 16; ++kk) {
-                            const uint32_t off = (kk >> 2) * (kTile * 128) + (kk & 3) * 32;
-                            mma_ss(t_s + (j & 1) * kTile, sw128_desc(s_q + p * C::kStageBytes + off, 16),
-                                   sw128_desc(s_ring + stage * C::kStageBytes + off, 16), instr_desc(kTile, false), (p | kk) != 0);
+                            for (int kk = 0; kk < C::kKCols / 16; ++kk)
+                                mma_ss<kCtas>(t_s + (j & 1) * kTile,
+                                              sw128_desc(s_q + (p * (C::kKCols / 64) + (kk >> 2)) * (kTile * 128) + (kk & 3) * 32, 16),
+                                              sw128_desc(s_ring + stage * C::kStageBytes + (kk >> 2) * (C::kKeysHeld * 128) + (kk & 3) * 32, 16),
+                                              instr_desc(kTile * kCtas, kTile, false), (p | kk) != 0);
+                            mma_commit<kCtas>(empty(stage));
                         }
-                        mma_commit(empty(stage));
+                        __syncwarp();
+                        if (++stage == C::kStages) stage = 0, ++round;
                     }
+                    if (lane == 0) mma_commit<kCtas>(s_full(j & 1));
                     __syncwarp();
-                    if (++stage == C::kStages) stage = 0, ++round;
+                };
+                if (n > 0) {
+                    bar_wait(q_full, 0, c.err, 82);
+                    scores(0);
                 }
-                if (lane == 0) mma_commit(s_full(j & 1));
-                __syncwarp();
-            };
-            if (n > 0) {
-                bar_wait(q_full, 0, c.err, 82);
-                scores(0);
-            }
-            for (int j = 0; j < n; ++j) {
-                if (j + 1 < n) scores(j + 1);
-                bar_wait(p_full(j & 1), (j >> 1) & 1, c.err, 83);
-                tc_fence_after();
-                for (int p = 0; p < C::kVSt; ++p) {
+                for (int j = 0; j < n; ++j) {
+                    if (j + 1 < n) scores(j + 1);
+                    bar_wait(p_full(j & 1), (j >> 1) & 1, c.err, 83);
                     bar_wait(full(stage), round & 1, c.err, 84);
                     tc_fence_after();
-                    // V rows that no row of the tile sees become zeros: they hold anything, and a zero weight times
-                    // NaN is NaN
-                    const int k0 = w.lo + (j0 + j) * kTile + p * C::kVKeys;
-                    if (k0 < w.any_lo || k0 + C::kVKeys > w.any_hi) {
-                        for (int i = lane; i < C::kVKeys * (C::kDv / 8); i += 32) {
-                            const int key = k0 + (i >> 3) % C::kVKeys;
-                            if (key < w.any_lo || key >= w.any_hi)
-                                *reinterpret_cast<uint4*>(gen + (s_ring - base) + stage * C::kStageBytes + i * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                    }
                     if (lane == 0) {
 #pragma unroll
-                        for (int kk = 0; kk < C::kVKeys / 16; ++kk)
-                            mma_ts(t_o, t_s + (j & 1) * kTile + (p * C::kVKeys + kk * 16) / 2,
-                                   sw128_desc(s_ring + stage * C::kStageBytes + kk * 2048, C::kVKeys * 128),
-                                   instr_desc(C::kDv, true), (j | p | kk) != 0);
-                        mma_commit(empty(stage));
+                        for (int kk = 0; kk < kTile / 16; ++kk)
+                            mma_ts<kCtas>(t_o, t_s + (j & 1) * kTile + kk * 8,
+                                          sw128_desc(s_ring + stage * C::kStageBytes + kk * 2048, kTile * 128),
+                                          instr_desc(kTile * kCtas, C::kDv, true), (j | kk) != 0);
+                        mma_commit<kCtas>(empty(stage));
+                        mma_commit<kCtas>(o_done(j & 1));
                     }
                     __syncwarp();
                     if (++stage == C::kStages) stage = 0, ++round;
                 }
-                if (lane == 0) mma_commit(o_done(j & 1));
-                __syncwarp();
             }
         } else {
             // ---------------- softmax, one row per thread
@@ -362,16 +496,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int r = quarter * 32 + lane;
             const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
             const int tok = r / c.group;
-            const bool mine = tok < c.tokens && w.t0 + tok < w.g.q_len;
+            const bool mine = tok < c.tokens && t0 + tok < w.g.q_len;
             int vis_lo = 0, vis_hi = 0;
             if (mine) {
-                const int pos = w.g.first + w.t0 + tok;
+                const int pos = w.g.first + t0 + tok;
                 vis_hi = min(max(pos + 1, 0), w.g.kv_len);
                 if (c.a.window > 0) vis_lo = max(0, pos - c.a.window + 1);
             }
-            // keys that every row of the tile sees (rows beyond the sequence do not matter)
-            const int all_hi = min(max(w.g.first + w.t0 + 1, 0), w.g.kv_len);
-            const int all_lo = c.a.window > 0 ? max(0, w.g.first + min(w.t0 + c.tokens, w.g.q_len) - c.a.window) : 0;
+            // keys that every row of this CTA sees (rows beyond the sequence do not matter)
+            const int all_hi = min(max(w.g.first + t0 + 1, 0), w.g.kv_len);
+            const int all_lo = c.a.window > 0 ? max(0, w.g.first + min(t0 + c.tokens, w.g.q_len) - c.a.window) : 0;
             const float scale2 = c.a.scale * kLog2e;
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < n; ++j) {
@@ -432,14 +566,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive(p_full(j & 1));
+                if (lane == 0) bar_arrive_cluster(in_first_cta(p_full(j & 1)));
             }
             // ---------------- epilogue
             if (n > 0) {
                 bar_wait(o_done((n - 1) & 1), ((n - 1) >> 1) & 1, c.err, 87);
                 tc_fence_after();
             }
-            const int64_t token = w.g.q0 + w.t0 + tok;
+            const int64_t token = w.g.q0 + t0 + tok;
             const int hd = h * c.group + r % c.group;
             if (c.splits == 1) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -461,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             } else {
-                const int64_t row = (((int64_t)blockIdx.z * c.slots + blockIdx.y) * c.a.hk + h) * kTile + r;
+                const int64_t row = ((((int64_t)blockIdx.z * c.slots + blockIdx.y) * c.a.hk + h) * kCtas + rank) * kTile + r;
                 if (n > 0) {
                     float* dst = c.part_o + row * D + half * C::kDv;
 #pragma unroll 1
@@ -480,15 +614,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     }
+    // The pair's MMAs read both CTAs' shared memory and signal both: neither leaves before the other is done.
     tc_fence_before();
     __syncthreads();
+    if constexpr (kCtas == 2) cluster_sync();
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+        if constexpr (kCtas == 2)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
     }
 }
 
-// Joins the splits of every row tile: one warp per row of a tile (blockIdx.x counts 8-row groups), 128 columns
+// Joins the splits of every row tile: one warp per row of a tile, 128 columns
 // at a time, the partials added in split order.
 template <int D>
 __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_constant__ ChunkCall c) {
@@ -497,12 +636,13 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_const
     wait_for_predecessor();
     release_successor();
     const int2 at = find_tile(c, blockIdx.y, true, lane);
-    const int r = blockIdx.x * 8 + warp, h = blockIdx.z;
+    constexpr int kRows = ChunkCfg<D>::kCtas * kTile;
+    const int row = blockIdx.x * 8 + warp, r = row % kTile, h = blockIdx.z;
     if (at.x < 0 || r >= c.tokens * c.group) return;
     const TileWork w = tile_work(c, at.x, at.y);
-    const int tok = r / c.group;
+    const int tok = row / kTile * c.tokens + r / c.group;
     if (w.t0 + tok >= w.g.q_len) return;
-    const int64_t row0 = ((int64_t)blockIdx.y * c.a.hk + h) * kTile + r, step = (int64_t)c.slots * c.a.hk * kTile;
+    const int64_t row0 = ((int64_t)blockIdx.y * c.a.hk + h) * kRows + row, step = (int64_t)c.slots * c.a.hk * kRows;
     float2 ml = make_float2(-INFINITY, 0.0f);
     if (lane < c.splits) ml = *reinterpret_cast<const float2*>(c.part_ml + (row0 + lane * step) * 2);
     float top = ml.x;
@@ -551,29 +691,30 @@ void launch_chunk_dim(const Attn& hd, const AttnCall& a, int few_rows, cudaStrea
     c.group = a.hq / a.hk;
     c.few_rows = few_rows;
     c.tokens = kTile / c.group;
+    c.tile_tokens = c.tokens * C::kCtas;
     c.box = std::min(1 << a.pv.page_shift, 64);
     // a sequence has at most one tile that is not full
-    const int64_t slots = std::min<int64_t>((int64_t)a.pv.rows / c.tokens + a.pv.n_seqs,
-                                            (int64_t)a.pv.n_seqs * ((a.pv.max_q + c.tokens - 1) / c.tokens));
+    const int64_t slots = std::min<int64_t>((int64_t)a.pv.rows / c.tile_tokens + a.pv.n_seqs,
+                                            (int64_t)a.pv.n_seqs * ((a.pv.max_q + c.tile_tokens - 1) / c.tile_tokens));
     if (slots > 65535) throw Error(G4Q_ERR_INVALID_ARGUMENT, "too many rows for one call");
     c.slots = (int)slots;
-    const int64_t ctas = slots * a.hk * C::kHalves;
+    const int64_t ctas = slots * a.hk * C::kHalves * C::kCtas;
     c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, device_sm_count() / ctas));
     c.part_o = hd.part_o;
     c.part_ml = hd.part_ml;
     c.err = device_scratch().err;
     const CUtensorMap tq = rows_map(a.q, a.q_t, a.q_h, a.hq, a.pv.rows, D, c.group, c.tokens);
     const CUtensorMap tk = paged_map(a, a.k, D, c.box), tv = paged_map(a, a.v, D, c.box);
-    launch_dependent(attn_chunk_kernel<D>, dim3((unsigned)(a.hk * C::kHalves), (unsigned)slots, (unsigned)c.splits), dim3(kThreads),
-                     C::kSmem, st, tq, tk, tv, c);
+    launch_dependent<C::kCtas>(attn_chunk_kernel<D>,
+                               dim3((unsigned)(a.hk * C::kHalves * C::kCtas), (unsigned)slots, (unsigned)c.splits), dim3(kThreads),
+                               C::kSmem, st, tq, tk, tv, c);
     if (c.splits > 1)
-        launch_dependent(attn_chunk_join_kernel<D>, dim3((unsigned)((c.tokens * c.group + 7) / 8), (unsigned)slots, (unsigned)a.hk),
-                         dim3(256), 0, st, c);
+        launch_dependent(attn_chunk_join_kernel<D>, dim3(C::kCtas * kTile / 8, (unsigned)slots, (unsigned)a.hk), dim3(256), 0, st, c);
 }
 
 }  // namespace
 
-size_t chunk_part_rows() { return (size_t)device_sm_count() * kTile; }   // splits x tiles x key heads <= SMs
+size_t chunk_part_rows() { return (size_t)device_sm_count() * kTile; }   // split launches have at most one CTA per SM
 
 void launch_chunk(const Attn& h, const AttnCall& a, int few_rows, cudaStream_t st) {
     switch (h.head_dim) {
