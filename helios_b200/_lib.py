@@ -203,7 +203,7 @@ def last_error() -> str:
 
 def call(name: str, *args) -> None:
     """Call a g4q entry point and raise G4qError on a non-OK status."""
-    status = getattr(load(), name)(*args)
+    status = getattr(_lib or load(), name)(*args)
     if status != G4Q_OK:
         msg = last_error()
         cls = G4qInvalidArgument if status == G4Q_ERR_INVALID_ARGUMENT else G4qError

@@ -28,6 +28,7 @@ __all__ = ["Rope", "PagedKVCache", "PagedBatch", "PagedAttention", "qk_norm_rope
 
 _BF16 = torch.bfloat16
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_HeadRows = _lib.G4qHeadRows
 
 
 def _head_rows(t: torch.Tensor, head_dim: int, device: int, name: str, out: bool = False) -> _lib.G4qHeadRows:
@@ -46,7 +47,7 @@ def _head_rows(t: torch.Tensor, head_dim: int, device: int, name: str, out: bool
         sh = max(sh, head_dim)
     if out and (sh < head_dim or (shape[0] > 1 and st < head_dim)):
         raise ValueError(f"{name}: its rows overlap")
-    return _lib.G4qHeadRows(data, st, sh, shape[1])
+    return _HeadRows(data, st, sh, shape[1])
 
 
 def _norm_weight(w: Optional[torch.Tensor], head_dim: int, device: int, name: str) -> Optional[int]:
@@ -69,12 +70,14 @@ def _same_device(device: int, **what) -> None:
             raise ValueError(f"{name} is on cuda:{x.device}, not on cuda:{device}")
 
 
-def _like(t: torch.Tensor, out: Optional[torch.Tensor], name: str) -> torch.Tensor:
+def _output(t: torch.Tensor, heads: int, head_dim: int, device: int, out: Optional[torch.Tensor], name: str):
+    """The output tensor for t's shape (a new contiguous one for None) and its C view."""
     if out is None:
-        return torch.empty_like(t, memory_format=torch.contiguous_format)
+        out = torch.empty_like(t, memory_format=torch.contiguous_format)
+        return out, _HeadRows(out.data_ptr(), heads * head_dim, head_dim, heads)
     if out.shape != t.shape:
         raise ValueError(f"{name} must be shaped {tuple(t.shape)}")
-    return out
+    return out, _head_rows(out, head_dim, device, name, True)
 
 
 class Rope:
@@ -209,10 +212,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rope
     if positions.dtype is not torch.int32 or positions.get_device() != dev or positions.shape != (n,) or (
             n > 1 and positions.stride(0) != 1):
         raise ValueError(f"positions must be a contiguous int32 tensor on cuda:{dev} with one entry per token")
-    q_out, k_out = _like(q, q_out, "q_out"), _like(k, k_out, "k_out")
+    q_out, co = _output(q, cq.n_heads, d, dev, q_out, "q_out")
+    k_out, cko = _output(k, ck.n_heads, d, dev, k_out, "k_out")
     _lib.call("g4q_qk_norm_rope", rope.handle, cq, ck, n, positions.data_ptr(),
-              _norm_weight(q_weight, d, dev, "q_weight"), _norm_weight(k_weight, d, dev, "k_weight"), eps,
-              _head_rows(q_out, d, dev, "q_out", True), _head_rows(k_out, d, dev, "k_out", True), _raw_stream(dev))
+              _norm_weight(q_weight, d, dev, "q_weight"), _norm_weight(k_weight, d, dev, "k_weight"), eps, co, cko,
+              _raw_stream(dev))
     return q_out, k_out
 
 
@@ -233,8 +237,7 @@ def kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cache
     cq = co = None
     if q is not None:
         cq = _head_rows(q, d, dev, "q")
-        q_out = _like(q, q_out, "q_out")
-        co = _head_rows(q_out, d, dev, "q_out", True)
+        q_out, co = _output(q, cq.n_heads, d, dev, q_out, "q_out")
     elif q_out is not None:
         raise ValueError("q_out without q")
     _lib.call("g4q_kv_append", rope.handle, cq, ck, cv, n, _norm_weight(q_weight, d, dev, "q_weight"),
@@ -270,9 +273,9 @@ class PagedAttention:
         d, dev = self.head_dim, self.device
         _same_device(dev, cache=cache, batch=batch)
         cq = _head_rows(q, d, dev, "q")
-        out = _like(q, out, "out")
+        out, co = _output(q, cq.n_heads, d, dev, out, "out")
         _lib.call("g4q_paged_attention", self.handle, cq, q.shape[0], cache.c, batch.view(cache.page_size),
-                  d ** -0.5 if scale is None else scale, window, _head_rows(out, d, dev, "out", True), _raw_stream(dev))
+                  d ** -0.5 if scale is None else scale, window, co, _raw_stream(dev))
         return out
 
     def free(self) -> None:

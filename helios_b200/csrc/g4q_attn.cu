@@ -7,8 +7,10 @@
 // The work is a list of (sequence, key head, 64-key tile), cut into equal contiguous ranges of tiles, one per
 // CTA: every SM streams the same number of bytes whatever the lengths are, and the TMA ring runs on from one
 // sequence to the next without a pause. A range that ends inside a sequence leaves its fp32 partial
-// (unnormalized output, running maximum and sum per row) in the handle's scratch, at most two per CTA, and the
-// combine kernel joins a sequence's partials in CTA order, so results do not depend on timing.
+// (unnormalized output, running maximum and sum per row) in the handle's scratch, at most two per CTA, and a
+// second kernel, launched while the first one drains, joins a sequence's partials in CTA order, so results do not
+// depend on timing. (Having the CTA that comes last join them instead was slower: one token over a window of 1024,
+// 10.4 us against 8.8; the last CTA waits for its stores, its ticket and the others' partials one after another.)
 //
 // In a CTA one warp feeds the ring (SWIZZLE_128B boxes of one page x 64 elements) and eight compute warps
 // share each tile: for the scores, warp w takes keys 8w..8w+7 against all query rows (mma.sync, rows padded
@@ -80,17 +82,24 @@ __device__ __forceinline__ SeqWork seq_work(const FewCall& c, int b) {
     return w;
 }
 
-__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    return v;
-}
+// The list of tiles cut into equal contiguous ranges: the first `more` CTAs have base + 1 tiles, the others base.
+struct Ranges {
+    uint32_t base, more;
+    __device__ __forceinline__ Ranges(uint32_t total, int ctas) : base(total / ctas), more(total % ctas) {}
+    __device__ __forceinline__ uint32_t first(uint32_t cta) const { return cta * base + min(cta, more); }
+    __device__ __forceinline__ uint32_t owner(uint32_t tile) const {
+        const uint32_t cut = more * (base + 1);
+        return tile < cut ? tile / (base + 1) : more + (tile - cut) / base;
+    }
+};
 
-// Tiles of sequences [0, end), summed by one warp.
-__device__ __forceinline__ int64_t tiles_before(const FewCall& c, int end, int lane) {
-    int64_t t = 0;
-    for (int b = lane; b < end; b += 32) t += seq_work(c, b).nt;
-    return warp_sum64(t) * c.a.hk;
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v, int lane) {   // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xFFFFFFFFu, v, o);
+        if (lane >= o) v += t;
+    }
+    return v;
 }
 
 // A position in the list of tiles.
@@ -126,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
                     const __grid_constant__ FewCall c) {
     using C = FewCfg<D, MT>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ int start[4];                 // b, h, t and the number of tiles of this CTA
+    __shared__ int start[4];                 // b, h, t of this CTA's first tile, and its tiles
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_addr(smem_raw));
     const uint32_t s_ring = base;
@@ -144,27 +153,27 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
     wait_for_predecessor();
     release_successor();
     if (warp == kComputeWarps) {
-        // this CTA's range of tiles and the place of its first one
-        const int64_t total = tiles_before(c, c.a.pv.n_seqs, lane);
-        const int64_t t0 = total * blockIdx.x / c.ctas, t1 = total * (blockIdx.x + 1) / c.ctas;
-        int64_t before = 0;
-        int found = -1;
-        int64_t rest = 0;
-        for (int b0 = 0; b0 < c.a.pv.n_seqs && found < 0 && t1 > t0; b0 += 32) {
+        // this CTA's range of tiles and the place of its first one; the first 32 sequences stay in registers
+        const int nt0 = lane < c.a.pv.n_seqs ? seq_work(c, lane).nt : 0;
+        const uint32_t scan0 = warp_scan(nt0 * c.a.hk, lane);
+        uint32_t total = __shfl_sync(0xFFFFFFFFu, scan0, 31);
+        for (int b0 = 32; b0 < c.a.pv.n_seqs; b0 += 32) {
             const int nt = b0 + lane < c.a.pv.n_seqs ? seq_work(c, b0 + lane).nt : 0;
-            int64_t inc = (int64_t)nt * c.a.hk;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-                if (lane >= o) inc += v;
-            }
+            total += __shfl_sync(0xFFFFFFFFu, warp_scan(nt * c.a.hk, lane), 31);
+        }
+        const Ranges ranges(total, c.ctas);
+        const uint32_t t0 = ranges.first(blockIdx.x), t1 = ranges.first(blockIdx.x + 1);
+        uint32_t before = 0;
+        int found = -1;
+        for (int b0 = 0; b0 < c.a.pv.n_seqs && found < 0 && t1 > t0; b0 += 32) {
+            const int nt = b0 == 0 ? nt0 : b0 + lane < c.a.pv.n_seqs ? seq_work(c, b0 + lane).nt : 0;
+            const uint32_t inc = b0 == 0 ? scan0 : warp_scan(nt * c.a.hk, lane);
             const unsigned past = __ballot_sync(0xFFFFFFFFu, before + inc > t0);
             if (past != 0) {
                 const int at = __ffs(past) - 1;
-                const int64_t end = __shfl_sync(0xFFFFFFFFu, inc, at);
-                const int n = __shfl_sync(0xFFFFFFFFu, nt, at);
+                const uint32_t end = __shfl_sync(0xFFFFFFFFu, inc, at), n = __shfl_sync(0xFFFFFFFFu, nt, at);
                 found = b0 + at;
-                rest = t0 - (before + end - (int64_t)n * c.a.hk);
+                const uint32_t rest = t0 - (before + end - n * c.a.hk);
                 if (lane == 0) {
                     start[0] = found;
                     start[1] = (int)(rest / n);
@@ -470,73 +479,120 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
     }
 }
 
-// Joins the partials of the units that CTA ranges cut. One CTA per (token row, query head, 128 columns); its
-// warps take the unit's partials in turn, in CTA order, and their sums are added in warp order.
-constexpr int kJoinWarps = 8;
+// Joins the partials of the units that CTA ranges cut. An item is 128 columns of one row of a unit; kWpi warps of
+// a block share it: they take the unit's partials in turn, in CTA order, and their sums are added in warp order.
+constexpr int kJoinBatch = 10;
 
-template <int D>
+template <int D, int kWpi, int kJoinWarps>
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const __grid_constant__ FewCall c) {
-    constexpr int kW = D < 128 ? D : 128;        // columns per CTA
+    constexpr int kW = D < 128 ? D : 128;        // columns of an item
     constexpr int kV = kW / 32;                  // per lane
-    __shared__ float s_ml[kJoinWarps][2];
+    constexpr int kItems = kJoinWarps / kWpi;    // of a block: consecutive rows
+    __shared__ float s_top[kJoinWarps], s_sum[kJoinWarps];
     __shared__ float s_o[kJoinWarps][kW];
     wait_for_predecessor();
     release_successor();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int b = blockIdx.y, h = blockIdx.x / c.part_rows, r = blockIdx.x % c.part_rows;
+    const int item = threadIdx.x / (32 * kWpi), warp = (threadIdx.x >> 5) % kWpi, lane = threadIdx.x & 31;
+    const int groups = (c.part_rows + kItems - 1) / kItems;
+    const int b = blockIdx.y, h = blockIdx.x / groups, r = blockIdx.x % groups * kItems + item;
     const SeqWork w = seq_work(c, b);
-    if (w.nt == 0 || r >= w.g.q_len * c.group) return;
+    const int rows = w.g.q_len * c.group;
+    if (w.nt <= 1 || blockIdx.x % groups * kItems >= rows) return;
     // the unit's tiles in the list, and the CTAs whose ranges hold its first and its last one
-    const int64_t total = tiles_before(c, c.a.pv.n_seqs, lane);
-    const int64_t u0 = tiles_before(c, b, lane) + (int64_t)h * w.nt, u1 = u0 + w.nt;
-    const int c0 = (int)(((u0 + 1) * c.ctas - 1) / total), c1 = (int)((u1 * c.ctas - 1) / total);
-    if (c0 == c1) return;                         // one CTA had all of it and wrote the result
-    const int col = blockIdx.z * kW + lane * kV;
-    // A CTA whose range starts with a tile of this unit after its first has it in slot 0; the CTA that has the
-    // unit's first tile, in slot 1.
-    float top = -INFINITY;
-    for (int i = c0 + lane; i <= c1; i += 32) {
-        const int64_t slot = (int64_t)i * 2 + (i == c0 ? 1 : 0);
-        if (total * (i + 1) / c.ctas > total * i / c.ctas) top = fmaxf(top, c.part_ml[(slot * c.part_rows + r) * 2]);
+    uint32_t total = 0, u0 = 0;
+    for (int b0 = 0; b0 < c.a.pv.n_seqs; b0 += 32) {
+        const int nt = b0 + lane < c.a.pv.n_seqs ? seq_work(c, b0 + lane).nt : 0;
+        const uint32_t inc = warp_scan(nt * c.a.hk, lane);
+        if (b >= b0 && b < b0 + 32) u0 = total + __shfl_sync(0xFFFFFFFFu, inc - nt * c.a.hk, b - b0);
+        total += __shfl_sync(0xFFFFFFFFu, inc, 31);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    const float ref = top == -INFINITY ? 0.0f : top;
+    u0 += (uint32_t)h * w.nt;
+    const Ranges ranges(total, c.ctas);
+    const int c0 = (int)ranges.owner(u0), parts = (int)ranges.owner(u0 + w.nt - 1) - c0 + 1;
+    if (parts == 1) return;                      // one CTA had all of it and wrote the result
     float acc[kV];
 #pragma unroll
     for (int e = 0; e < kV; ++e) acc[e] = 0.0f;
-    float sum = 0.0f;
-#pragma unroll 4
-    for (int i = c0 + warp; i <= c1; i += kJoinWarps) {
-        if (total * (i + 1) / c.ctas <= total * i / c.ctas) continue;
-        const int64_t at = ((int64_t)i * 2 + (i == c0 ? 1 : 0)) * c.part_rows + r;
-        const float f = fast_exp2(c.part_ml[at * 2] - ref);
-        sum += f * c.part_ml[at * 2 + 1];
-        if constexpr (kV == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(c.part_o + at * D + col);
-            acc[0] += f * v.x, acc[1] += f * v.y, acc[2] += f * v.z, acc[3] += f * v.w;
-        } else {
-            const float2 v = *reinterpret_cast<const float2*>(c.part_o + at * D + col);
-            acc[0] += f * v.x, acc[1] += f * v.y;
+    float top = -INFINITY, sum = 0.0f;           // of this warp's partials so far
+    if (r < rows) {
+        // The CTA that has the unit's first tile left its partial in slot 1, the ones whose ranges start inside the
+        // unit in slot 0. This warp's partials are warp, warp + kWpi, ...: lane k has the k-th one's numbers.
+        auto row_of = [&](int i) { return ((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * c.part_rows + r; };
+        for (int i0 = warp; i0 < parts; i0 += kJoinBatch * kWpi) {
+            const int mine = i0 + lane * kWpi;
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (lane < kJoinBatch && mine < parts) ml = *reinterpret_cast<const float2*>(c.part_ml + row_of(mine) * 2);
+            float v[kJoinBatch][kV];
+#pragma unroll
+            for (int k = 0; k < kJoinBatch; ++k) {
+                const int i = i0 + k * kWpi;
+                if (i < parts) {
+                    const float* p = c.part_o + row_of(i) * D + blockIdx.z * kW + lane * kV;
+                    if constexpr (kV == 4) {
+                        const float4 t = *reinterpret_cast<const float4*>(p);
+                        v[k][0] = t.x, v[k][1] = t.y, v[k][2] = t.z, v[k][3] = t.w;
+                    } else {
+                        const float2 t = *reinterpret_cast<const float2*>(p);
+                        v[k][0] = t.x, v[k][1] = t.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kV; ++e) v[k][e] = 0.0f;
+                }
+            }
+            float now = fmaxf(top, ml.x);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xFFFFFFFFu, now, o));
+            const float ref = now == -INFINITY ? 0.0f : now, back = fast_exp2(top - ref), f = fast_exp2(ml.x - ref);
+            top = now;
+            sum = sum * back + f * ml.y;
+#pragma unroll
+            for (int e = 0; e < kV; ++e) acc[e] *= back;
+#pragma unroll
+            for (int k = 0; k < kJoinBatch; ++k) {
+                const float g = __shfl_sync(0xFFFFFFFFu, f, k);
+#pragma unroll
+                for (int e = 0; e < kV; ++e) acc[e] += g * v[k][e];
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    }
+    if constexpr (kWpi > 1) {   // the item's warps, each relative to its own maximum
+        if (lane == 0) s_top[item * kWpi + warp] = top;
+        __syncthreads();
+        float all = s_top[item * kWpi + lane % kWpi];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
+        const float scale = top == -INFINITY ? 0.0f : fast_exp2(top - all);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) s_o[item * kWpi + warp][lane * kV + e] = acc[e] * scale;
+        if (lane == 0) s_sum[item * kWpi + warp] = sum * scale;
+        __syncthreads();
+        if (warp != 0) return;
+        sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < kV; ++e) acc[e] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWpi; ++i) {
+            sum += s_sum[item * kWpi + i];
+#pragma unroll
+            for (int e = 0; e < kV; ++e) acc[e] += s_o[item * kWpi + i][lane * kV + e];
         }
     }
+    if (r >= rows) return;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int tok = r / c.group, hd = h * c.group + r % c.group;
+    uint16_t* dst = c.a.out + (int64_t)(w.g.q0 + tok) * c.a.o_t + (int64_t)hd * c.a.o_h + blockIdx.z * kW + lane * kV;
 #pragma unroll
-    for (int e = 0; e < kV; ++e) s_o[warp][lane * kV + e] = acc[e];
-    if (lane == 0) s_ml[warp][0] = sum;
-    __syncthreads();
-    if (threadIdx.x < kW / 2) {
-        float lsum = 0.0f, x = 0.0f, y = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kJoinWarps; ++i) {
-            lsum += s_ml[i][0];
-            x += s_o[i][2 * threadIdx.x];
-            y += s_o[i][2 * threadIdx.x + 1];
-        }
-        const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-        const int tok = r / c.group, hd = h * c.group + r % c.group;
-        *reinterpret_cast<uint32_t*>(c.a.out + (int64_t)(w.g.q0 + tok) * c.a.o_t + (int64_t)hd * c.a.o_h +
-                                     blockIdx.z * kW + 2 * threadIdx.x) = pack_bf16(x * inv, y * inv);
-    }
+    for (int e = 0; e < kV; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16(acc[e] * inv, acc[e + 1] * inv);
+}
+
+template <int D, int kWpi, int kJoinWarps>
+void launch_join(const FewCall& c, cudaStream_t st) {
+    constexpr int kItems = kJoinWarps / kWpi;
+    const dim3 grid((unsigned)((c.part_rows + kItems - 1) / kItems * c.a.hk), (unsigned)c.a.pv.n_seqs, D < 128 ? 1 : D / 128);
+    launch_dependent(attn_join_kernel<D, kWpi, kJoinWarps>, grid, dim3(kJoinWarps * 32), 0, st, c);
 }
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -570,12 +626,18 @@ void launch_few(const Attn& h, const AttnCall& a, cudaStream_t st) {
     int64_t cap = (int64_t)a.pv.max_pages << a.pv.page_shift;
     if (a.window > 0) cap = std::min<int64_t>(cap, (int64_t)a.window + c.max_rows / c.group + c.box);
     const int64_t per_unit = std::max<int64_t>(1, (cap + kKeys - 1) / kKeys);
+    if (per_unit * a.hk * a.pv.n_seqs > 0x7FFFFFFF) throw Error(G4Q_ERR_UNSUPPORTED_CONFIG, "too many key tiles for one call");
     c.ctas = (int)std::min<int64_t>(few_ctas<D, MT>(), per_unit * a.hk * a.pv.n_seqs);
     const CUtensorMap tk = paged_map(a, a.k, D, c.box), tv = paged_map(a, a.v, D, c.box);
     launch_dependent(attn_few_kernel<D, MT>, dim3((unsigned)c.ctas), dim3(kThreads), C::kSmem, st, tk, tv, c);
     if (per_unit > 1) {   // a unit of one tile is never cut
-        const dim3 grid((unsigned)(c.part_rows * a.hk), (unsigned)a.pv.n_seqs, D < 128 ? 1 : D / 128);
-        launch_dependent(attn_join_kernel<D>, grid, dim3(kJoinWarps * 32), 0, st, c);
+        // Few items with possibly many partials each: a block to an item. Else two warps: the blocks are few then,
+        // and a unit has about as many partials as CTAs there are to a unit.
+        const int64_t items = (int64_t)c.part_rows * a.hk * a.pv.n_seqs * (D < 128 ? 1 : D / 128);
+        if (per_unit > 64 && items <= 256)
+            launch_join<D, 16, 16>(c, st);
+        else
+            launch_join<D, 2, 4>(c, st);
     }
 }
 

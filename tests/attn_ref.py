@@ -4,9 +4,9 @@ Every function returns (value, bound) in float64. The bounds, with u = 2^-24 (fp
 of half a step:
 
 * norm and rotation of a head of D elements: the sum of squares is D/32 (at most 16) fmas and 5 adds of
-  positive terms in fp32, so off by at most 21 u, its root by half of that; the mean, the reciprocal root, two
-  products, the sine and cosine (2 ulp and pi u for the reduced angle) and the rotation's two operations add
-  at most 15 u: below 2^-19 of |y_i| + |y_j| of the pair.
+  positive terms in fp32, so off by at most 21 u, its root by half of that; the mean, the reciprocal root, the
+  weight's and the scale's products and the rotation's two operations add at most 8 u, the reduced angle pi u
+  and the hardware sine and cosine 2^-21.2 = 7 u: below 2^-19 = 32 u of |y_i| + |y_j| of the pair.
 * attention: each score is a sum of D exact products in fp32, off by at most D 2^-23 sum|q k|, the sum's
   running value being at most that; the exponential and the running rescaling add 2^-20 relative. A weight is
   rounded to bf16 (2^-9 to either side), and the sum of the weights takes them rounded, so numerator and
