@@ -642,8 +642,7 @@ void launch_few(const Attn& h, const AttnCall& a, cudaStream_t st) {
 }
 
 template <int D>
-void launch_few_rows(const Attn& h, const AttnCall& a, cudaStream_t st) {
-    const int64_t rows = (int64_t)a.pv.max_q * (a.hq / a.hk);
+void launch_few_rows(const Attn& h, const AttnCall& a, int64_t rows, cudaStream_t st) {
     if (rows <= 16)
         launch_few<D, 1>(h, a, st);
     else if (rows <= 32)
@@ -701,25 +700,28 @@ size_t attn_part_rows(int head_dim) {
     return std::max(few, chunk_part_rows());
 }
 
-void launch_few_any(const Attn& h, const AttnCall& a, cudaStream_t st) {
+void launch_few_any(const Attn& h, const AttnCall& a, int64_t rows, cudaStream_t st) {
     switch (h.head_dim) {
-        case 64: return launch_few_rows<64>(h, a, st);
-        case 128: return launch_few_rows<128>(h, a, st);
-        case 256: return launch_few_rows<256>(h, a, st);
-        case 512: return launch_few_rows<512>(h, a, st);
+        case 64: return launch_few_rows<64>(h, a, rows, st);
+        case 128: return launch_few_rows<128>(h, a, rows, st);
+        case 256: return launch_few_rows<256>(h, a, rows, st);
+        case 512: return launch_few_rows<512>(h, a, rows, st);
     }
 }
 
 void launch_attention(const Attn& h, const AttnCall& a, cudaStream_t st) {
-    // A sequence goes by its own rows (new tokens x group): at most 64 to the kernel above, which shares the keys
-    // evenly over the SMs, more to the chunk kernel. Only the lengths on the device say which are there; where
-    // every row belongs to a sequence of max_q tokens, or there is one sequence only, the host knows.
+    // A sequence goes by its own rows (new tokens x group): few to the kernel above, which shares the keys evenly over
+    // the SMs, more to the chunk kernel. Only the lengths on the device say which are there; where every row belongs
+    // to a sequence of max_q tokens, or there is one sequence only, the host knows. In a mixed step the few are the
+    // single tokens (16 rows unless the group is larger): with 64 rows the kernel's products outweigh the bytes
+    // (two tokens beside four prompts, head_dim 256: 20.8 us against 8).
     const int group = a.hq / a.hk;
     const int64_t rows = (int64_t)a.pv.max_q * group;
-    if (rows <= kFewRows) return launch_few_any(h, a, st);
+    if (rows <= kFewRows) return launch_few_any(h, a, rows, st);
     if ((int64_t)a.pv.n_seqs * a.pv.max_q == a.pv.rows) return launch_chunk(h, a, 0, st);
-    launch_few_any(h, a, st);
-    launch_chunk(h, a, kFewRows, st);
+    const int few = group <= 16 ? 16 : group <= 32 ? 32 : 64;
+    launch_few_any(h, a, few, st);
+    launch_chunk(h, a, few, st);
 }
 
 }  // namespace g4q

@@ -8,8 +8,9 @@
 // and half of a V tile's columns, and the pair's MMAs read both halves: on single CTAs the fetches of 128 rows' K
 // and V (64 bytes per cycle and SM at head_dim 256) outran L2 and took 3000-4000 cycles a tile. The pair walks
 // the 128-key tiles that its rows see, warp-specialised in each CTA:
-//   warp 0      fills a ring of up to 32 KB stages by TMA (boxes of one page x 64 elements, SWIZZLE_128B), K and V
-//               in the order they are used.
+//   warps 0, 6  fill a ring of K and a ring of V stages (up to 32 KB each) by TMA: boxes of one page x 64 elements,
+//               SWIZZLE_128B. A warp issues a box in about 90 cycles, and pages of 16 slots make 16 boxes a stage: one
+//               warp for both took 3200 cycles a tile.
 //   warp 1      of the first CTA: one thread issues the MMAs: S = Q K^T (both operands K-major in shared memory,
 //               M = 256, N = 128) into one of two TMEM buffers, and O += P V (P from TMEM, V as it lies, MN-major)
 //               into up to 256 TMEM columns. S of tile j+1 is computed before P V of tile j, so the tensor cores
@@ -22,8 +23,10 @@
 // for the softmax they take: single CTAs (cta_group::1) run the same code.
 // head_dim 512: O would take all of TMEM, so a CTA computes half of the output columns and the scores whole
 // (1.5 times the products of a single pass; a row tile of 64 would halve the tensor cores' rate instead).
-// Few tiles for many SMs (a drafted block, a small chunk over a long context): the keys of a tile are split
-// over grid.z and a join kernel adds the fp32 partials in split order.
+// The row tiles (x key heads x halves) that fill the GPU in whole waves are computed whole, the longest of a causal
+// chunk first. The rest, which would leave SMs idle for a wave (or all of them, for a drafted block or a small chunk
+// over a long context), have their keys cut into as many pieces as there are CTAs for them, 6 key tiles or more
+// each; a join kernel adds the fp32 partials in piece order.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -36,11 +39,12 @@ namespace g4q {
 namespace {
 
 constexpr int kTile = 128;             // query rows and keys of a tile
-constexpr int kThreads = 192;
+constexpr int kThreads = 224;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 8.0f;         // how far (log2) a score may exceed the maximum in use
 constexpr uint32_t kTmemCols = 512;
-constexpr int kMaxSplits = 16;
+constexpr int kMaxSplits = 32;         // pieces of a tile's keys
+constexpr int kMinPiece = 6;           // key tiles of a piece, at least
 
 template <int D>
 struct ChunkCfg {
@@ -55,8 +59,11 @@ struct ChunkCfg {
     static constexpr int kQBytes = kTile * D * 2;
     static constexpr int kFit = (227 * 1024 - 1024 - 256 - kQBytes) / kStageBytes;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
+    static constexpr int kVStages = kStages / 2 < 1 ? 1 : (kStages - (kKSt - 1)) / 2;   // of the ring of V tiles
+    static constexpr int kKStages = kStages - kVStages;                                 // of the ring of K tiles
     static constexpr int kSmem = 1024 + kQBytes + kStages * kStageBytes + 256;
-    static_assert(kKeysHeld * kKCols == kTile * kVCols && kVCols % 64 == 0 && kStages >= 3, "stages hold either operand");
+    static_assert(kKeysHeld * kKCols == kTile * kVCols && kVCols % 64 == 0, "stages hold either operand");
+    static_assert(kVStages >= 1 && kKStages >= kKSt, "a tile of each fits");
 };
 
 struct ChunkCall {
@@ -66,11 +73,17 @@ struct ChunkCall {
     int tokens;          // tokens of a CTA's 128 rows: 128 / group
     int tile_tokens;     // tokens of a tile: of all the CTAs that share it
     int box;
-    int splits;
-    int slots;           // tiles the grid has room for
-    float* part_o;       // [splits][slots * hk][CTAs of a tile * 128][D]
-    float* part_ml;      // [splits][slots * hk][CTAs of a tile * 128][2]
+    int wave;            // tiles that the GPU computes at once
+    float* part_o;       // [pieces, at most a wave][CTAs of a tile * 128][output columns of a CTA]
+    float* part_ml;      // [pieces][CTAs of a tile * 128][2]
     int* err;
+};
+
+// A tile of work: rows of sequence b, key head, half of the output columns, and the piece of its keys.
+struct Work {
+    int b, tile, h, half;
+    int piece, pieces;   // of the keys
+    int slot;            // place of the piece's partial
 };
 
 struct TileWork {
@@ -85,17 +98,22 @@ __device__ __forceinline__ int tiles_of(const ChunkCall& c, int b) {
     return g.q_len * c.group > c.few_rows ? (g.q_len + c.tile_tokens - 1) / c.tile_tokens : 0;
 }
 
-// The sequence and place of row tile `t` of the batch, found by one warp: {b, tile in b}, b < 0 past the end.
-// `reverse`: counted from the end of the batch.
-__device__ __forceinline__ int2 find_tile(const ChunkCall& c, int t, bool reverse, int lane) {
-    if (reverse) {
-        int total = 0;
-        for (int b = lane; b < c.a.pv.n_seqs; b += 32) total += tiles_of(c, b);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
-        t = total - 1 - t;
-        if (t < 0) return make_int2(-1, 0);
+// The sequence and place of the t-th row tile of the batch (t < total), found by one warp. The longest come first:
+// a sequence's last tile, and up to 32 sequences by their lengths (more: the batch's last first).
+__device__ __forceinline__ int2 find_tile(const ChunkCall& c, int t, int total, int lane) {
+    if (c.a.pv.n_seqs <= 32) {
+        const int nt = lane < c.a.pv.n_seqs ? tiles_of(c, lane) : 0, kv = lane < c.a.pv.n_seqs ? c.a.pv.kv_lens[lane] : -1;
+        int before = 0;
+        for (int o = 0; o < c.a.pv.n_seqs; ++o) {
+            const int kv_o = __shfl_sync(0xFFFFFFFFu, kv, o), nt_o = __shfl_sync(0xFFFFFFFFu, nt, o);
+            if (kv_o > kv || (kv_o == kv && o < lane)) before += nt_o;
+        }
+        const unsigned here = __ballot_sync(0xFFFFFFFFu, t >= before && t < before + nt);
+        const int at = here != 0 ? __ffs(here) - 1 : 0;
+        const int first = __shfl_sync(0xFFFFFFFFu, before, at), n = __shfl_sync(0xFFFFFFFFu, nt, at);
+        return here != 0 ? make_int2(at, n - 1 - (t - first)) : make_int2(-1, 0);
     }
+    t = total - 1 - t;
     int before = 0;
     for (int b0 = 0; b0 < c.a.pv.n_seqs; b0 += 32) {
         const int nt = b0 + lane < c.a.pv.n_seqs ? tiles_of(c, b0 + lane) : 0;
@@ -125,6 +143,40 @@ __device__ __forceinline__ TileWork tile_work(const ChunkCall& c, int b, int til
     w.any_lo = c.a.window > 0 ? max(0, w.g.first + w.t0 - c.a.window + 1) : 0;
     w.lo = min(w.any_lo, w.any_hi) & ~(c.box - 1);
     w.n = max(1, (w.any_hi - w.lo + kTile - 1) / kTile);    // rows that see nothing still become zeros
+    return w;
+}
+
+// The work of the index-th CTA (pair) of the launch, or of the index-th tile of the last wave (kLast); b < 0: none.
+// One warp. Tiles of the whole waves come first, each one CTA pair's; then every tile of the rest `cuts` times.
+template <int D, bool kLast>
+__device__ __forceinline__ Work find_work(const ChunkCall& c, int index, int lane) {
+    constexpr int kHalves = ChunkCfg<D>::kHalves;
+    Work w;
+    w.b = -1;
+    int total = 0;
+    for (int b = lane; b < c.a.pv.n_seqs; b += 32) total += tiles_of(c, b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+    const int per_tile = c.a.hk * kHalves, items = total * per_tile;
+    const int whole = items / c.wave * c.wave, rest = items - whole;
+    const int cuts = rest > 0 ? min(kMaxSplits, c.wave / rest) : 1;
+    int item = index, piece = 0;
+    if (kLast) {
+        if (index >= rest) return w;
+        item = whole + index;
+    } else if (index >= whole) {
+        item = whole + (index - whole) / cuts;
+        piece = (index - whole) % cuts;
+    }
+    if (item >= items) return w;
+    const int2 at = find_tile(c, item / per_tile, total, lane);
+    w.tile = at.y;
+    w.h = item % per_tile / kHalves;
+    w.half = item % kHalves;
+    w.pieces = item < whole ? 1 : max(1, min(cuts, tile_work(c, at.x, at.y).n / kMinPiece));
+    w.piece = piece;
+    w.slot = (item - whole) * cuts + piece;
+    if (piece < w.pieces) w.b = at.x;
     return w;
 }
 
@@ -286,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     using C = ChunkCfg<D>;
     constexpr int kCtas = C::kCtas;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ int2 found;
+    __shared__ Work found;
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_addr(smem_raw));
     const uint32_t s_q = base, s_ring = s_q + C::kQBytes, s_bar = s_ring + C::kStages * C::kStageBytes;
@@ -296,15 +348,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto p_full = [&](int b) { return s_bar + 8u * (2 * C::kStages + 2 + b); };
     const uint32_t q_full = s_bar + 8u * (2 * C::kStages + 4);
     auto o_done = [&](int b) { return q_full + 8u + 8u * b; };    // products of the even and the odd tiles
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (s_bar - base) + 8u * (2 * C::kStages + 7));
+    const uint32_t edge_full = q_full + 24;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (s_bar - base) + 8u * (2 * C::kStages + 8));
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = blockIdx.x % kCtas;                 // place in the pair (clusters run along x)
-    const int half = blockIdx.x / kCtas % C::kHalves, h = blockIdx.x / (kCtas * C::kHalves);
-    wait_for_predecessor();
-    release_successor();
+    const int rank = blockIdx.x % kCtas;                 // place in the pair
     if (warp == 0) {
-        const int2 f = find_tile(c, blockIdx.y, true, lane);    // the longest tiles of a causal chunk start first
+        wait_for_predecessor();
+        const Work f = find_work<D, false>(c, blockIdx.x / kCtas, lane);
         if (lane == 0) found = f;
     } else if (warp == 1) {
         if constexpr (kCtas == 2) {
@@ -327,32 +378,39 @@ __global__ void __launch_bounds__(kThreads, 1)
             bar_init(o_done(b), 1);
         }
         bar_init(q_full, kCtas);
+        bar_init(edge_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (const CUtensorMap* map : {&tm_q, &tm_k, &tm_v})
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
     }
+    wait_for_predecessor();
+    release_successor();
     tc_fence_before();
     __syncthreads();
     if constexpr (kCtas == 2) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const uint32_t t_o = tmem, t_s = tmem + 256;     // output, two score buffers of 128 columns
-    const int2 at = found;
+    const Work at = found;
+    const int h = at.h, half = at.half;
 
-    if (at.x >= 0) {
-        const TileWork w = tile_work(c, at.x, at.y);
+    if (at.b >= 0) {
+        const TileWork w = tile_work(c, at.b, at.tile);
         const int t0 = w.t0 + rank * c.tokens;       // this CTA's first token
-        // this split's key tiles
-        const int j0 = (int)((int64_t)w.n * blockIdx.z / c.splits), n = (int)((int64_t)w.n * (blockIdx.z + 1) / c.splits) - j0;
-        if (warp == 0) {
-            // ---------------- producer
-            if (n > 0 && lane == 0) {
+        // this piece's key tiles
+        const int j0 = w.n * at.piece / at.pieces, n = w.n * (at.piece + 1) / at.pieces - j0;
+        if (warp == 0 || warp == 6) {
+            // ---------------- producers: Q and K tiles (warp 0), V tiles (warp 6)
+            if (warp == 0 && lane == 0) {
                 const uint32_t qb = in_first_cta(q_full);
                 bar_expect_tx_cluster(qb, (uint32_t)(c.tokens * c.group) * 128u * (D / 64));
                 for (int x = 0; x < D / 64; ++x)
                     tma_rows<kCtas>(s_q + x * (kTile * 128), &tm_q, x * 64, h * c.group, w.g.q0 + t0, qb);
             }
             __syncwarp();
-            int stage = 0;
-            uint32_t round = 0;
+            const int first_stage = warp == 0 ? 0 : C::kKStages, last_stage = warp == 0 ? C::kKStages : C::kStages;
+            int stage = first_stage;
+            uint32_t round = 0, edge_round = 0;
             const PagedView& pv = c.a.pv;
             const int page_mask = (1 << pv.page_shift) - 1;
             const uint32_t box_bytes = (uint32_t)c.box * 128u;
@@ -363,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int key = w.lo + (j0 + j) * kTile + lane * c.box;
                 int page = pv.n_pages;                    // outside the map: reads zeros
                 if (j < n && lane < boxes && key < w.any_hi) {
-                    page = pv.table[at.x * pv.table_ld + (key >> pv.page_shift)];
+                    page = pv.table[at.b * pv.table_ld + (key >> pv.page_shift)];
                     if (page < 0 || page >= pv.n_pages) {
                         record_input_error(pv.err, kErrPage);
                         page = pv.n_pages;
@@ -373,8 +431,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             // boxes [b0, b1) of the stage's keys k0.. (`keys` of them, the first one box `first` of its tile) by TMA,
             // columns [col0, col0 + 64 * blocks)
-            auto fill = [&](const CUtensorMap* map, int pages, int k0, int keys, int first, int b0, int b1, int col0, int blocks) {
-                const uint32_t bar = in_first_cta(full(stage));
+            auto fill = [&](const CUtensorMap* map, uint32_t bar, int pages, int k0, int keys, int first, int b0, int b1, int col0,
+                            int blocks) {
                 if (lane == 0) bar_expect_tx_cluster(bar, (uint32_t)((b1 - b0) * blocks) * box_bytes);
                 __syncwarp();
                 for (int i0 = 0; i0 < (b1 - b0) * blocks; i0 += 32) {
@@ -384,7 +442,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tma_page<kCtas>(s_ring + stage * C::kStageBytes + cb * (keys * 128) + box * box_bytes, map, col0 + cb * 64,
                                         (k0 + box * c.box) & page_mask, h, page, bar);
                 }
-                if (++stage == C::kStages) stage = 0, ++round;
             };
             auto load_k = [&](int j, int pages) {
                 const int k0 = w.lo + (j0 + j) * kTile + rank * C::kKeysHeld;
@@ -392,63 +449,52 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int nb = max(0, min(C::kKeysHeld / c.box, (w.any_hi - k0 + c.box - 1) / c.box));
                 for (int p = 0; p < C::kKSt; ++p) {
                     if (round > 0) bar_wait(empty(stage), (round - 1) & 1, c.err, 80);
-                    fill(&tm_k, pages, k0, C::kKeysHeld, rank * C::kKeysHeld / c.box, 0, nb, p * C::kKCols, C::kKCols / 64);
+                    fill(&tm_k, in_first_cta(full(stage)), pages, k0, C::kKeysHeld, rank * C::kKeysHeld / c.box, 0, nb,
+                         p * C::kKCols, C::kKCols / 64);
+                    if (++stage == last_stage) stage = first_stage, ++round;
                 }
             };
             auto load_v = [&](int j, int pages) {
                 const int k0 = w.lo + (j0 + j) * kTile, col0 = half * C::kDv + rank * C::kVCols;
                 if (round > 0) bar_wait(empty(stage), (round - 1) & 1, c.err, 80);
-                // Keys that no row of the tile sees hold anything, and a zero weight times NaN is NaN: only boxes of
-                // seen keys come by TMA, the others row by row, with zeros for the keys that are not seen.
-                const int b1 = min(kTile, max(0, w.any_hi - k0)) / c.box;
-                const int b0 = min(b1, max(0, (w.any_lo - k0 + c.box - 1) / c.box));
-                if (b1 - b0 < boxes) {
-                    const int head = b0 * c.box, tail = b1 * c.box;      // rows [0, head) and [tail, 128) by hand
-                    const int rows = head + kTile - tail;
-                    constexpr int kChunks = C::kVCols / 8, kBatch = 8;   // loads in flight per lane
-                    for (int i0 = 0; i0 < rows * kChunks; i0 += 32 * kBatch) {
-                        uint4 v[kBatch];
-#pragma unroll
-                        for (int u = 0; u < kBatch; ++u) {
-                            const int i = i0 + u * 32 + lane, ch = i % kChunks;
-                            int row = min(i / kChunks, rows - 1);
-                            if (row >= head) row += tail - head;
-                            const int key = k0 + row;
-                            const int page = __shfl_sync(0xFFFFFFFFu, pages, row / c.box);
-                            v[u] = make_uint4(0, 0, 0, 0);
-                            if (key >= w.any_lo && key < w.any_hi && page < pv.n_pages)
-                                v[u] = *reinterpret_cast<const uint4*>(c.a.v + page * c.a.page_stride + h * c.a.head_stride +
-                                                                       (key & ((1 << pv.page_shift) - 1)) * c.a.slot_stride + col0 + ch * 8);
-                        }
-#pragma unroll
-                        for (int u = 0; u < kBatch; ++u) {
-                            const int i = i0 + u * 32 + lane, ch = i % kChunks;
-                            int row = i / kChunks;
-                            if (row >= rows) continue;
-                            if (row >= head) row += tail - head;
-                            *reinterpret_cast<uint4*>(gen + (s_ring - base) + stage * C::kStageBytes + (ch >> 3) * (kTile * 128) +
-                                                      row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = v[u];
-                        }
+                const int b1 = max(0, min(boxes, (w.any_hi - k0 + c.box - 1) / c.box));
+                if (k0 >= w.any_lo && k0 + kTile <= w.any_hi) {
+                    fill(&tm_v, in_first_cta(full(stage)), pages, k0, kTile, 0, 0, boxes, col0, C::kVCols / 64);
+                } else {
+                    // Keys that no row of the tile sees hold anything, and a zero weight times NaN is NaN: the stage
+                    // is filled on a barrier of this CTA's own, their rows are zeroed, and it is handed over then.
+                    const int b0 = max(0, w.any_lo - k0) / c.box;
+                    fill(&tm_v, edge_full, pages, k0, kTile, 0, min(b0, b1), b1, col0, C::kVCols / 64);
+                    bar_wait(edge_full, edge_round++ & 1, c.err, 88);
+                    const int lo = min(kTile, max(0, w.any_lo - k0)), hi = min(kTile, max(lo, w.any_hi - k0));
+                    for (int i = lane; i < (lo + kTile - hi) * (C::kVCols / 8); i += 32) {
+                        const int ch = i & 7, x = i >> 3, cb = x % (C::kVCols / 64);
+                        int row = x / (C::kVCols / 64);
+                        if (row >= lo) row += hi - lo;
+                        *reinterpret_cast<uint4*>(gen + (s_ring - base) + stage * C::kStageBytes + cb * (kTile * 128) + row * 128 +
+                                                  ch * 16) = make_uint4(0, 0, 0, 0);
                     }
                     asm volatile("fence.proxy.async.shared::cta;\n\tfence.acq_rel.cluster;" ::: "memory");
                     __syncwarp();
+                    if (lane == 0) bar_expect_tx_cluster(in_first_cta(full(stage)), 0);
                 }
-                fill(&tm_v, pages, k0, kTile, 0, b0, b1, col0, C::kVCols / 64);
+                if (++stage == last_stage) stage = first_stage, ++round;
             };
             int pages = look_up(0), pages1 = look_up(1);
-            if (n > 0) load_k(0, pages);
             for (int j = 0; j < n; ++j) {
                 const int pages2 = look_up(j + 2);
-                if (j + 1 < n) load_k(j + 1, pages1);
-                load_v(j, pages);
+                if (warp == 0)
+                    load_k(j, pages);
+                else
+                    load_v(j, pages);
                 pages = pages1;
                 pages1 = pages2;
             }
         } else if (warp == 1) {
             // ---------------- MMA issuer (of the pair's first CTA)
             if (rank == 0) {
-                int stage = 0;
-                uint32_t round = 0;
+                int stage = 0, v_stage = C::kKStages;
+                uint32_t round = 0, v_round = 0;
                 auto scores = [&](int j) {
                     for (int p = 0; p < C::kKSt; ++p) {
                         bar_wait(full(stage), round & 1, c.err, 81);
@@ -463,31 +509,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                             mma_commit<kCtas>(empty(stage));
                         }
                         __syncwarp();
-                        if (++stage == C::kStages) stage = 0, ++round;
+                        if (++stage == C::kKStages) stage = 0, ++round;
                     }
                     if (lane == 0) mma_commit<kCtas>(s_full(j & 1));
                     __syncwarp();
                 };
-                if (n > 0) {
-                    bar_wait(q_full, 0, c.err, 82);
-                    scores(0);
-                }
+                bar_wait(q_full, 0, c.err, 82);
+                scores(0);
                 for (int j = 0; j < n; ++j) {
                     if (j + 1 < n) scores(j + 1);
                     bar_wait(p_full(j & 1), (j >> 1) & 1, c.err, 83);
-                    bar_wait(full(stage), round & 1, c.err, 84);
+                    bar_wait(full(v_stage), v_round & 1, c.err, 84);
                     tc_fence_after();
                     if (lane == 0) {
 #pragma unroll
                         for (int kk = 0; kk < kTile / 16; ++kk)
                             mma_ts<kCtas>(t_o, t_s + (j & 1) * kTile + kk * 8,
-                                          sw128_desc(s_ring + stage * C::kStageBytes + kk * 2048, kTile * 128),
+                                          sw128_desc(s_ring + v_stage * C::kStageBytes + kk * 2048, kTile * 128),
                                           instr_desc(kTile * kCtas, C::kDv, true), (j | kk) != 0);
-                        mma_commit<kCtas>(empty(stage));
+                        mma_commit<kCtas>(empty(v_stage));
                         mma_commit<kCtas>(o_done(j & 1));
                     }
                     __syncwarp();
-                    if (++stage == C::kStages) stage = 0, ++round;
+                    if (++v_stage == C::kStages) v_stage = C::kKStages, ++v_round;
                 }
             }
         } else {
@@ -519,8 +563,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tmem_wait_ld(s, kTile);
                 if (k0 < all_lo || k0 + kTile > all_hi) {
 #pragma unroll
-                    for (int i = 0; i < kTile; ++i)
-                        if (k0 + i < vis_lo || k0 + i >= vis_hi) s[i] = 0xFF800000u;   // -inf
+                    for (int x = 0; x < kTile; x += 32) {
+                        // bit i: key k0 + x + i is seen
+                        const int lo = min(max(vis_lo - k0 - x, 0), 32), hi = min(max(vis_hi - k0 - x, 0), 32);
+                        const uint32_t seen = (hi == 32 ? 0xFFFFFFFFu : (1u << hi) - 1u) & ~(lo == 32 ? 0xFFFFFFFFu : (1u << lo) - 1u);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if ((seen & (1u << i)) == 0) s[x + i] = 0xFF800000u;       // -inf
+                    }
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -569,15 +619,42 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) bar_arrive_cluster(in_first_cta(p_full(j & 1)));
             }
             // ---------------- epilogue
-            if (n > 0) {
-                bar_wait(o_done((n - 1) & 1), ((n - 1) >> 1) & 1, c.err, 87);
-                tc_fence_after();
-            }
-            const int64_t token = w.g.q0 + t0 + tok;
-            const int hd = h * c.group + r % c.group;
-            if (c.splits == 1) {
+            bar_wait(o_done((n - 1) & 1), ((n - 1) >> 1) & 1, c.err, 87);
+            tc_fence_after();
+            if (at.pieces == 1) {
+                // through the ring's memory (nothing is in flight any more), so that a warp writes whole rows
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                uint16_t* dst = c.a.out + token * c.a.o_t + (int64_t)hd * c.a.o_h + half * C::kDv;
+                constexpr int kChunks = C::kDv / 8;                    // 16-byte chunks of a row
+                const uint32_t rows = s_ring + quarter * (32 * C::kDv * 2);
+                uint8_t* mem = gen + (rows - base);
+#pragma unroll 1
+                for (int x = 0; x < C::kDv; x += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(t_o + lanes + x, o);
+                    tmem_wait_ld(o, 32);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t pk[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            pk[e] = pack_bf16(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+                        *reinterpret_cast<uint4*>(mem + (lane * kChunks + ((x / 8 + i) ^ (lane & 7))) * 16) =
+                            make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                    }
+                }
+                __syncwarp();
+                constexpr int kAtOnce = 32 / kChunks;                  // rows of a store
+                const int64_t my_row = mine ? (int64_t)(w.g.q0 + t0 + tok) * c.a.o_t + (int64_t)(h * c.group + r % c.group) * c.a.o_h : -1;
+#pragma unroll 8
+                for (int r0 = 0; r0 < 32; r0 += kAtOnce) {
+                    const int rl = r0 + lane / kChunks, ch = lane % kChunks;
+                    const uint4 v = *reinterpret_cast<const uint4*>(mem + (rl * kChunks + (ch ^ (rl & 7))) * 16);
+                    const int64_t to = __shfl_sync(0xFFFFFFFFu, my_row, rl);
+                    if (to >= 0) *reinterpret_cast<uint4*>(c.a.out + to + half * C::kDv + ch * 8) = v;
+                }
+            } else {
+                const int64_t row = ((int64_t)at.slot * kCtas + rank) * kTile + r;
+                float* dst = c.part_o + row * C::kDv;
 #pragma unroll 1
                 for (int x = 0; x < C::kDv; x += 32) {
                     uint32_t o[32];
@@ -585,32 +662,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_wait_ld(o, 32);
                     if (mine) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            uint32_t pk[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                pk[e] = pack_bf16(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
-                            *reinterpret_cast<uint4*>(dst + x + i) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-                        }
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<uint4*>(dst + x + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                     }
                 }
-            } else {
-                const int64_t row = ((((int64_t)blockIdx.z * c.slots + blockIdx.y) * c.a.hk + h) * kCtas + rank) * kTile + r;
-                if (n > 0) {
-                    float* dst = c.part_o + row * D + half * C::kDv;
-#pragma unroll 1
-                    for (int x = 0; x < C::kDv; x += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(t_o + lanes + x, o);
-                        tmem_wait_ld(o, 32);
-                        if (mine) {
-#pragma unroll
-                            for (int i = 0; i < 32; i += 4)
-                                *reinterpret_cast<uint4*>(dst + x + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                        }
-                    }
-                }
-                if (half == 0) *reinterpret_cast<float2*>(c.part_ml + row * 2) = make_float2(m, l);   // no tile: -inf, 0
+                *reinterpret_cast<float2*>(c.part_ml + row * 2) = make_float2(m, l);
             }
         }
     }
@@ -627,42 +683,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// Joins the splits of every row tile: one warp per row of a tile, 128 columns
-// at a time, the partials added in split order.
+// Joins the pieces of the last wave's tiles (blockIdx.y), the partials added in piece order: a warp has every eighth
+// of 32 rows.
+constexpr int kJoinRows = 32;
+
 template <int D>
 __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_constant__ ChunkCall c) {
-    constexpr int kW = D < 128 ? D : 128, kV = kW / 32;
+    using C = ChunkCfg<D>;
+    constexpr int kRows = C::kCtas * kTile, kV = C::kDv / 32;         // output columns of a lane
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     wait_for_predecessor();
     release_successor();
-    const int2 at = find_tile(c, blockIdx.y, true, lane);
-    constexpr int kRows = ChunkCfg<D>::kCtas * kTile;
-    const int row = blockIdx.x * 8 + warp, r = row % kTile, h = blockIdx.z;
-    if (at.x < 0 || r >= c.tokens * c.group) return;
-    const TileWork w = tile_work(c, at.x, at.y);
-    const int tok = row / kTile * c.tokens + r / c.group;
-    if (w.t0 + tok >= w.g.q_len) return;
-    const int64_t row0 = ((int64_t)blockIdx.y * c.a.hk + h) * kRows + row, step = (int64_t)c.slots * c.a.hk * kRows;
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    if (lane < c.splits) ml = *reinterpret_cast<const float2*>(c.part_ml + (row0 + lane * step) * 2);
-    float top = ml.x;
+    const Work at = find_work<D, true>(c, blockIdx.y, lane);
+    if (at.b < 0 || at.pieces == 1) return;
+    const TileWork w = tile_work(c, at.b, at.tile);
+    for (int i = 0; i < kJoinRows; i += 8) {
+        const int row = blockIdx.x * kJoinRows + i + warp, r = row % kTile;
+        const int tok = row / kTile * c.tokens + r / c.group;
+        if (r >= c.tokens * c.group || w.t0 + tok >= w.g.q_len) continue;
+        const int64_t row0 = (int64_t)at.slot * kRows + row;
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (lane < at.pieces) ml = *reinterpret_cast<const float2*>(c.part_ml + (row0 + lane * kRows) * 2);
+        float top = ml.x;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    const float f = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
-    float total = f * ml.y;
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        const float f = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
+        float total = f * ml.y;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
-    const float mine = total == 0.0f ? 0.0f : f / total;
-    uint16_t* dst = c.a.out + (w.g.q0 + w.t0 + tok) * c.a.o_t + (int64_t)(h * c.group + r % c.group) * c.a.o_h;
-#pragma unroll 1
-    for (int x = 0; x < D; x += kW) {
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+        const float mine = total == 0.0f ? 0.0f : f / total;
         float acc[kV];
 #pragma unroll
         for (int e = 0; e < kV; ++e) acc[e] = 0.0f;
-        for (int z = 0; z < c.splits; ++z) {
+#pragma unroll 4
+        for (int z = 0; z < at.pieces; ++z) {
             const float g = __shfl_sync(0xFFFFFFFFu, mine, z);
-            if ((int64_t)w.n * (z + 1) / c.splits == (int64_t)w.n * z / c.splits) continue;   // had no keys
-            const float* src = c.part_o + (row0 + z * step) * D + x + lane * kV;
+            const float* src = c.part_o + (row0 + (int64_t)z * kRows) * C::kDv + lane * kV;
 #pragma unroll
             for (int e = 0; e < kV; e += 2) {
                 const float2 v = *reinterpret_cast<const float2*>(src + e);
@@ -670,9 +726,10 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_const
                 acc[e + 1] += g * v.y;
             }
         }
+        uint16_t* dst = c.a.out + (int64_t)(w.g.q0 + w.t0 + tok) * c.a.o_t + (int64_t)(at.h * c.group + r % c.group) * c.a.o_h +
+                        at.half * C::kDv + lane * kV;
 #pragma unroll
-        for (int e = 0; e < kV; e += 2)
-            *reinterpret_cast<uint32_t*>(dst + x + lane * kV + e) = pack_bf16(acc[e], acc[e + 1]);
+        for (int e = 0; e < kV; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16(acc[e], acc[e + 1]);
     }
 }
 
@@ -693,23 +750,23 @@ void launch_chunk_dim(const Attn& hd, const AttnCall& a, int few_rows, cudaStrea
     c.tokens = kTile / c.group;
     c.tile_tokens = c.tokens * C::kCtas;
     c.box = std::min(1 << a.pv.page_shift, 64);
+    c.wave = device_sm_count() / C::kCtas;
     // a sequence has at most one tile that is not full
-    const int64_t slots = std::min<int64_t>((int64_t)a.pv.rows / c.tile_tokens + a.pv.n_seqs,
+    const int64_t tiles = std::min<int64_t>((int64_t)a.pv.rows / c.tile_tokens + a.pv.n_seqs,
                                             (int64_t)a.pv.n_seqs * ((a.pv.max_q + c.tile_tokens - 1) / c.tile_tokens));
-    if (slots > 65535) throw Error(G4Q_ERR_INVALID_ARGUMENT, "too many rows for one call");
-    c.slots = (int)slots;
-    const int64_t ctas = slots * a.hk * C::kHalves * C::kCtas;
-    c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, device_sm_count() / ctas));
+    const int64_t ctas = (tiles * a.hk * C::kHalves + c.wave) * C::kCtas;
+    if (ctas > 0x7FFFFFFF) throw Error(G4Q_ERR_INVALID_ARGUMENT, "too many rows for one call");
     c.part_o = hd.part_o;
     c.part_ml = hd.part_ml;
     c.err = device_scratch().err;
     const CUtensorMap tq = rows_map(a.q, a.q_t, a.q_h, a.hq, a.pv.rows, D, c.group, c.tokens);
     const CUtensorMap tk = paged_map(a, a.k, D, c.box), tv = paged_map(a, a.v, D, c.box);
-    launch_dependent<C::kCtas>(attn_chunk_kernel<D>,
-                               dim3((unsigned)(a.hk * C::kHalves * C::kCtas), (unsigned)slots, (unsigned)c.splits), dim3(kThreads),
-                               C::kSmem, st, tq, tk, tv, c);
-    if (c.splits > 1)
-        launch_dependent(attn_chunk_join_kernel<D>, dim3(C::kCtas * kTile / 8, (unsigned)slots, (unsigned)a.hk), dim3(256), 0, st, c);
+    launch_dependent<C::kCtas>(attn_chunk_kernel<D>, dim3((unsigned)ctas), dim3(kThreads), C::kSmem, st, tq, tk, tv, c);
+    // no tile is long enough for two pieces: nothing to join
+    int64_t cap = (int64_t)a.pv.max_pages << a.pv.page_shift;
+    if (a.window > 0) cap = std::min<int64_t>(cap, (int64_t)a.window + c.tile_tokens + c.box);
+    if ((cap + kTile - 1) / kTile >= 2 * kMinPiece)
+        launch_dependent(attn_chunk_join_kernel<D>, dim3(C::kCtas * kTile / kJoinRows, (unsigned)c.wave), dim3(256), 0, st, c);
 }
 
 }  // namespace
