@@ -16,13 +16,14 @@
 // eighth of a bf16 step at most takes part in a rounding that is half a step.
 //
 // Bound by HBM for a prompt's chunk: every element is read and written once (16 query and 8 key heads of 256,
-// 2048 tokens: 50 MB). The instructions come close: with the library's sincospi for every head, and weight, norm
-// and rotation applied one after the other, a head took 305 warp instructions and the kernel 18.7 us, issue-bound
-// at 13 % of DRAM. So one warp takes several heads of one token and of one kind (queries, keys or values), and
-// what they share is folded into two factors per element before the heads are looked at:
+// 2048 tokens: 50 MB, 11.0 us from L2). The instructions come close: with the library's sincospi for every head,
+// and weight, norm and rotation applied one after the other, a head took 305 warp instructions and the kernel
+// 18.7 us, issue-bound at 13 % of DRAM. So a block takes one token, and what the token's heads share is folded
+// into two factors per element before the heads are looked at:
 //   out_i = inv * (x_i * A_i + x_partner * B_i),   A = w_i cos, B = -+ w_partner sin,   inv = 1 / rms(x)
-// A lane has a 16-byte chunk of 8 elements of a head (two at D = 512; two or four heads side by side at D = 128,
-// 64); the partner chunk comes from another lane as it was read, four shuffles.
+// A warp takes heads of one kind (queries, keys or values); a lane has a 16-byte chunk of 8 elements of a head (two at
+// D = 512; two or four heads side by side at D = 128, 64), and the partner chunk comes from another lane as it was
+// read, four shuffles.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -35,7 +36,7 @@
 namespace g4q {
 namespace {
 
-constexpr int kWarps = 8;      // of a block, at most: the heads of one token
+constexpr int kWarps = 16;      // of a block, at most: the heads of one token
 
 __device__ __forceinline__ void unpack8(const uint4& v, float* f) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -80,7 +81,9 @@ __global__ void __launch_bounds__(kWarps * 32) head_rows_kernel(const __grid_con
     release_successor();
     const int lane = threadIdx.x & 31, l = lane % LPH, sub = lane / LPH;
     const int gq = (p.hq + kGroup - 1) / kGroup, gk = (p.hk + kGroup - 1) / kGroup, gv = (p.hv + kGroup - 1) / kGroup;
-    __shared__ float s_cos[256], s_sin[256];
+    // A and B of a query head and of a key head: [kind][A, B][which four of a chunk's eight][chunk][4], so that a
+    // warp's 16-byte reads do not conflict
+    __shared__ float s_f[2][2][2][D / 8][4];
     const int64_t m = blockIdx.x;
     int g = (int)(blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5));
     const bool in_range = g < gq + gk + gv;
@@ -126,39 +129,34 @@ __global__ void __launch_bounds__(kWarps * 32) head_rows_kernel(const __grid_con
         pos = p.positions[m];
     }
 
-    for (int i = threadIdx.x; i < p.rotary / 2; i += blockDim.x) {
-        const uint64_t turn = (uint64_t)(int64_t)pos * p.turns[i];
-        const float angle = (float)(int32_t)(turn >> 32) * 1.4629180792671596e-9f;   // 2 pi * 2^-32
-        s_cos[i] = __cosf(angle);
-        s_sin[i] = __sinf(angle);
-    }
-    __syncthreads();
-    if (!in_range) return;
-
-    // A and B of this lane's elements; chunk c of a head holds elements 8c..8c+7, its partner is chunk c +- off
-    const int off = p.rotary / 16;
-    float fa[NV][8], fb[NV][8];
-    if (!is_v) {
-        const uint16_t* wt = is_q ? p.q_weight : p.k_weight;
+    const int half = p.rotary / 2;
+    auto put = [&](int kind, int i, float fa, float fb) {
+        s_f[kind][0][(i >> 2) & 1][i >> 3][i & 3] = fa;
+        s_f[kind][1][(i >> 2) & 1][i >> 3][i & 3] = fb;
+    };
+    for (int i = threadIdx.x; i < D - half; i += blockDim.x) {
+        float cs = 1.0f, sn = 0.0f;
+        if (i < half) {
+            const uint64_t turn = (uint64_t)(int64_t)pos * p.turns[i];
+            const float angle = (float)(int32_t)(turn >> 32) * 1.4629180792671596e-9f;   // 2 pi * 2^-32
+            cs = __cosf(angle);
+            sn = __sinf(angle);
+        }
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int c = l + j * LPH, pc = c < off ? c + off : c < 2 * off ? c - off : c;
-            uint4 wv = make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u), wp = wv;   // bf16 1.0 pairs
-            if (wt != nullptr) {
-                wv = *reinterpret_cast<const uint4*>(wt + c * 8);
-                wp = *reinterpret_cast<const uint4*>(wt + pc * 8);
-            }
-            unpack8(wv, fa[j]);
-            unpack8(wp, fb[j]);
-            const int pair = 8 * min(c, pc);
-            const float sign = c < off ? -1.0f : 1.0f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                fa[j][e] *= c < 2 * off ? s_cos[pair + e] : 1.0f;
-                fb[j][e] *= c < 2 * off ? sign * s_sin[pair + e] : 0.0f;
+        for (int kind = 0; kind < 2; ++kind) {
+            const uint16_t* wt = kind == 0 ? p.q_weight : p.k_weight;
+            if (i < half) {   // the pair (i, i + half)
+                const float w0 = wt != nullptr ? bf16_bits_to_f32(wt[i]) : 1.0f, w1 = wt != nullptr ? bf16_bits_to_f32(wt[i + half]) : 1.0f;
+                put(kind, i, w0 * cs, -w1 * sn);
+                put(kind, i + half, w1 * cs, w0 * sn);
+            } else if (i + half >= p.rotary) {   // an element that is not rotated
+                put(kind, i + half, wt != nullptr ? bf16_bits_to_f32(wt[i + half]) : 1.0f, 0.0f);
             }
         }
     }
+    __syncthreads();
+    if (!in_range) return;
+    const int off = p.rotary / 16, kind = is_q ? 0 : 1;   // chunk c of a head holds 8c..8c+7, its partner is chunk c +- off
 
 #pragma unroll
     for (int i = 0; i < IPW; ++i) {
@@ -202,11 +200,12 @@ __global__ void __launch_bounds__(kWarps * 32) head_rows_kernel(const __grid_con
                 float y[8];
                 unpack8(other[j], y);
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const F2 r = fma2({y[e], y[e + 1]}, {fb[j][e], fb[j][e + 1]},
-                                      mul2({x[j][e], x[j][e + 1]}, {fa[j][e], fa[j][e + 1]}));
-                    x[j][e] = r.x;
-                    x[j][e + 1] = r.y;
+                for (int q = 0; q < 2; ++q) {
+                    const float4 fa = *reinterpret_cast<const float4*>(s_f[kind][0][q][l + j * LPH]);
+                    const float4 fb = *reinterpret_cast<const float4*>(s_f[kind][1][q][l + j * LPH]);
+                    const F2 r0 = fma2({y[4 * q], y[4 * q + 1]}, {fb.x, fb.y}, mul2({x[j][4 * q], x[j][4 * q + 1]}, {fa.x, fa.y}));
+                    const F2 r1 = fma2({y[4 * q + 2], y[4 * q + 3]}, {fb.z, fb.w}, mul2({x[j][4 * q + 2], x[j][4 * q + 3]}, {fa.z, fa.w}));
+                    x[j][4 * q] = r0.x, x[j][4 * q + 1] = r0.y, x[j][4 * q + 2] = r1.x, x[j][4 * q + 3] = r1.y;
                 }
             }
         }
@@ -243,15 +242,16 @@ void launch_one(const HeadRowsCall& c, cudaStream_t st) {
 
 template <int D>
 void launch_dim(const HeadRowsCall& c, bool append, cudaStream_t st) {
-    // One head per warp keeps a single token's latency low; with more rows than fill the GPU a warp takes four,
-    // so what the heads share is computed once for them (24 heads of 256, 2048 tokens: two heads 14.8 us, four
-    // 12.2, eight 12.7, before the sines moved to the block).
+    // One head per warp keeps a single token's latency low; with more rows than fill the GPU a warp takes several, so
+    // fewer warps pass through (24 heads of 256, 2048 tokens: one head 13.7 us, two 11.9, four 11.0; 18 heads of 512:
+    // one 21.2, two 17.7, four 27.3, whose registers leave too few warps to cover the loads).
+    constexpr int kWide = D > 256 ? 2 : 4;
     const int heads = c.hq + c.hk + c.hv;
     const bool wide = c.rows * heads >= (int64_t)device_sm_count() * 64;
     if (append)
-        wide ? launch_one<D, 4, true>(c, st) : launch_one<D, 1, true>(c, st);
+        wide ? launch_one<D, kWide, true>(c, st) : launch_one<D, 1, true>(c, st);
     else
-        wide ? launch_one<D, 4, false>(c, st) : launch_one<D, 1, false>(c, st);
+        wide ? launch_one<D, kWide, false>(c, st) : launch_one<D, 1, false>(c, st);
 }
 
 }  // namespace
