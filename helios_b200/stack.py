@@ -27,8 +27,10 @@ from typing import List, Optional
 
 import torch
 
+from .attention import PagedAttention, PagedBatch, PagedKVCache, Rope, kv_append
 from .quantized import (PHASE_ALLREDUCE, PHASE_ARGMAX, PHASE_GEGLU, QMM_RMS_SCALE, DecodePlan, QuantizedWeight,
-                        lm_head_argmax, quantized_matmul, synth_matrix, synth_normal)
+                        lm_head_argmax, quantized_matmul, quantized_matmul_geglu, rms_norm, rms_norm_residual,
+                        synth_matrix, synth_normal)
 
 BASE_SEED = 0x48454C494F53
 PROJ_IDS = {"q": 0, "k": 1, "v": 2, "o": 3, "gate": 4, "up": 5, "down": 6, "lm": 7}
@@ -366,8 +368,8 @@ def norm_weight(seed: int, n: int, device=None) -> torch.Tensor:
 
 class DecoderStack:
     """Seeded synthetic weights with the real decoder layer's structure around the quantized linears
-    (layer_forward, native_model.cc:899-970, attention left out: q stands in for its output, as in
-    SyntheticStack): per layer q|k|v, o, a paired gate|up weight whose phase applies the GeGLU, down,
+    (layer_forward, native_model.cc:899-970; in the decode plan attention is left out: q stands in for its
+    output, as in SyntheticStack; :meth:`forward` runs the layers with their attention as separate launches): per layer q|k|v, o, a paired gate|up weight whose phase applies the GeGLU, down,
     the four RMSNorm weights (input, post-attention, pre-feed-forward, post-feed-forward) and the
     layer scalar, then the final norm and the LM head. ``build_plan`` makes the whole step ONE decode
     plan with the norms, residual adds and scalars as phase prologues:
@@ -481,6 +483,56 @@ class DecoderStack:
                       values=self.values[:M], keys=self.keys[:M], logits=logits)
         return self.keys[:M]
 
+    def attach_attention(self, n_pages: int, page_size: int = 64, *, head_dim: int = 256, window: int = 1024,
+                         scale: Optional[float] = None, base: float = 10000.0, rotary_dim: Optional[int] = None) -> None:
+        """Give every layer a paged key/value cache of ``n_pages`` pages and seeded query and key norm weights,
+        for :meth:`forward`. ``window``: of the sliding-window layers (0: none); ``scale``: of the scores
+        (default ``head_dim ** -0.5``)."""
+        if self.size != 1:
+            raise ValueError("attention in the stack runs on one GPU")
+        if self.nq % head_dim or self.nkv % head_dim:
+            raise ValueError("q_out and kv_out must be whole heads")
+        self.head_dim, self.window, self.scale = head_dim, window, scale
+        hq, hk = self.nq // head_dim, self.nkv // head_dim
+        self.rope = Rope(head_dim, base, rotary_dim=rotary_dim)
+        self.attend = PagedAttention(hq, hk, head_dim)
+        for i, L in enumerate(self.layers):
+            s = BASE_SEED ^ 0xB000 ^ (i * 8)
+            L["q_norm"], L["k_norm"] = norm_weight(s, head_dim), norm_weight(s + 1, head_dim)
+            L["cache"] = PagedKVCache.allocate(n_pages, page_size, hk, head_dim)
+
+    def forward(self, h: torch.Tensor, batch: PagedBatch, *, rows: Optional[torch.Tensor] = None,
+                keep: Optional[list] = None):
+        """One step of real decoder layers with their attention (layer_forward with attention_forward,
+        native_model.cc:788-970): the new tokens h [tokens, hidden] of ``batch``'s sequences (a prompt's chunk,
+        one decoded token each, drafted blocks, or a mix) go through every layer, and their keys and values
+        into the layers' caches (:meth:`attach_attention`). ``rows``: the rows whose greedy token is wanted
+        (int64 index tensor). Returns (keys of those rows or None, the residual stream after the last layer).
+        ``keep``: a list that receives every layer's qkv, q (normed, rotated) and attention output."""
+        c, d = self.cfg, self.head_dim
+        M = h.shape[0]
+        res = h
+        for i, L in enumerate(self.layers):
+            qkv = quantized_matmul(rms_norm(res, L["in_norm"], c.eps), L["qkv"])
+            q, k, v = (t.unflatten(1, (-1, d)) for t in qkv.split((self.nq, self.nkv, self.nkv), 1))
+            q = kv_append(q, k, v, L["cache"], batch, self.rope, L["q_norm"], L["k_norm"], eps=c.eps)
+            # the last partly filled block of a padded step belongs to no sequence: zeros, not what memory held
+            out = torch.zeros_like(q)
+            attn = self.attend(q, L["cache"], batch, scale=self.scale, window=self.window, out=out)
+            if keep is not None:
+                keep.append({"qkv": qkv, "q": q, "attn": attn})
+            o = quantized_matmul(attn.flatten(1), L["o"])
+            res = rms_norm_residual(o, L["post_attn"], res, eps=c.eps)
+            x = rms_norm(res, L["pre_ffn"], c.eps)
+            y = torch.empty((M, L["gu"].rows), dtype=torch.bfloat16, device=h.device) if 9 <= M <= 16 else None
+            down = quantized_matmul(quantized_matmul_geglu(x, L["gu"], y=y), L["down"])
+            res = rms_norm_residual(down, L["post_ffn"], res, L["scalar"], c.eps)
+        if rows is None:
+            return None, res
+        last = rms_norm(res[rows], self.final_norm, c.eps)
+        keys = [lm_head_argmax(x, self.lm, softcap=c.softcap, row_offset=self.v_rows[0])[2] for x in last.split(16)]
+        return torch.cat(keys), res
+
     def local_weight_bytes(self) -> int:
         mats = [w for L in self.layers for k, w in L.items() if k in ("qkv", "o", "gu", "down")] + [self.lm]
         return sum(w.rows * w.cols * 9 // 16 for w in mats)
@@ -493,6 +545,9 @@ class DecoderStack:
             for k in ("qkv", "o", "gu", "down"):
                 L[k].free()
         self.lm.free()
+        if getattr(self, "attend", None) is not None:
+            self.attend.free()
+            self.rope.free()
 
 
 def decode_keys(keys: torch.Tensor):

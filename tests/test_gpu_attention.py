@@ -466,3 +466,46 @@ def test_side_stream_and_empty_step(cuda):
     s.t_off.zero_()
     assert attend(empty, s.cache, s.batch).shape == (0, 4, 64)
     no_device_error()
+
+
+# ---- the operators together, in the layers that call them ------------------------------------------------
+
+@pytest.mark.parametrize("hq,hk,d,window", [(4, 2, 64, 40), (2, 1, 256, 0)])
+def test_decoder_stack_forward(cuda, hq, hk, d, window):
+    """Prompts in chunks, drafted blocks and single tokens of three sequences through two real decoder layers: in
+    every layer and step, the queries, the cache and the attention output against the 64-bit forms on the GPU's own
+    q|k|v."""
+    from helios_b200 import attention as A
+    from helios_b200.quantized import synth_normal
+    from helios_b200.stack import DecoderStack, StackConfig
+    cfg = StackConfig(layers=2, hidden=512, q_out=hq * d, kv_out=hk * d, inter=1024, vocab=2048)
+    st = DecoderStack(cfg)
+    st.attach_attention(40, 16, head_dim=d, window=window)
+    table = torch.randperm(39, generator=torch.Generator().manual_seed(3))[:36].reshape(3, 12).to(torch.int32)
+    f = freqs(d, 10000.0)
+    have = [0, 0, 0]
+    for q_lens in ([70, 9, 0], [33, 1, 150], [1, 1, 1], [5, 5, 5], [1, 0, 1]):
+        have = [a + b for a, b in zip(have, q_lens)]
+        off = [sum(q_lens[:b]) for b in range(4)]
+        n = off[-1]
+        batch = A.PagedBatch(torch.tensor(off, dtype=torch.int32, device="cuda"),
+                             torch.tensor(have, dtype=torch.int32, device="cuda"), table.cuda(), max_q=max(q_lens))
+        h = synth_normal(100 + n, (n, cfg.hidden))
+        keep = []
+        rows = torch.tensor([o - 1 for o, q in zip(off[1:], q_lens) if q], device="cuda")
+        keys, res = st.forward(h, batch, rows=rows, keep=keep)
+        no_device_error()
+        assert keys.shape == (len(rows),) and torch.isfinite(res).all()
+        toks = R.tokens(off, have)
+        pos = torch.tensor([t[2] for t in toks])
+        page_id, slot = torch.tensor([int(table[b, p // 16]) for _, b, p in toks]), pos % 16
+        for L, kept in zip(st.layers, keep):
+            qkv = kept["qkv"].cpu()
+            q, k, v = (t.unflatten(1, (-1, d)) for t in qkv.split((hq * d, hk * d, hk * d), 1))
+            kc, vc = L["cache"].k.cpu(), L["cache"].v.cpu()
+            close(kept["q"], *R.norm_rope(q, pos, f, d, L["q_norm"].cpu(), cfg.eps))
+            close(kc[page_id, :, slot], *R.norm_rope(k, pos, f, d, L["k_norm"].cpu(), cfg.eps))
+            want = R.norm(v, None, cfg.eps)
+            close(vc[page_id, :, slot], want, R.half_step(want) + 2.0 ** -19 * want.abs())
+            close(kept["attn"], *R.attention(kept["q"].cpu(), kc, vc, off, have, table.tolist(), d ** -0.5, window))
+    st.free()
