@@ -117,6 +117,50 @@ struct Cursor {
     }
 };
 
+// This CTA's first tile, and how many it has. Every warp finds it by itself: handing it over through shared memory
+// costs a barrier and another round of loads at the start, where nothing else can run.
+__device__ __forceinline__ Cursor first_place(const FewCall& c, int lane, int& left) {
+    auto work_of = [&](int b) {
+        SeqWork w;
+        w.g.q0 = w.g.q_len = w.g.first = w.g.kv_len = w.lo = w.nt = 0;
+        if (b < c.a.pv.n_seqs) w = seq_work(c, b);
+        return w;
+    };
+    SeqWork w = work_of(lane);                       // the first 32 sequences stay in registers
+    uint32_t inc = warp_scan(w.nt * c.a.hk, lane), total = __shfl_sync(0xFFFFFFFFu, inc, 31);
+    for (int b0 = 32; b0 < c.a.pv.n_seqs; b0 += 32)
+        total += __shfl_sync(0xFFFFFFFFu, warp_scan(work_of(b0 + lane).nt * c.a.hk, lane), 31);
+    const Ranges ranges(total, c.ctas);
+    const uint32_t t0 = ranges.first(blockIdx.x);
+    Cursor cur;
+    cur.b = cur.h = cur.t = 0;
+    left = (int)(ranges.first(blockIdx.x + 1) - t0);
+    uint32_t before = 0;
+    for (int b0 = 0; b0 < c.a.pv.n_seqs && left > 0; b0 += 32) {
+        if (b0 > 0) {
+            w = work_of(b0 + lane);
+            inc = warp_scan(w.nt * c.a.hk, lane);
+        }
+        const unsigned past = __ballot_sync(0xFFFFFFFFu, before + inc > t0);
+        if (past != 0) {
+            const int at = __ffs(past) - 1;
+            cur.b = b0 + at;
+            cur.w.g.q0 = __shfl_sync(0xFFFFFFFFu, w.g.q0, at);
+            cur.w.g.q_len = __shfl_sync(0xFFFFFFFFu, w.g.q_len, at);
+            cur.w.g.first = __shfl_sync(0xFFFFFFFFu, w.g.first, at);
+            cur.w.g.kv_len = __shfl_sync(0xFFFFFFFFu, w.g.kv_len, at);
+            cur.w.lo = __shfl_sync(0xFFFFFFFFu, w.lo, at);
+            cur.w.nt = __shfl_sync(0xFFFFFFFFu, w.nt, at);
+            const uint32_t rest = t0 - (before + __shfl_sync(0xFFFFFFFFu, inc, at) - (uint32_t)cur.w.nt * c.a.hk);
+            cur.h = (int)(rest / (uint32_t)cur.w.nt);
+            cur.t = (int)(rest % (uint32_t)cur.w.nt);
+            break;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, inc, 31);
+    }
+    return cur;
+}
+
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
@@ -135,7 +179,6 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
                     const __grid_constant__ FewCall c) {
     using C = FewCfg<D, MT>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ int start[4];                 // b, h, t of this CTA's first tile, and its tiles
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_addr(smem_raw));
     const uint32_t s_ring = base;
@@ -150,56 +193,21 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
     auto empty = [&](int s) { return s_bar + 8u * (C::kStages + s); };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    wait_for_predecessor();
-    release_successor();
-    if (warp == kComputeWarps) {
-        // this CTA's range of tiles and the place of its first one; the first 32 sequences stay in registers
-        const int nt0 = lane < c.a.pv.n_seqs ? seq_work(c, lane).nt : 0;
-        const uint32_t scan0 = warp_scan(nt0 * c.a.hk, lane);
-        uint32_t total = __shfl_sync(0xFFFFFFFFu, scan0, 31);
-        for (int b0 = 32; b0 < c.a.pv.n_seqs; b0 += 32) {
-            const int nt = b0 + lane < c.a.pv.n_seqs ? seq_work(c, b0 + lane).nt : 0;
-            total += __shfl_sync(0xFFFFFFFFu, warp_scan(nt * c.a.hk, lane), 31);
+    if (threadIdx.x == kComputeWarps * 32) {
+        for (int s = 0; s < C::kStages; ++s) {
+            bar_init(full(s), 1);
+            bar_init(empty(s), 1);
         }
-        const Ranges ranges(total, c.ctas);
-        const uint32_t t0 = ranges.first(blockIdx.x), t1 = ranges.first(blockIdx.x + 1);
-        uint32_t before = 0;
-        int found = -1;
-        for (int b0 = 0; b0 < c.a.pv.n_seqs && found < 0 && t1 > t0; b0 += 32) {
-            const int nt = b0 == 0 ? nt0 : b0 + lane < c.a.pv.n_seqs ? seq_work(c, b0 + lane).nt : 0;
-            const uint32_t inc = b0 == 0 ? scan0 : warp_scan(nt * c.a.hk, lane);
-            const unsigned past = __ballot_sync(0xFFFFFFFFu, before + inc > t0);
-            if (past != 0) {
-                const int at = __ffs(past) - 1;
-                const uint32_t end = __shfl_sync(0xFFFFFFFFu, inc, at), n = __shfl_sync(0xFFFFFFFFu, nt, at);
-                found = b0 + at;
-                const uint32_t rest = t0 - (before + end - n * c.a.hk);
-                if (lane == 0) {
-                    start[0] = found;
-                    start[1] = (int)(rest / n);
-                    start[2] = (int)(rest % n);
-                }
-            }
-            before += __shfl_sync(0xFFFFFFFFu, inc, 31);
-        }
-        if (lane == 0) {
-            start[3] = found < 0 ? 0 : (int)(t1 - t0);
-            for (int s = 0; s < C::kStages; ++s) {
-                bar_init(full(s), 1);
-                bar_init(empty(s), 1);
-            }
-            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
     }
     __syncthreads();
-    int left = start[3];
-    Cursor cur;
-    cur.b = start[0];
-    cur.h = start[1];
-    cur.t = start[2];
+    wait_for_predecessor();
+    release_successor();
+    int left;
+    Cursor cur = first_place(c, lane, left);
     if (left > 0) {
-        cur.w = seq_work(c, cur.b);
-
         if (warp == kComputeWarps) {
             // ---------------- producer: K then V of every tile, in ring order
             int stage = 0;
@@ -251,15 +259,23 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
                 const int rows = g.q_len * c.group;
                 const int n = min(left, cur.w.nt - cur.t);
                 const bool whole = n == cur.w.nt, first_part = cur.t > 0;
-                for (int i = threadIdx.x; i < C::kRows * (D / 8); i += 256) {
-                    const int r = i / (D / 8), ch = i % (D / 8);
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (r < rows) {
+                constexpr int kPieces = C::kRows * (D / 8), kLoads = (kPieces + 255) / 256;
+                uint4 qv[kLoads];
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    const int r = (threadIdx.x + i * 256) / (D / 8), ch = (threadIdx.x + i * 256) % (D / 8);
+                    qv[i] = make_uint4(0, 0, 0, 0);
+                    if (r < rows) {      // rows <= kRows
                         const int tok = r / c.group, hd = cur.h * c.group + r % c.group;
-                        v = *reinterpret_cast<const uint4*>(c.a.q + (int64_t)(g.q0 + tok) * c.a.q_t + (int64_t)hd * c.a.q_h + ch * 8);
+                        qv[i] = *reinterpret_cast<const uint4*>(c.a.q + (int64_t)(g.q0 + tok) * c.a.q_t + (int64_t)hd * c.a.q_h + ch * 8);
                     }
-                    *reinterpret_cast<uint4*>(gen + (s_q - base) + (ch >> 3) * (C::kRows * 128) + r * 128 +
-                                              (((ch & 7) ^ (r & 7)) << 4)) = v;
+                }
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    const int r = (threadIdx.x + i * 256) / (D / 8), ch = (threadIdx.x + i * 256) % (D / 8);
+                    if (kPieces % 256 == 0 || r < C::kRows)
+                        *reinterpret_cast<uint4*>(gen + (s_q - base) + (ch >> 3) * (C::kRows * 128) + r * 128 +
+                                                  (((ch & 7) ^ (r & 7)) << 4)) = qv[i];
                 }
                 // keys a row sees: [vis_lo, vis_hi)
                 int vis_lo = 0, vis_hi = 0;
@@ -282,11 +298,12 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
                 for (int it = 0; it < n; ++it) {
                     const int k0 = cur.w.lo + (cur.t + it) * kKeys;
                     // ---- scores of keys 8w..8w+7
-                    float s[MT][4];
+                    // two sums per score, of the even and the odd products: half the chain of dependent MMAs
+                    float s[MT][2][4];
 #pragma unroll
                     for (int a = 0; a < MT; ++a)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[a][e] = 0.0f;
+                        for (int e = 0; e < 8; ++e) s[a][e >> 2][e & 3] = 0.0f;
                     int st = stage;
                     uint32_t rd = round;
 #pragma unroll
@@ -307,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
                                     uint32_t a0, a1, a2, a3;
                                     ldmatrix4(s_q + (qc >> 3) * (C::kRows * 128) + qr * 128 + (((qc & 7) ^ (qr & 7)) << 4),
                                               a0, a1, a2, a3);
-                                    mma_bf16_16816(s[a], a0, a1, a2, a3, half ? b2 : b0, half ? b3 : b1);
+                                    mma_bf16_16816(s[a][half], a0, a1, a2, a3, half ? b2 : b0, half ? b3 : b1);
                                 }
                             }
                         }
@@ -316,8 +333,9 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
 #pragma unroll
                     for (int a = 0; a < MT; ++a) {
                         float* sr = s_s + (16 * a + gi) * C::kSLd + 8 * warp + 2 * t4;
-                        *reinterpret_cast<float2*>(sr) = make_float2(s[a][0], s[a][1]);
-                        *reinterpret_cast<float2*>(sr + 8 * C::kSLd) = make_float2(s[a][2], s[a][3]);
+                        *reinterpret_cast<float2*>(sr) = make_float2(s[a][0][0] + s[a][1][0], s[a][0][1] + s[a][1][1]);
+                        *reinterpret_cast<float2*>(sr + 8 * C::kSLd) =
+                            make_float2(s[a][0][2] + s[a][1][2], s[a][0][3] + s[a][1][3]);
                     }
                     compute_sync();
                     // every warp is past this tile's K and the previous tile's V
