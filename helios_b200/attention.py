@@ -155,7 +155,7 @@ class PagedKVCache:
 
 class PagedBatch:
     """The sequences of one step. int32 CUDA tensors, read on the device when the kernels run (a captured
-    graph replays with what they hold then): ``q_offsets`` [n + 1], sequence b's new tokens are the rows
+    graph replays with what they hold then; change them in place): ``q_offsets`` [n + 1], sequence b's new tokens are the rows
     q_offsets[b] .. q_offsets[b + 1]; ``kv_lens`` [n], its tokens in the cache with the new ones, which are
     the last; ``block_table`` [n, max_pages], position j is in page block_table[b, j // page_size]. ``max_q``:
     at least the longest sequence's new tokens. ``max_kv``: at least the longest kv_len where the caller
@@ -175,8 +175,8 @@ class PagedBatch:
         self.device = kv_lens.get_device()
         if q_offsets.get_device() != self.device or block_table.get_device() != self.device:
             raise ValueError("q_offsets, kv_lens and block_table must be on one device")
-        if max_q < 1 or (max_kv is not None and max_kv < 1):
-            raise ValueError("max_q and max_kv must be >= 1")
+        if not 1 <= max_q < 2 ** 31 or (max_kv is not None and max_kv < 1):
+            raise ValueError("max_q and max_kv must be >= 1 (and max_q below 2^31)")
         self.max_q, self.max_kv = max_q, max_kv
         self._views = {}
 
@@ -226,7 +226,7 @@ def kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cache
     """The new tokens of a step, at their positions: keys normalized, weighted and rotated into the cache's
     pages, values normalized (without a weight; ``norm_values=False`` stores them as they are) beside them,
     and the queries, treated like the keys with ``q_weight``, returned (None for q None). One launch. ``v``
-    may be ``k``. Rows that belong to no sequence are left as they were (in ``q_out`` too)."""
+    may be ``k``. Sequences may share pages of a common prefix, but no two may append to one slot. Rows that belong to no sequence are left as they were (in ``q_out`` too)."""
     d, dev = rope.head_dim, rope.device
     _same_device(dev, cache=cache, batch=batch)
     ck = _head_rows(k, d, dev, "k")
@@ -269,10 +269,13 @@ class PagedAttention:
         """``softmax(scale * q k^T + mask) v``: q [tokens, q_heads, head_dim] as :func:`kv_append` returns it;
         the query at position t sees the keys j <= t, and j > t - window when window > 0. ``scale`` defaults
         to ``head_dim ** -0.5``. Single tokens, drafted blocks and prompt chunks may be mixed. A row that sees
-        no key is zero; rows that belong to no sequence are left as they were (in ``out``)."""
+        no key is zero; rows that belong to no sequence are left as they were (in ``out``, which must not overlap
+        q)."""
         d, dev = self.head_dim, self.device
         _same_device(dev, cache=cache, batch=batch)
         cq = _head_rows(q, d, dev, "q")
+        if not 0 <= window < 2 ** 31:
+            raise ValueError("window must be >= 0 (0: none) and below 2^31")
         out, co = _output(q, cq.n_heads, d, dev, out, "out")
         _lib.call("g4q_paged_attention", self.handle, cq, q.shape[0], cache.c, batch.view(cache.page_size),
                   d ** -0.5 if scale is None else scale, window, co, _raw_stream(dev))

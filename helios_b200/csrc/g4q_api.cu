@@ -1240,6 +1240,9 @@ G4qStatus g4q_paged_attention(const G4qAttn* attn, const G4qHeadRows* q, int64_t
         check_heads(out, a->head_dim, "out");
         require(q->n_heads == a->hq && out->n_heads == a->hq, G4Q_ERR_INVALID_ARGUMENT,
                 "q and out must have the handle's query heads");
+        require(M == 1 || q->token_stride >= a->head_dim, G4Q_ERR_INVALID_ARGUMENT, "q.token_stride must be >= head_dim");
+        // several CTAs read a query row, and one may write its result before another has read it
+        require(out->data != q->data, G4Q_ERR_INVALID_ARGUMENT, "out must not be q");
         AttnCall c = {};
         c.q = q->data, c.q_t = q->token_stride, c.q_h = q->head_stride;
         c.out = out->data, c.o_t = out->token_stride, c.o_h = out->head_stride;
@@ -1247,7 +1250,8 @@ G4qStatus g4q_paged_attention(const G4qAttn* attn, const G4qHeadRows* q, int64_t
         c.page_stride = cache->page_stride, c.head_stride = cache->head_stride, c.slot_stride = cache->slot_stride;
         c.hq = a->hq, c.hk = a->hk;
         c.scale = scale;
-        c.window = window;
+        // a window as long as the table hides nothing
+        c.window = window >= ((int64_t)pv.max_pages << pv.page_shift) ? 0 : window;
         c.pv = pv;
         launch_attention(*a, c, reinterpret_cast<cudaStream_t>(stream));
     });

@@ -81,6 +81,7 @@ struct ChunkCall {
 
 // A tile of work: rows of sequence b, key head, half of the output columns, and the piece of its keys.
 struct Work {
+    SeqGeom g;
     int b, tile, h, half;
     int piece, pieces;   // of the keys
     int slot;            // place of the piece's partial
@@ -93,50 +94,13 @@ struct TileWork {
     int any_lo, any_hi;  // keys that some row of the tile sees
 };
 
-__device__ __forceinline__ int tiles_of(const ChunkCall& c, int b) {
-    const SeqGeom g = seq_geom(c.a.pv, b);
+__device__ __forceinline__ int tiles_of(const ChunkCall& c, const SeqGeom& g) {
     return g.q_len * c.group > c.few_rows ? (g.q_len + c.tile_tokens - 1) / c.tile_tokens : 0;
 }
 
-// The sequence and place of the t-th row tile of the batch (t < total), found by one warp. The longest come first:
-// a sequence's last tile, and up to 32 sequences by their lengths (more: the batch's last first).
-__device__ __forceinline__ int2 find_tile(const ChunkCall& c, int t, int total, int lane) {
-    if (c.a.pv.n_seqs <= 32) {
-        const int nt = lane < c.a.pv.n_seqs ? tiles_of(c, lane) : 0, kv = lane < c.a.pv.n_seqs ? c.a.pv.kv_lens[lane] : -1;
-        int before = 0;
-        for (int o = 0; o < c.a.pv.n_seqs; ++o) {
-            const int kv_o = __shfl_sync(0xFFFFFFFFu, kv, o), nt_o = __shfl_sync(0xFFFFFFFFu, nt, o);
-            if (kv_o > kv || (kv_o == kv && o < lane)) before += nt_o;
-        }
-        const unsigned here = __ballot_sync(0xFFFFFFFFu, t >= before && t < before + nt);
-        const int at = here != 0 ? __ffs(here) - 1 : 0;
-        const int first = __shfl_sync(0xFFFFFFFFu, before, at), n = __shfl_sync(0xFFFFFFFFu, nt, at);
-        return here != 0 ? make_int2(at, n - 1 - (t - first)) : make_int2(-1, 0);
-    }
-    t = total - 1 - t;
-    int before = 0;
-    for (int b0 = 0; b0 < c.a.pv.n_seqs; b0 += 32) {
-        const int nt = b0 + lane < c.a.pv.n_seqs ? tiles_of(c, b0 + lane) : 0;
-        int inc = nt;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-            if (lane >= o) inc += v;
-        }
-        const unsigned past = __ballot_sync(0xFFFFFFFFu, before + inc > t);
-        if (past != 0) {
-            const int at = __ffs(past) - 1;
-            const int end = __shfl_sync(0xFFFFFFFFu, inc, at), n = __shfl_sync(0xFFFFFFFFu, nt, at);
-            return make_int2(b0 + at, t - (before + end - n));
-        }
-        before += __shfl_sync(0xFFFFFFFFu, inc, 31);
-    }
-    return make_int2(-1, 0);
-}
-
-__device__ __forceinline__ TileWork tile_work(const ChunkCall& c, int b, int tile) {
+__device__ __forceinline__ TileWork tile_work(const ChunkCall& c, const SeqGeom& g, int tile) {
     TileWork w;
-    w.g = seq_geom(c.a.pv, b);
+    w.g = g;
     w.t0 = tile * c.tile_tokens;
     const int last = w.g.first + min(w.t0 + c.tile_tokens, w.g.q_len) - 1;
     w.any_hi = min(max(last + 1, 0), w.g.kv_len);
@@ -147,14 +111,23 @@ __device__ __forceinline__ TileWork tile_work(const ChunkCall& c, int b, int til
 }
 
 // The work of the index-th CTA (pair) of the launch, or of the index-th tile of the last wave (kLast); b < 0: none.
-// One warp. Tiles of the whole waves come first, each one CTA pair's; then every tile of the rest `cuts` times.
+// One warp. Tiles of the whole waves come first, each one CTA pair's; then the rest's first pieces, second pieces
+// and so on. The longest tiles come first: a sequence's last one, and up to 32 sequences by their lengths (more: the
+// batch's last first).
 template <int D, bool kLast>
 __device__ __forceinline__ Work find_work(const ChunkCall& c, int index, int lane) {
     constexpr int kHalves = ChunkCfg<D>::kHalves;
+    const int n_seqs = c.a.pv.n_seqs;
+    auto geom_of = [&](int b) {
+        SeqGeom g;
+        g.q0 = g.q_len = g.first = g.kv_len = 0;
+        return b < n_seqs ? seq_geom(c.a.pv, b) : g;
+    };
     Work w;
     w.b = -1;
-    int total = 0;
-    for (int b = lane; b < c.a.pv.n_seqs; b += 32) total += tiles_of(c, b);
+    SeqGeom g = geom_of(lane);                   // the first 32 sequences stay in registers
+    int nt = tiles_of(c, g), total = nt;
+    for (int b = lane + 32; b < n_seqs; b += 32) total += tiles_of(c, seq_geom(c.a.pv, b));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
     const int per_tile = c.a.hk * kHalves, items = total * per_tile;
@@ -164,19 +137,55 @@ __device__ __forceinline__ Work find_work(const ChunkCall& c, int index, int lan
     if (kLast) {
         if (index >= rest) return w;
         item = whole + index;
-    } else if (index >= whole) {
-        item = whole + (index - whole) / cuts;
-        piece = (index - whole) % cuts;
+    } else if (index >= whole && rest > 0) {
+        item = whole + (index - whole) % rest;
+        piece = (index - whole) / rest;
     }
-    if (item >= items) return w;
-    const int2 at = find_tile(c, item / per_tile, total, lane);
-    w.tile = at.y;
+    if (item >= items || piece >= cuts) return w;
+    int t = item / per_tile, at = 0;
+    if (n_seqs <= 32) {
+        int before = 0;                          // tiles of the sequences that come before this lane's
+        for (int o = 0; o < n_seqs; ++o) {
+            const int kv_o = __shfl_sync(0xFFFFFFFFu, g.kv_len, o), nt_o = __shfl_sync(0xFFFFFFFFu, nt, o);
+            if (kv_o > g.kv_len || (kv_o == g.kv_len && o < lane)) before += nt_o;
+        }
+        at = __ffs(__ballot_sync(0xFFFFFFFFu, t >= before && t < before + nt)) - 1;
+        t -= __shfl_sync(0xFFFFFFFFu, before, at);
+        w.tile = __shfl_sync(0xFFFFFFFFu, nt, at) - 1 - t;
+        w.b = at;
+    } else {
+        t = total - 1 - t;
+        int before = 0;
+        for (int b0 = 0;; b0 += 32) {            // t < total: ends
+            g = geom_of(b0 + lane);
+            nt = tiles_of(c, g);
+            int inc = nt;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+                if (lane >= o) inc += v;
+            }
+            const unsigned past = __ballot_sync(0xFFFFFFFFu, before + inc > t);
+            if (past != 0) {
+                at = __ffs(past) - 1;
+                w.tile = t - (before + __shfl_sync(0xFFFFFFFFu, inc - nt, at));
+                w.b = b0 + at;
+                break;
+            }
+            before += __shfl_sync(0xFFFFFFFFu, inc, 31);
+            if (b0 + 32 >= n_seqs) return w;     // the lengths changed while they were read
+        }
+    }
+    w.g.q0 = __shfl_sync(0xFFFFFFFFu, g.q0, at);
+    w.g.q_len = __shfl_sync(0xFFFFFFFFu, g.q_len, at);
+    w.g.first = __shfl_sync(0xFFFFFFFFu, g.first, at);
+    w.g.kv_len = __shfl_sync(0xFFFFFFFFu, g.kv_len, at);
     w.h = item % per_tile / kHalves;
     w.half = item % kHalves;
-    w.pieces = item < whole ? 1 : max(1, min(cuts, tile_work(c, at.x, at.y).n / kMinPiece));
+    w.pieces = item < whole ? 1 : max(1, min(cuts, tile_work(c, w.g, w.tile).n / kMinPiece));
     w.piece = piece;
     w.slot = (item - whole) * cuts + piece;
-    if (piece < w.pieces) w.b = at.x;
+    if (piece >= w.pieces) w.b = -1;
     return w;
 }
 
@@ -395,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int h = at.h, half = at.half;
 
     if (at.b >= 0) {
-        const TileWork w = tile_work(c, at.b, at.tile);
+        const TileWork w = tile_work(c, at.g, at.tile);
         const int t0 = w.t0 + rank * c.tokens;       // this CTA's first token
         // this piece's key tiles
         const int j0 = w.n * at.piece / at.pieces, n = w.n * (at.piece + 1) / at.pieces - j0;
@@ -696,7 +705,7 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_const
     release_successor();
     const Work at = find_work<D, true>(c, blockIdx.y, lane);
     if (at.b < 0 || at.pieces == 1) return;
-    const TileWork w = tile_work(c, at.b, at.tile);
+    const TileWork w = tile_work(c, at.g, at.tile);
     for (int i = 0; i < kJoinRows; i += 8) {
         const int row = blockIdx.x * kJoinRows + i + warp, r = row % kTile;
         const int tok = row / kTile * c.tokens + r / c.group;

@@ -309,7 +309,8 @@ typedef struct G4qPagedCache {
 /* The sequences of one step (device arrays of int32, read by the kernels, so a captured graph replays with
  * what they hold then): sequence b owns the rows [q_offsets[b], q_offsets[b+1]) of the step's M new tokens,
  * which are the last ones of its kv_lens[b] tokens (the new ones included); its position j is in page
- * block_table[b * table_stride + j / page_size] at slot j % page_size. Table entries of pages without a token
+ * block_table[b * table_stride + j / page_size] at slot j % page_size. Sequences may share pages (a common
+ * prefix), but no two may append to one slot. Table entries of pages without a token
  * to read or write are not looked at. max_q: at least the longest q_offsets[b+1] - q_offsets[b]. Rows before
  * q_offsets[0] or behind q_offsets[n_seqs] belong to no sequence and are left as they were. What the arrays
  * hold is checked on the device: nothing outside of the cache, the table or the rows is touched, and
@@ -352,7 +353,7 @@ G4qStatus g4q_kv_append(const G4qRope* rope, const G4qHeadRows* q, const G4qHead
 
 /* out = softmax(scale * q . k^T) v over the cache, query head h against key head h / (n_q_heads / n_kv_heads);
  * the query at position t sees the keys j <= t, and j > t - window when window > 0. Single tokens, drafted
- * blocks and prompt chunks may be mixed in one call. A row that sees no key is zero. What the cache holds at
+ * blocks and prompt chunks may be mixed in one call. A row that sees no key is zero. out must not overlap q. What the cache holds at
  * slots that no query of a sequence's step sees does not matter (NaN included); a non-finite value that some
  * query of the step sees may reach the step's other queries of that sequence. The handle owns the scratch of
  * partial results: calls on one handle must not overlap on the GPU (one stream, or events), replays of graphs

@@ -238,6 +238,34 @@ def test_attention_cache_orders(cuda, order):
     check_attention([1, 3], [90, 200], 8, 4, 128, 32, 0, order=order)
 
 
+@pytest.mark.parametrize("n", [1, 90])
+def test_attention_window_as_long_as_the_table(cuda, n):
+    """Windows that hide nothing, up to the largest."""
+    from helios_b200 import attention as A
+    s = Step([n], [200], 2, 128, 16, 7)
+    q = randn(n, 4, 128, seed=8)
+    attend = A.PagedAttention(4, 2, 128)
+    want = attend(q, s.cache, s.batch)
+    for window in (200, 208, 5000, 2 ** 31 - 1):
+        assert torch.equal(attend(q, s.cache, s.batch, window=window), want)
+
+
+def test_attention_shared_prefix_pages_and_max_kv(cuda):
+    """Two sequences over the same pages, and a table wider than the step's lengths."""
+    from helios_b200 import attention as A
+    s = Step([3, 2], [100, 100], 2, 128, 16, 9)
+    s.table[1] = s.table[0]
+    s.t_table.copy_(s.table)
+    q = randn(5, 4, 128, seed=8)
+    wide = torch.full((2, 400), -1, dtype=torch.int32, device="cuda")
+    wide[:, :7] = s.t_table
+    attend = A.PagedAttention(4, 2, 128)
+    for batch in (s.batch, A.PagedBatch(s.t_off, s.t_kv, wide, max_q=3), A.PagedBatch(s.t_off, s.t_kv, wide, max_q=3, max_kv=100)):
+        out = attend(q, s.cache, batch)
+        no_device_error()
+        close(out, *s.reference(q, 128 ** -0.5, 0))
+
+
 def test_attention_peaked_scores(cuda):
     check_attention([1, 2], [900, 300], 16, 1, 512, 64, 0, scale=1.0)
 
@@ -375,8 +403,17 @@ def test_refusals(cuda):
     for bad in (float("nan"), 0.0, -1.0):
         with pytest.raises(ValueError, match="scale"):
             attend(q, s.cache, s.batch, scale=bad)
-    with pytest.raises(ValueError, match="window"):
-        attend(q, s.cache, s.batch, window=-1)
+    for bad in (-1, 2 ** 31, 2 ** 32 + 5):
+        with pytest.raises(ValueError, match="window"):
+            attend(q, s.cache, s.batch, window=bad)
+    with pytest.raises(ValueError, match="out must not be q"):
+        attend(q, s.cache, s.batch, out=q)
+    with pytest.raises(ValueError, match="token_stride"):
+        attend(q.expand(3, 4, 128), s.cache, s.batch)
+    with pytest.raises(ValueError, match="max_q"):
+        A.PagedBatch(s.t_off, s.t_kv, s.t_table, max_q=0)
+    with pytest.raises(ValueError, match="must hold 2"):
+        A.PagedBatch(s.t_off[:1], s.t_kv, s.t_table, max_q=1)
     with pytest.raises(ValueError, match="query heads"):
         attend(q[:, :2], s.cache, s.batch)
     with pytest.raises(ValueError, match="heads are not the handle's"):
