@@ -205,9 +205,33 @@ def call(name: str, *args) -> None:
     """Call a g4q entry point and raise G4qError on a non-OK status."""
     status = getattr(_lib or load(), name)(*args)
     if status != G4Q_OK:
-        msg = last_error()
-        cls = G4qInvalidArgument if status == G4Q_ERR_INVALID_ARGUMENT else G4qError
-        raise cls(status, msg, name)
+        raise_status(status, name)
+
+
+def raise_status(status: int, name: str) -> None:
+    """Raise the error of a non-OK status, with the calling thread's last message."""
+    cls = G4qInvalidArgument if status == G4Q_ERR_INVALID_ARGUMENT else G4qError
+    raise cls(status, last_error(), name)
+
+
+_torch_ops = None
+
+
+def torch_ops():
+    """The CPython module of the attention calls (_g4q_torch.so), bound to the loaded libg4q.so."""
+    global _torch_ops
+    if _torch_ops is None:
+        lib = load()
+        try:
+            from . import _g4q_torch as ops
+        except ImportError as e:
+            raise G4qUnavailable(f"_g4q_torch.so is missing or cannot load ({e}): build it with "
+                                 "`python -m helios_b200.build`") from e
+        entry = [ctypes.cast(getattr(lib, n), ctypes.c_void_p).value
+                 for n in ("g4q_qk_norm_rope", "g4q_kv_append", "g4q_paged_attention")]
+        ops.bind(*entry, raise_status)
+        _torch_ops = ops
+    return _torch_ops
 
 
 def device_error(reset: bool = True) -> int:

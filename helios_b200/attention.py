@@ -11,7 +11,8 @@ sliding-window mask. A layer's step is two launches around the matmuls::
     attn = attention(q, cache, batch, scale=scale, window=1024)      # PagedAttention
     o = quantized_matmul(attn.flatten(1), w_o)
 
-All compute runs in libg4q.so on the current CUDA stream; tensors are torch CUDA tensors, bf16.
+All compute runs in libg4q.so on the current CUDA stream; tensors are torch CUDA tensors, bf16. The calls of a
+step go through a small CPython module (csrc/g4q_torch.cpp), which checks the tensors and makes the outputs.
 """
 from __future__ import annotations
 
@@ -26,36 +27,7 @@ from . import _lib
 __all__ = ["Rope", "PagedKVCache", "PagedBatch", "PagedAttention", "qk_norm_rope", "kv_append"]
 
 
-_BF16 = torch.bfloat16
 _raw_stream = torch._C._cuda_getCurrentRawStream
-_HeadRows = _lib.G4qHeadRows
-
-
-def _head_rows(t: torch.Tensor, head_dim: int, device: int, name: str, out: bool = False) -> _lib.G4qHeadRows:
-    """The C view of a [tokens, heads, head_dim] tensor (any strides that keep 16-byte chunks whole). These
-    checks run on every call of a decode step, so they stay a few attribute reads per tensor."""
-    if t.dtype is not _BF16 or t.get_device() != device:
-        raise ValueError(f"{name} must be a bfloat16 CUDA tensor on cuda:{device} (got {t.dtype} on {t.device})")
-    shape = t.shape
-    if len(shape) != 3 or shape[2] != head_dim:
-        raise ValueError(f"{name} must be [tokens, heads, {head_dim}] (got {tuple(shape)})")
-    st, sh, sd = t.stride()
-    data = t.data_ptr()
-    if sd != 1 or (st | sh) & 7 or data & 15:
-        raise ValueError(f"{name}: the last dimension must be contiguous, strides multiples of 8 and data 16-byte aligned")
-    if shape[1] == 1:
-        sh = max(sh, head_dim)
-    if out and (sh < head_dim or (shape[0] > 1 and st < head_dim)):
-        raise ValueError(f"{name}: its rows overlap")
-    return _HeadRows(data, st, sh, shape[1])
-
-
-def _norm_weight(w: Optional[torch.Tensor], head_dim: int, device: int, name: str) -> Optional[int]:
-    if w is None:
-        return None
-    if w.dtype is not _BF16 or w.get_device() != device or w.shape != (head_dim,) or not w.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous bf16 tensor of shape ({head_dim},) on cuda:{device}")
-    return w.data_ptr()
 
 
 def _int32(t: torch.Tensor, dims: int, name: str) -> torch.Tensor:
@@ -64,20 +36,9 @@ def _int32(t: torch.Tensor, dims: int, name: str) -> torch.Tensor:
     return t
 
 
-def _same_device(device: int, **what) -> None:
-    for name, x in what.items():
-        if x.device != device:
-            raise ValueError(f"{name} is on cuda:{x.device}, not on cuda:{device}")
-
-
-def _output(t: torch.Tensor, heads: int, head_dim: int, device: int, out: Optional[torch.Tensor], name: str):
-    """The output tensor for t's shape (a new contiguous one for None) and its C view."""
-    if out is None:
-        out = torch.empty_like(t, memory_format=torch.contiguous_format)
-        return out, _HeadRows(out.data_ptr(), heads * head_dim, head_dim, heads)
-    if out.shape != t.shape:
-        raise ValueError(f"{name} must be shaped {tuple(t.shape)}")
-    return out, _head_rows(out, head_dim, device, name, True)
+def _same_device(device: int, cache, batch) -> None:
+    if cache.device != device or batch.device != device:
+        raise ValueError(f"the cache (cuda:{cache.device}) and the batch (cuda:{batch.device}) must be on cuda:{device}")
 
 
 class Rope:
@@ -104,6 +65,7 @@ class Rope:
         _lib.call("g4q_rope_create", head_dim, rotary_dim, arr, ctypes.byref(self._h))
         self.head_dim, self.rotary_dim = head_dim, rotary_dim
         self.device = torch.cuda.current_device()
+        self._ops = _lib.torch_ops()
 
     @property
     def handle(self) -> ctypes.c_void_p:
@@ -144,6 +106,7 @@ class PagedKVCache:
         d = self.head_dim
         self.c = _lib.G4qPagedCache(k.data_ptr(), v.data_ptr(), self.n_pages, self.page_size, self.n_kv_heads, d,
                                     max(sp, d) if self.n_pages == 1 else sp, max(sh, d) if self.n_kv_heads == 1 else sh, ss)
+        self.c_addr = ctypes.addressof(self.c)
 
     @classmethod
     def allocate(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int) -> "PagedKVCache":
@@ -180,12 +143,13 @@ class PagedBatch:
         self.max_q, self.max_kv = max_q, max_kv
         self._views = {}
 
-    def view(self, page_size: int) -> _lib.G4qPagedBatch:
-        """The C view for a cache of this page size."""
+    def view(self, page_size: int) -> int:
+        """Address of the C view for a cache of this page size."""
         v = self._views.get(page_size)
         if v is None:
-            v = self._views[page_size] = self._view(page_size)
-        return v
+            c = self._view(page_size)
+            v = self._views[page_size] = (ctypes.addressof(c), c)
+        return v[0]
 
     def _view(self, page_size: int) -> _lib.G4qPagedBatch:
         t = self.block_table
@@ -204,20 +168,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rope
     """``rope(rms_norm(q) * q_weight)`` and the same for k, in one launch: q [tokens, q_heads, head_dim],
     k [tokens, kv_heads, head_dim] (views of the q|k|v matmul's output qualify), ``positions`` int32 [tokens].
     fp32 inside, one rounding at the end. The outputs may be the inputs (in place)."""
-    d, dev = rope.head_dim, rope.device
-    cq, ck = _head_rows(q, d, dev, "q"), _head_rows(k, d, dev, "k")
-    n = q.shape[0]
-    if k.shape[0] != n:
-        raise ValueError("q and k must have the same number of tokens")
-    if positions.dtype is not torch.int32 or positions.get_device() != dev or positions.shape != (n,) or (
-            n > 1 and positions.stride(0) != 1):
-        raise ValueError(f"positions must be a contiguous int32 tensor on cuda:{dev} with one entry per token")
-    q_out, co = _output(q, cq.n_heads, d, dev, q_out, "q_out")
-    k_out, cko = _output(k, ck.n_heads, d, dev, k_out, "k_out")
-    _lib.call("g4q_qk_norm_rope", rope.handle, cq, ck, n, positions.data_ptr(),
-              _norm_weight(q_weight, d, dev, "q_weight"), _norm_weight(k_weight, d, dev, "k_weight"), eps, co, cko,
-              _raw_stream(dev))
-    return q_out, k_out
+    dev = rope.device
+    return rope._ops.qk_norm_rope(rope.handle.value, rope.head_dim, dev, _raw_stream(dev), q, k, positions, q_weight, k_weight,
+                                  eps, q_out, k_out)
 
 
 def kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache, batch: PagedBatch,
@@ -227,23 +180,11 @@ def kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cache
     pages, values normalized (without a weight; ``norm_values=False`` stores them as they are) beside them,
     and the queries, treated like the keys with ``q_weight``, returned (None for q None). One launch. ``v``
     may be ``k``. Sequences may share pages of a common prefix, but no two may append to one slot. Rows that belong to no sequence are left as they were (in ``q_out`` too)."""
-    d, dev = rope.head_dim, rope.device
-    _same_device(dev, cache=cache, batch=batch)
-    ck = _head_rows(k, d, dev, "k")
-    cv = ck if v is k else _head_rows(v, d, dev, "v")
-    n = k.shape[0]
-    if v.shape[0] != n or (q is not None and q.shape[0] != n):
-        raise ValueError("q, k and v must have the same number of tokens")
-    cq = co = None
-    if q is not None:
-        cq = _head_rows(q, d, dev, "q")
-        q_out, co = _output(q, cq.n_heads, d, dev, q_out, "q_out")
-    elif q_out is not None:
-        raise ValueError("q_out without q")
-    _lib.call("g4q_kv_append", rope.handle, cq, ck, cv, n, _norm_weight(q_weight, d, dev, "q_weight"),
-              _norm_weight(k_weight, d, dev, "k_weight"), eps, 0 if norm_values else _lib.APPEND_RAW_VALUES, co,
-              cache.c, batch.view(cache.page_size), _raw_stream(dev))
-    return q_out
+    dev = rope.device
+    _same_device(dev, cache, batch)
+    return rope._ops.kv_append(rope.handle.value, rope.head_dim, dev, _raw_stream(dev), q, k, v, cache.c_addr,
+                               batch.view(cache.page_size), q_weight, k_weight, eps,
+                               0 if norm_values else _lib.APPEND_RAW_VALUES, q_out)
 
 
 class PagedAttention:
@@ -257,6 +198,7 @@ class PagedAttention:
         _lib.call("g4q_attn_create", n_q_heads, n_kv_heads, head_dim, ctypes.byref(self._h))
         self.n_q_heads, self.n_kv_heads, self.head_dim = n_q_heads, n_kv_heads, head_dim
         self.device = torch.cuda.current_device()
+        self._ops = _lib.torch_ops()
 
     @property
     def handle(self) -> ctypes.c_void_p:
@@ -271,15 +213,11 @@ class PagedAttention:
         to ``head_dim ** -0.5``. Single tokens, drafted blocks and prompt chunks may be mixed. A row that sees
         no key is zero; rows that belong to no sequence are left as they were (in ``out``, which must not overlap
         q)."""
-        d, dev = self.head_dim, self.device
-        _same_device(dev, cache=cache, batch=batch)
-        cq = _head_rows(q, d, dev, "q")
-        if not 0 <= window < 2 ** 31:
-            raise ValueError("window must be >= 0 (0: none) and below 2^31")
-        out, co = _output(q, cq.n_heads, d, dev, out, "out")
-        _lib.call("g4q_paged_attention", self.handle, cq, q.shape[0], cache.c, batch.view(cache.page_size),
-                  d ** -0.5 if scale is None else scale, window, co, _raw_stream(dev))
-        return out
+        dev = self.device
+        _same_device(dev, cache, batch)
+        return self._ops.paged_attention(self.handle.value, self.head_dim, dev, _raw_stream(dev), q, cache.c_addr,
+                                         batch.view(cache.page_size), self.head_dim ** -0.5 if scale is None else scale, window,
+                                         out)
 
     def free(self) -> None:
         if self._h:

@@ -1,4 +1,5 @@
-"""Builds libg4q.so (the C-ABI kernel library) in-tree with nvcc for sm_100a.
+"""Builds libg4q.so (the C-ABI kernel library) in-tree with nvcc for sm_100a, and _g4q_torch.so (the Python
+side of the attention calls, a CPython module over torch's headers) with the host compiler.
 
 ``python -m helios_b200.build`` or ``helios_b200.build.build()``. The shared library lands
 next to this file so it travels with the source tree; no JIT cache is involved.
@@ -15,6 +16,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libg4q.so"
+TORCH_SRC = CSRC / "g4q_torch.cpp"
+TORCH_LIB = PKG / "_g4q_torch.so"
 OBJDIR = PKG / "_build"
 
 SOURCES = ["g4q_api.cu", "g4q_layout.cu", "g4q_gemv.cu", "g4q_gemv2.cu", "g4q_gemm.cu", "g4q_decode.cu",
@@ -43,8 +46,21 @@ def _stale(target: Path, deps) -> bool:
     return any(Path(d).stat().st_mtime > t for d in deps)
 
 
+def _torch_command() -> list:
+    """The host compiler's command for _g4q_torch.so."""
+    import sysconfig
+
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"],
+           INCLUDE]
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{i}" for i in inc), str(TORCH_SRC),
+            "-o", str(TORCH_LIB), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+
+
 def build(verbose: bool = False, force: bool = False) -> Path:
-    """Compile every .cu under csrc/ for sm_100a and link libg4q.so. Returns its path."""
+    """Compile every .cu under csrc/ for sm_100a, link libg4q.so and build _g4q_torch.so. Returns libg4q.so's path."""
     OBJDIR.mkdir(exist_ok=True)
     nvcc = _nvcc()
     common_deps = [CSRC / h for h in HEADERS] + [INCLUDE / "g4q.h"]
@@ -54,6 +70,8 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         objs.append(obj)
         if force or _stale(obj, [CSRC / src] + common_deps):
             cmds.append([nvcc, *NVCC_FLAGS, "-I", str(INCLUDE), "-I", str(CSRC), "-c", str(CSRC / src), "-o", str(obj)])
+    if force or _stale(TORCH_LIB, [TORCH_SRC, INCLUDE / "g4q.h"]):
+        cmds.append(_torch_command())
     # translation units compile independently: one nvcc per source, a few at a time
     from concurrent.futures import ThreadPoolExecutor
 

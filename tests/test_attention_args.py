@@ -59,9 +59,28 @@ def test_attn_create_refuses(hq, hk, d, expect, message):
 
 def test_python_layer_refuses_before_the_library():
     from helios_b200 import attention as A
+    ops = _lib.torch_ops()
     cpu = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
-    with pytest.raises(ValueError, match="CUDA tensor"):
-        A._head_rows(cpu, 64, 0, "q")
+    for bad, word in ((cpu, "CUDA tensor"), (cpu.float(), "bfloat16"), (None, "torch tensor"), (3, "torch tensor")):
+        with pytest.raises(ValueError, match=word):
+            ops.paged_attention(0, 64, 0, 0, bad, 0, 0, 1.0, 0, None)
+        with pytest.raises(ValueError, match=word):
+            ops.qk_norm_rope(0, 64, 0, 0, bad, cpu, cpu, None, None, 1e-6, None, None)
+        with pytest.raises(ValueError, match=word):
+            ops.kv_append(0, 64, 0, 0, None, bad, cpu, 0, 0, None, None, 1e-6, 0, None)
+    for window in (-1, 2 ** 31):
+        with pytest.raises(ValueError, match="window"):
+            ops.paged_attention(0, 64, 0, 0, cpu, 0, 0, 1.0, window, None)
+    with pytest.raises(TypeError):
+        ops.paged_attention(0, 64)
+    with pytest.raises(TypeError):
+        ops.paged_attention("x", 64, 0, 0, cpu, 0, 0, 1.0, 0, None)
+    with pytest.raises(TypeError):
+        ops.paged_attention(0, 64, 0, 0, cpu, 0, 0, "x", 0, None)
+    with pytest.raises(OverflowError):
+        ops.paged_attention(0, 64, 0, 0, cpu, 0, 0, 1.0, 2 ** 70, None)
+    with pytest.raises(TypeError):
+        ops.bind(0, 0, 0, None)
     with pytest.raises(ValueError, match="4-D bfloat16 CUDA"):
         A.PagedKVCache(torch.zeros(2, 1, 16, 64, dtype=torch.bfloat16), torch.zeros(2, 1, 16, 64, dtype=torch.bfloat16))
     with pytest.raises(ValueError, match="int32 CUDA"):
