@@ -129,29 +129,36 @@ __global__ void __launch_bounds__(kWarps * 32) head_rows_kernel(const __grid_con
         pos = p.positions[m];
     }
 
-    const int half = p.rotary / 2;
-    auto put = [&](int kind, int i, float fa, float fb) {
-        s_f[kind][0][(i >> 2) & 1][i >> 3][i & 3] = fa;
-        s_f[kind][1][(i >> 2) & 1][i >> 3][i & 3] = fb;
-    };
-    for (int i = threadIdx.x; i < D - half; i += blockDim.x) {
-        float cs = 1.0f, sn = 0.0f;
-        if (i < half) {
-            const uint64_t turn = (uint64_t)(int64_t)pos * p.turns[i];
-            const float angle = (float)(int32_t)(turn >> 32) * 1.4629180792671596e-9f;   // 2 pi * 2^-32
-            cs = __cosf(angle);
-            sn = __sinf(angle);
-        }
+    // four consecutive elements of a kind per thread: pairs (i, i + half), and the elements that are not rotated
+    const int half = p.rotary / 2, pairs4 = half / 4, units = pairs4 + (D - p.rotary) / 4;
+    for (int u = threadIdx.x; u < 2 * units; u += blockDim.x) {
+        const int kd = u >= units ? 1 : 0, v = u - kd * units;
+        const uint16_t* wt = kd == 0 ? p.q_weight : p.k_weight;
+        auto weights = [&](int i) {
+            const uint2 w = wt != nullptr ? *reinterpret_cast<const uint2*>(wt + i) : make_uint2(0x3F803F80u, 0x3F803F80u);   // bf16 1.0
+            return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16),
+                               __uint_as_float(w.y & 0xFFFF0000u));
+        };
+        auto put = [&](int ab, int i, float4 f) { *reinterpret_cast<float4*>(s_f[kd][ab][(i >> 2) & 1][i >> 3]) = f; };
+        if (v < pairs4) {
+            const int i = 4 * v;
+            float cs[4], sn[4];
 #pragma unroll
-        for (int kind = 0; kind < 2; ++kind) {
-            const uint16_t* wt = kind == 0 ? p.q_weight : p.k_weight;
-            if (i < half) {   // the pair (i, i + half)
-                const float w0 = wt != nullptr ? bf16_bits_to_f32(wt[i]) : 1.0f, w1 = wt != nullptr ? bf16_bits_to_f32(wt[i + half]) : 1.0f;
-                put(kind, i, w0 * cs, -w1 * sn);
-                put(kind, i + half, w1 * cs, w0 * sn);
-            } else if (i + half >= p.rotary) {   // an element that is not rotated
-                put(kind, i + half, wt != nullptr ? bf16_bits_to_f32(wt[i + half]) : 1.0f, 0.0f);
+            for (int e = 0; e < 4; ++e) {
+                const uint64_t turn = (uint64_t)(int64_t)pos * p.turns[i + e];
+                const float angle = (float)(int32_t)(turn >> 32) * 1.4629180792671596e-9f;   // 2 pi * 2^-32
+                cs[e] = __cosf(angle);
+                sn[e] = __sinf(angle);
             }
+            const float4 w0 = weights(i), w1 = weights(i + half);
+            put(0, i, make_float4(w0.x * cs[0], w0.y * cs[1], w0.z * cs[2], w0.w * cs[3]));
+            put(1, i, make_float4(-w1.x * sn[0], -w1.y * sn[1], -w1.z * sn[2], -w1.w * sn[3]));
+            put(0, i + half, make_float4(w1.x * cs[0], w1.y * cs[1], w1.z * cs[2], w1.w * cs[3]));
+            put(1, i + half, make_float4(w0.x * sn[0], w0.y * sn[1], w0.z * sn[2], w0.w * sn[3]));
+        } else {
+            const int i = p.rotary + 4 * (v - pairs4);
+            put(0, i, weights(i));
+            put(1, i, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
         }
     }
     __syncthreads();
@@ -197,6 +204,14 @@ __global__ void __launch_bounds__(kWarps * 32) head_rows_kernel(const __grid_con
             }
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
+                if (j > 0 && 2 * off <= 32) {            // none of these chunks is rotated
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const float4 fa = *reinterpret_cast<const float4*>(s_f[kind][0][q][l + j * LPH]);
+                        x[j][4 * q] *= fa.x, x[j][4 * q + 1] *= fa.y, x[j][4 * q + 2] *= fa.z, x[j][4 * q + 3] *= fa.w;
+                    }
+                    continue;
+                }
                 float y[8];
                 unpack8(other[j], y);
 #pragma unroll
