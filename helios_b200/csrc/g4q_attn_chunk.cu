@@ -62,6 +62,7 @@ struct ChunkCfg {
     static constexpr int kVStages = kStages / 2 < 1 ? 1 : (kStages - (kKSt - 1)) / 2;   // of the ring of V tiles
     static constexpr int kKStages = kStages - kVStages;                                 // of the ring of K tiles
     static constexpr int kSmem = 1024 + kQBytes + kStages * kStageBytes + 256;
+    static_assert(kKeysHeld / 16 * (kKCols / 64) <= 32 && kTile / 16 * (kVCols / 64) <= 32, "a lane issues one box of a stage");
     static_assert(kKeysHeld * kKCols == kTile * kVCols && kVCols % 64 == 0, "stages hold either operand");
     static_assert(kVStages >= 1 && kKStages >= kKSt, "a tile of each fits");
 };
@@ -74,6 +75,7 @@ struct ChunkCall {
     int tile_tokens;     // tokens of a tile: of all the CTAs that share it
     int box;
     int wave;            // tiles that the GPU computes at once
+    int clusters;        // CTAs or CTA pairs of the launch
     float* part_o;       // [pieces, at most a wave][CTAs of a tile * 128][output columns of a CTA]
     float* part_ml;      // [pieces][CTAs of a tile * 128][2]
     int* err;
@@ -85,6 +87,7 @@ struct Work {
     int b, tile, h, half;
     int piece, pieces;   // of the keys
     int slot;            // place of the piece's partial
+    int count;           // of all the work of the launch
 };
 
 struct TileWork {
@@ -110,12 +113,11 @@ __device__ __forceinline__ TileWork tile_work(const ChunkCall& c, const SeqGeom&
     return w;
 }
 
-// The work of the index-th CTA (pair) of the launch, or of the index-th tile of the last wave (kLast); b < 0: none.
-// One warp. Tiles of the whole waves come first, each one CTA pair's; then the rest's first pieces, second pieces
-// and so on. The longest tiles come first: a sequence's last one, and up to 32 sequences by their lengths (more: the
+// The index-th piece of work of the launch, or the index-th tile of the last wave (kLast); b < 0: none. One warp.
+// Tiles of the whole waves come first, each one piece; then the rest's first pieces, second pieces and so on. The longest tiles come first: a sequence's last one, and up to 32 sequences by their lengths (more: the
 // batch's last first).
 template <int D, bool kLast>
-__device__ __forceinline__ Work find_work(const ChunkCall& c, int index, int lane) {
+__device__ __noinline__ Work find_work(const ChunkCall& c, int index, int lane) {
     constexpr int kHalves = ChunkCfg<D>::kHalves;
     const int n_seqs = c.a.pv.n_seqs;
     auto geom_of = [&](int b) {
@@ -133,6 +135,7 @@ __device__ __forceinline__ Work find_work(const ChunkCall& c, int index, int lan
     const int per_tile = c.a.hk * kHalves, items = total * per_tile;
     const int whole = items / c.wave * c.wave, rest = items - whole;
     const int cuts = rest > 0 ? min(kMaxSplits, c.wave / rest) : 1;
+    w.count = whole + rest * cuts;
     int item = index, piece = 0;
     if (kLast) {
         if (index >= rest) return w;
@@ -192,14 +195,11 @@ __device__ __forceinline__ Work find_work(const ChunkCall& c, int index, int lan
 // Shared-memory descriptor of a SWIZZLE_128B operand. K-major: rows of 128 bytes, 8-row groups 1024 bytes
 // apart (lbo unused). MN-major: 64 elements of the MN dimension per 128-byte row, one row per k, 8 k's 1024
 // bytes apart, the next 64 elements lbo bytes on.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr & 0x3FFFFu) >> 4);
-    d |= (uint64_t)(lbo >> 4) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
+// The upper word is the same for all of them; the lower one is the address in units of 16 bytes, below lbo, so a step
+// of a tile is one addition.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t lbo) {
+    return ((saddr & 0x3FFFFu) >> 4) | ((lbo >> 4) << 16);
 }
 
 // kind::f16 instruction descriptor: D f32, A and B bf16; b_mn: B is MN-major.
@@ -210,38 +210,38 @@ constexpr uint32_t instr_desc(int m, int n, bool b_mn) {
 // D += A B with A in shared memory (mma_ss) or TMEM (mma_ts). On a CTA pair each CTA holds its 128 rows of A and
 // D, and half of B's columns.
 template <int kCtas>
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
     if constexpr (kCtas == 2)
         asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+            "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+            "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescHigh)
             : "memory");
     else
         asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+            "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+            "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescHigh)
             : "memory");
 }
 
 template <int kCtas>
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
     if constexpr (kCtas == 2)
         asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-            "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+            "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+            "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescHigh)
             : "memory");
     else
         asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-            "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+            "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+            "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescHigh)
             : "memory");
 }
 
@@ -347,8 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     using C = ChunkCfg<D>;
     constexpr int kCtas = C::kCtas;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ Work found;
-    const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+        const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_addr(smem_raw));
     const uint32_t s_q = base, s_ring = s_q + C::kQBytes, s_bar = s_ring + C::kStages * C::kStageBytes;
     auto full = [&](int s) { return s_bar + 8u * s; };
@@ -357,16 +356,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto p_full = [&](int b) { return s_bar + 8u * (2 * C::kStages + 2 + b); };
     const uint32_t q_full = s_bar + 8u * (2 * C::kStages + 4);
     auto o_done = [&](int b) { return q_full + 8u + 8u * b; };    // products of the even and the odd tiles
-    const uint32_t edge_full = q_full + 24;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (s_bar - base) + 8u * (2 * C::kStages + 8));
+    const uint32_t edge_full = q_full + 24, q_free = q_full + 32;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (s_bar - base) + 8u * (2 * C::kStages + 9));
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = blockIdx.x % kCtas;                 // place in the pair
-    if (warp == 0) {
-        wait_for_predecessor();
-        const Work f = find_work<D, false>(c, blockIdx.x / kCtas, lane);
-        if (lane == 0) found = f;
-    } else if (warp == 1) {
+    const int cluster = blockIdx.x / kCtas;
+    if (warp == 1) {
         if constexpr (kCtas == 2) {
             asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
                          "r"(kTmemCols));
@@ -387,6 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bar_init(o_done(b), 1);
         }
         bar_init(q_full, kCtas);
+        bar_init(q_free, 1);
         bar_init(edge_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         for (const CUtensorMap* map : {&tm_q, &tm_k, &tm_v})
@@ -400,23 +397,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const uint32_t t_o = tmem, t_s = tmem + 256;     // output, two score buffers of 128 columns
-    const Work at = found;
-    const int h = at.h, half = at.half;
 
-    if (at.b >= 0) {
-        const TileWork w = tile_work(c, at.g, at.tile);
-        const int t0 = w.t0 + rank * c.tokens;       // this CTA's first token
+    // The work of this cluster: every warp walks the same list, the way back and forth over the clusters, so that who
+    // had a long tile in one round has a short one in the next.
+    Work at;
+    TileWork w;
+    int t0 = 0, j0 = 0, n = 0, h = 0, half = 0;
+    auto find = [&](int r) {
+        return find_work<D, false>(c, r * c.clusters + ((r & 1) ? c.clusters - 1 - cluster : cluster), lane);
+    };
+    auto begin = [&](const Work& next) {
+        at = next;
+        if (at.b < 0) return false;
+        w = tile_work(c, at.g, at.tile);
+        t0 = w.t0 + rank * c.tokens;             // this CTA's first token
         // this piece's key tiles
-        const int j0 = w.n * at.piece / at.pieces, n = w.n * (at.piece + 1) / at.pieces - j0;
+        j0 = w.n * at.piece / at.pieces;
+        n = w.n * (at.piece + 1) / at.pieces - j0;
+        h = at.h;
+        half = at.half;
+        return true;
+    };
+    Work next = find(0);
+    uint32_t done = 0;     // tiles of work done, and the key tiles of them: the phases of the barriers go on
+    uint32_t g = 0;
+    {
         if (warp == 0 || warp == 6) {
             // ---------------- producers: Q and K tiles (warp 0), V tiles (warp 6)
-            if (warp == 0 && lane == 0) {
-                const uint32_t qb = in_first_cta(q_full);
-                bar_expect_tx_cluster(qb, (uint32_t)(c.tokens * c.group) * 128u * (D / 64));
-                for (int x = 0; x < D / 64; ++x)
-                    tma_rows<kCtas>(s_q + x * (kTile * 128), &tm_q, x * 64, h * c.group, w.g.q0 + t0, qb);
-            }
-            __syncwarp();
             const int first_stage = warp == 0 ? 0 : C::kKStages, last_stage = warp == 0 ? C::kKStages : C::kStages;
             int stage = first_stage;
             uint32_t round = 0, edge_round = 0;
@@ -438,42 +445,40 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 return page;
             };
-            // boxes [b0, b1) of the stage's keys k0.. (`keys` of them, the first one box `first` of its tile) by TMA,
-            // columns [col0, col0 + 64 * blocks)
-            auto fill = [&](const CUtensorMap* map, uint32_t bar, int pages, int k0, int keys, int first, int b0, int b1, int col0,
+            // Fills the next stage with boxes [b0, b1) of its keys k0.. (`keys` of them, the first one box `first` of
+            // its tile), columns [col0, col0 + 64 * blocks): at most one box a lane. All of it is worked out before the
+            // stage is free: with two or three stages, what happens between its release and the copies is waited for.
+            auto fill = [&](const CUtensorMap* map, bool edge, int pages, int k0, int keys, int first, int b0, int b1, int col0,
                             int blocks) {
-                if (lane == 0) bar_expect_tx_cluster(bar, (uint32_t)((b1 - b0) * blocks) * box_bytes);
+                const int box = b0 + lane / blocks, cb = lane % blocks;
+                const int page = __shfl_sync(0xFFFFFFFFu, pages, (first + box) & 31);
+                const uint32_t dst = s_ring + stage * C::kStageBytes + cb * (keys * 128) + box * box_bytes;
+                const int slot = (k0 + box * c.box) & page_mask, count = (b1 - b0) * blocks;
+                const uint32_t bar = edge ? edge_full : in_first_cta(full(stage));
+                if (round > 0) bar_wait(empty(stage), (round - 1) & 1, c.err, 80);
+                if (lane == 0) bar_expect_tx_cluster(bar, (uint32_t)count * box_bytes);
                 __syncwarp();
-                for (int i0 = 0; i0 < (b1 - b0) * blocks; i0 += 32) {
-                    const int i = i0 + lane, box = b0 + i / blocks, cb = i % blocks;
-                    const int page = __shfl_sync(0xFFFFFFFFu, pages, (first + box) & 31);
-                    if (i < (b1 - b0) * blocks)
-                        tma_page<kCtas>(s_ring + stage * C::kStageBytes + cb * (keys * 128) + box * box_bytes, map, col0 + cb * 64,
-                                        (k0 + box * c.box) & page_mask, h, page, bar);
-                }
+                if (lane < count) tma_page<kCtas>(dst, map, col0 + cb * 64, slot, h, page, bar);
             };
             auto load_k = [&](int j, int pages) {
                 const int k0 = w.lo + (j0 + j) * kTile + rank * C::kKeysHeld;
                 // a box without a key that some row sees is left out: its scores are masked
                 const int nb = max(0, min(C::kKeysHeld / c.box, (w.any_hi - k0 + c.box - 1) / c.box));
                 for (int p = 0; p < C::kKSt; ++p) {
-                    if (round > 0) bar_wait(empty(stage), (round - 1) & 1, c.err, 80);
-                    fill(&tm_k, in_first_cta(full(stage)), pages, k0, C::kKeysHeld, rank * C::kKeysHeld / c.box, 0, nb,
-                         p * C::kKCols, C::kKCols / 64);
+                    fill(&tm_k, false, pages, k0, C::kKeysHeld, rank * C::kKeysHeld / c.box, 0, nb, p * C::kKCols, C::kKCols / 64);
                     if (++stage == last_stage) stage = first_stage, ++round;
                 }
             };
             auto load_v = [&](int j, int pages) {
                 const int k0 = w.lo + (j0 + j) * kTile, col0 = half * C::kDv + rank * C::kVCols;
-                if (round > 0) bar_wait(empty(stage), (round - 1) & 1, c.err, 80);
                 const int b1 = max(0, min(boxes, (w.any_hi - k0 + c.box - 1) / c.box));
                 if (k0 >= w.any_lo && k0 + kTile <= w.any_hi) {
-                    fill(&tm_v, in_first_cta(full(stage)), pages, k0, kTile, 0, 0, boxes, col0, C::kVCols / 64);
+                    fill(&tm_v, false, pages, k0, kTile, 0, 0, boxes, col0, C::kVCols / 64);
                 } else {
                     // Keys that no row of the tile sees hold anything, and a zero weight times NaN is NaN: the stage
                     // is filled on a barrier of this CTA's own, their rows are zeroed, and it is handed over then.
                     const int b0 = max(0, w.any_lo - k0) / c.box;
-                    fill(&tm_v, edge_full, pages, k0, kTile, 0, min(b0, b1), b1, col0, C::kVCols / 64);
+                    fill(&tm_v, true, pages, k0, kTile, 0, min(b0, b1), b1, col0, C::kVCols / 64);
                     bar_wait(edge_full, edge_round++ & 1, c.err, 88);
                     const int lo = min(kTile, max(0, w.any_lo - k0)), hi = min(kTile, max(lo, w.any_hi - k0));
                     for (int i = lane; i < (lo + kTile - hi) * (C::kVCols / 8); i += 32) {
@@ -489,15 +494,31 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (++stage == last_stage) stage = first_stage, ++round;
             };
-            int pages = look_up(0), pages1 = look_up(1);
-            for (int j = 0; j < n; ++j) {
-                const int pages2 = look_up(j + 2);
-                if (warp == 0)
-                    load_k(j, pages);
-                else
-                    load_v(j, pages);
-                pages = pages1;
-                pages1 = pages2;
+            for (int r = 0; r * c.clusters < next.count; ++r) {
+                const bool some = begin(next);
+                next = find(r + 1);
+                if (!some) continue;
+                if (warp == 0) {
+                    if (done > 0) bar_wait(q_free, (done - 1) & 1, c.err, 89);
+                    if (lane == 0) {
+                        const uint32_t qb = in_first_cta(q_full);
+                        bar_expect_tx_cluster(qb, (uint32_t)(c.tokens * c.group) * 128u * (D / 64));
+                        for (int x = 0; x < D / 64; ++x)
+                            tma_rows<kCtas>(s_q + x * (kTile * 128), &tm_q, x * 64, h * c.group, w.g.q0 + t0, qb);
+                    }
+                    __syncwarp();
+                }
+                int pages = look_up(0), pages1 = look_up(1);
+                for (int j = 0; j < n; ++j) {
+                    const int pages2 = look_up(j + 2);
+                    if (warp == 0)
+                        load_k(j, pages);
+                    else
+                        load_v(j, pages);
+                    pages = pages1;
+                    pages1 = pages2;
+                }
+                ++done;
             }
         } else if (warp == 1) {
             // ---------------- MMA issuer (of the pair's first CTA)
@@ -509,173 +530,179 @@ __global__ void __launch_bounds__(kThreads, 1)
                         bar_wait(full(stage), round & 1, c.err, 81);
                         tc_fence_after();
                         if (lane == 0) {
+                            const uint32_t q = desc_low(s_q + p * (C::kKCols / 64) * (kTile * 128), 16);
+                            const uint32_t k = desc_low(s_ring + stage * C::kStageBytes, 16);
+                            const uint32_t d = t_s + ((g + j) & 1) * kTile;
 #pragma unroll
                             for (int kk = 0; kk < C::kKCols / 16; ++kk)
-                                mma_ss<kCtas>(t_s + (j & 1) * kTile,
-                                              sw128_desc(s_q + (p * (C::kKCols / 64) + (kk >> 2)) * (kTile * 128) + (kk & 3) * 32, 16),
-                                              sw128_desc(s_ring + stage * C::kStageBytes + (kk >> 2) * (C::kKeysHeld * 128) + (kk & 3) * 32, 16),
+                                mma_ss<kCtas>(d, q + ((kk >> 2) * (kTile * 128) + (kk & 3) * 32) / 16,
+                                              k + ((kk >> 2) * (C::kKeysHeld * 128) + (kk & 3) * 32) / 16,
                                               instr_desc(kTile * kCtas, kTile, false), (p | kk) != 0);
                             mma_commit<kCtas>(empty(stage));
                         }
                         __syncwarp();
                         if (++stage == C::kKStages) stage = 0, ++round;
                     }
-                    if (lane == 0) mma_commit<kCtas>(s_full(j & 1));
-                    __syncwarp();
-                };
-                bar_wait(q_full, 0, c.err, 82);
-                scores(0);
-                for (int j = 0; j < n; ++j) {
-                    if (j + 1 < n) scores(j + 1);
-                    bar_wait(p_full(j & 1), (j >> 1) & 1, c.err, 83);
-                    bar_wait(full(v_stage), v_round & 1, c.err, 84);
-                    tc_fence_after();
                     if (lane == 0) {
-#pragma unroll
-                        for (int kk = 0; kk < kTile / 16; ++kk)
-                            mma_ts<kCtas>(t_o, t_s + (j & 1) * kTile + kk * 8,
-                                          sw128_desc(s_ring + v_stage * C::kStageBytes + kk * 2048, kTile * 128),
-                                          instr_desc(kTile * kCtas, C::kDv, true), (j | kk) != 0);
-                        mma_commit<kCtas>(empty(v_stage));
-                        mma_commit<kCtas>(o_done(j & 1));
+                        mma_commit<kCtas>(s_full((g + j) & 1));
+                        if (j + 1 == n) mma_commit<kCtas>(q_free);     // Q has been read
                     }
                     __syncwarp();
-                    if (++v_stage == C::kStages) v_stage = C::kKStages, ++v_round;
+                };
+                for (int r = 0; r * c.clusters < next.count; ++r) {
+                    if (!begin(next)) {
+                        next = find(r + 1);
+                        continue;
+                    }
+                    bar_wait(q_full, done & 1, c.err, 82);
+                    scores(0);
+                    for (int j = 0; j < n; ++j) {
+                        if (j + 1 < n) scores(j + 1);
+                        const uint32_t b = (g + j) & 1;
+                        bar_wait(p_full(b), ((g + j) >> 1) & 1, c.err, 83);
+                        bar_wait(full(v_stage), v_round & 1, c.err, 84);
+                        tc_fence_after();
+                        if (lane == 0) {
+                            const uint32_t v = desc_low(s_ring + v_stage * C::kStageBytes, kTile * 128);
+#pragma unroll
+                            for (int kk = 0; kk < kTile / 16; ++kk)
+                                mma_ts<kCtas>(t_o, t_s + b * kTile + kk * 8, v + kk * (2048 / 16),
+                                              instr_desc(kTile * kCtas, C::kDv, true), (j | kk) != 0);
+                            mma_commit<kCtas>(empty(v_stage));
+                            mma_commit<kCtas>(o_done(b));
+                        }
+                        __syncwarp();
+                        if (++v_stage == C::kStages) v_stage = C::kKStages, ++v_round;
+                    }
+                    g += n;
+                    ++done;
+                    next = find(r + 1);                                // while the last products run
                 }
             }
         } else {
             // ---------------- softmax, one row per thread
             const int quarter = warp & 3;
-            const int r = quarter * 32 + lane;
+            const int row_in = quarter * 32 + lane;
             const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-            const int tok = r / c.group;
-            const bool mine = tok < c.tokens && t0 + tok < w.g.q_len;
-            int vis_lo = 0, vis_hi = 0;
-            if (mine) {
-                const int pos = w.g.first + t0 + tok;
-                vis_hi = min(max(pos + 1, 0), w.g.kv_len);
-                if (c.a.window > 0) vis_lo = max(0, pos - c.a.window + 1);
-            }
-            // keys that every row of this CTA sees (rows beyond the sequence do not matter)
-            const int all_hi = min(max(w.g.first + t0 + 1, 0), w.g.kv_len);
-            const int all_lo = c.a.window > 0 ? max(0, w.g.first + min(t0 + c.tokens, w.g.q_len) - c.a.window) : 0;
+            const int tok = row_in / c.group;
             const float scale2 = c.a.scale * kLog2e;
-            float m = -INFINITY, l = 0.0f;
-            for (int j = 0; j < n; ++j) {
-                const int k0 = w.lo + (j0 + j) * kTile;
-                const uint32_t ts = t_s + (j & 1) * kTile + lanes;
-                bar_wait(s_full(j & 1), (j >> 1) & 1, c.err, 85);
-                tc_fence_after();
-                uint32_t s[kTile];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, s + 32 * i);
-                tmem_wait_ld(s, kTile);
-                if (k0 < all_lo || k0 + kTile > all_hi) {
-#pragma unroll
-                    for (int x = 0; x < kTile; x += 32) {
-                        // bit i: key k0 + x + i is seen
-                        const int lo = min(max(vis_lo - k0 - x, 0), 32), hi = min(max(vis_hi - k0 - x, 0), 32);
-                        const uint32_t seen = (hi == 32 ? 0xFFFFFFFFu : (1u << hi) - 1u) & ~(lo == 32 ? 0xFFFFFFFFu : (1u << lo) - 1u);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if ((seen & (1u << i)) == 0) s[x + i] = 0xFF800000u;       // -inf
-                    }
+            for (int r = 0; r * c.clusters < next.count; ++r) {
+                if (!begin(next)) {
+                    next = find(r + 1);
+                    continue;
                 }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                const bool mine = tok < c.tokens && t0 + tok < w.g.q_len;
+                int vis_lo = 0, vis_hi = 0;
+                if (mine) {
+                    const int pos = w.g.first + t0 + tok;
+                    vis_hi = min(max(pos + 1, 0), w.g.kv_len);
+                    if (c.a.window > 0) vis_lo = max(0, pos - c.a.window + 1);
+                }
+                // keys that every row of this CTA sees (rows beyond the sequence do not matter)
+                const int all_hi = min(max(w.g.first + t0 + 1, 0), w.g.kv_len);
+                const int all_lo = c.a.window > 0 ? max(0, w.g.first + min(t0 + c.tokens, w.g.q_len) - c.a.window) : 0;
+                float m = -INFINITY, l = 0.0f;
+                for (int j = 0; j < n; ++j) {
+                    const int k0 = w.lo + (j0 + j) * kTile;
+                    const uint32_t b = (g + j) & 1, ts = t_s + b * kTile + lanes;
+                    bar_wait(s_full(b), ((g + j) >> 1) & 1, c.err, 85);
+                    tc_fence_after();
+                    uint32_t s[kTile];
 #pragma unroll
-                for (int i = 0; i < kTile; i += 4)
+                    for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, s + 32 * i);
+                    tmem_wait_ld(s, kTile);
+                    if (k0 < all_lo || k0 + kTile > all_hi) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], __uint_as_float(s[i + e]));
-                const float tile_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
-                if (__any_sync(0xFFFFFFFFu, tile_max > m + kRaise)) {
-                    const float m_new = fmaxf(m, tile_max);
-                    const float f = fast_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));
-                    if (j > 0) {
-                        bar_wait(o_done((j - 1) & 1), ((j - 1) >> 1) & 1, c.err, 86);
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int x = 0; x < C::kDv; x += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(t_o + lanes + x, o);
-                            tmem_wait_ld(o, 32);
+                        for (int x = 0; x < kTile; x += 32) {
+                            // bit i: key k0 + x + i is seen
+                            const int lo = min(max(vis_lo - k0 - x, 0), 32), hi = min(max(vis_hi - k0 - x, 0), 32);
+                            const uint32_t seen = (hi == 32 ? 0xFFFFFFFFu : (1u << hi) - 1u) & ~(lo == 32 ? 0xFFFFFFFFu : (1u << lo) - 1u);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tmem_st32(t_o + lanes + x, o);
+                            for (int i = 0; i < 32; ++i)
+                                if ((seen & (1u << i)) == 0) s[x + i] = 0xFF800000u;       // -inf
                         }
                     }
-                    l *= f;
-                    m = m_new;
-                }
-                const float ref = m == -INFINITY ? 0.0f : m;           // a row that has seen nothing yet
-                float sum[2] = {0.0f, 0.0f};
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    uint32_t pk[32];
+                    for (int i = 0; i < kTile; i += 4)
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float e0 = fast_exp2(fmaf(__uint_as_float(s[64 * x + 2 * i]), scale2, -ref));
-                        const float e1 = fast_exp2(fmaf(__uint_as_float(s[64 * x + 2 * i + 1]), scale2, -ref));
-                        sum[0] += e0;
-                        sum[1] += e1;
-                        pk[i] = pack_bf16(e0, e1);
+                        for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], __uint_as_float(s[i + e]));
+                    const float tile_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
+                    if (__any_sync(0xFFFFFFFFu, tile_max > m + kRaise)) {
+                        const float m_new = fmaxf(m, tile_max);
+                        const float f = fast_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));
+                        if (j > 0) {
+                            bar_wait(o_done(b ^ 1), ((g + j - 1) >> 1) & 1, c.err, 86);
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int x = 0; x < C::kDv; x += 32) {
+                                uint32_t o[32];
+                                tmem_ld32(t_o + lanes + x, o);
+                                tmem_wait_ld(o, 32);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tmem_st32(t_o + lanes + x, o);
+                            }
+                        }
+                        l *= f;
+                        m = m_new;
                     }
-                    tmem_st32(ts + 32 * x, pk);
+                    const float ref = m == -INFINITY ? 0.0f : m;           // a row that has seen nothing yet
+                    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        uint32_t pk[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const float e0 = fast_exp2(fmaf(__uint_as_float(s[64 * x + 2 * i]), scale2, -ref));
+                            const float e1 = fast_exp2(fmaf(__uint_as_float(s[64 * x + 2 * i + 1]), scale2, -ref));
+                            sum[0] += e0;
+                            sum[1] += e1;
+                            pk[i] = pack_bf16(e0, e1);
+                        }
+                        tmem_st32(ts + 32 * x, pk);
+                    }
+                    l += sum[0] + sum[1];
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive_cluster(in_first_cta(p_full(b)));
                 }
-                l += sum[0] + sum[1];
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive_cluster(in_first_cta(p_full(j & 1)));
-            }
-            // ---------------- epilogue
-            bar_wait(o_done((n - 1) & 1), ((n - 1) >> 1) & 1, c.err, 87);
-            tc_fence_after();
-            if (at.pieces == 1) {
-                // through the ring's memory (nothing is in flight any more), so that a warp writes whole rows
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                constexpr int kChunks = C::kDv / 8;                    // 16-byte chunks of a row
-                const uint32_t rows = s_ring + quarter * (32 * C::kDv * 2);
-                uint8_t* mem = gen + (rows - base);
+                next = find(r + 1);                                    // while the last products run
+                // ---------------- epilogue (before the next work's first weights, so its products do not start yet)
+                bar_wait(o_done((g + n - 1) & 1), ((g + n - 1) >> 1) & 1, c.err, 87);
+                tc_fence_after();
+                const bool last = at.pieces == 1;
+                const float inv = !last ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+                const int64_t row = ((int64_t)at.slot * kCtas + rank) * kTile + row_in;
+                uint16_t* dst = c.a.out + (int64_t)(w.g.q0 + t0 + tok) * c.a.o_t + (int64_t)(h * c.group + row_in % c.group) * c.a.o_h +
+                                half * C::kDv;
+                float* part = c.part_o + row * C::kDv;
 #pragma unroll 1
                 for (int x = 0; x < C::kDv; x += 32) {
                     uint32_t o[32];
                     tmem_ld32(t_o + lanes + x, o);
                     tmem_wait_ld(o, 32);
+                    if (!mine) continue;
+                    if (last) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t pk[4];
+                        for (int i = 0; i < 32; i += 8) {
+                            uint32_t pk[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            pk[e] = pack_bf16(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-                        *reinterpret_cast<uint4*>(mem + (lane * kChunks + ((x / 8 + i) ^ (lane & 7))) * 16) =
-                            make_uint4(pk[0], pk[1], pk[2], pk[3]);
-                    }
-                }
-                __syncwarp();
-                constexpr int kAtOnce = 32 / kChunks;                  // rows of a store
-                const int64_t my_row = mine ? (int64_t)(w.g.q0 + t0 + tok) * c.a.o_t + (int64_t)(h * c.group + r % c.group) * c.a.o_h : -1;
-#pragma unroll 8
-                for (int r0 = 0; r0 < 32; r0 += kAtOnce) {
-                    const int rl = r0 + lane / kChunks, ch = lane % kChunks;
-                    const uint4 v = *reinterpret_cast<const uint4*>(mem + (rl * kChunks + (ch ^ (rl & 7))) * 16);
-                    const int64_t to = __shfl_sync(0xFFFFFFFFu, my_row, rl);
-                    if (to >= 0) *reinterpret_cast<uint4*>(c.a.out + to + half * C::kDv + ch * 8) = v;
-                }
-            } else {
-                const int64_t row = ((int64_t)at.slot * kCtas + rank) * kTile + r;
-                float* dst = c.part_o + row * C::kDv;
-#pragma unroll 1
-                for (int x = 0; x < C::kDv; x += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(t_o + lanes + x, o);
-                    tmem_wait_ld(o, 32);
-                    if (mine) {
+                            for (int e = 0; e < 4; ++e)
+                                pk[e] = pack_bf16(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
+                            *reinterpret_cast<uint4*>(dst + x + i) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                        }
+                    } else {
 #pragma unroll
                         for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<uint4*>(dst + x + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                            *reinterpret_cast<uint4*>(part + x + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                     }
                 }
-                *reinterpret_cast<float2*>(c.part_ml + row * 2) = make_float2(m, l);
+                if (!last) *reinterpret_cast<float2*>(c.part_ml + row * 2) = make_float2(m, l);
+                tc_fence_before();      // the next first weights say that the output has been read
+                g += n;
+                ++done;
             }
         }
     }
@@ -763,18 +790,21 @@ void launch_chunk_dim(const Attn& hd, const AttnCall& a, int few_rows, cudaStrea
     // a sequence has at most one tile that is not full
     const int64_t tiles = std::min<int64_t>((int64_t)a.pv.rows / c.tile_tokens + a.pv.n_seqs,
                                             (int64_t)a.pv.n_seqs * ((a.pv.max_q + c.tile_tokens - 1) / c.tile_tokens));
-    const int64_t ctas = (tiles * a.hk * C::kHalves + c.wave) * C::kCtas;
-    if (ctas > 0x7FFFFFFF) throw Error(G4Q_ERR_INVALID_ARGUMENT, "too many rows for one call");
+    if ((tiles * a.hk * C::kHalves + c.wave) * kMaxSplits > 0x7FFFFFFF)
+        throw Error(G4Q_ERR_INVALID_ARGUMENT, "too many rows for one call");
+    // as many as run at once, unless there can be less work: a tile has at most kMaxSplits pieces, of kMinPiece key tiles
+    int64_t cap = (int64_t)a.pv.max_pages << a.pv.page_shift;
+    if (a.window > 0) cap = std::min<int64_t>(cap, (int64_t)a.window + c.tile_tokens + c.box);
+    const int64_t pieces = std::max<int64_t>(1, (cap + kTile - 1) / kTile / kMinPiece);
+    c.clusters = (int)std::min<int64_t>(c.wave, tiles * a.hk * C::kHalves * std::min<int64_t>(pieces, kMaxSplits));
     c.part_o = hd.part_o;
     c.part_ml = hd.part_ml;
     c.err = device_scratch().err;
     const CUtensorMap tq = rows_map(a.q, a.q_t, a.q_h, a.hq, a.pv.rows, D, c.group, c.tokens);
     const CUtensorMap tk = paged_map(a, a.k, D, c.box), tv = paged_map(a, a.v, D, c.box);
-    launch_dependent<C::kCtas>(attn_chunk_kernel<D>, dim3((unsigned)ctas), dim3(kThreads), C::kSmem, st, tq, tk, tv, c);
-    // no tile is long enough for two pieces: nothing to join
-    int64_t cap = (int64_t)a.pv.max_pages << a.pv.page_shift;
-    if (a.window > 0) cap = std::min<int64_t>(cap, (int64_t)a.window + c.tile_tokens + c.box);
-    if ((cap + kTile - 1) / kTile >= 2 * kMinPiece)
+    launch_dependent<C::kCtas>(attn_chunk_kernel<D>, dim3((unsigned)(c.clusters * C::kCtas)), dim3(kThreads), C::kSmem, st, tq,
+                               tk, tv, c);
+    if (pieces > 1)   // else no tile is long enough for two pieces
         launch_dependent(attn_chunk_join_kernel<D>, dim3(C::kCtas * kTile / kJoinRows, (unsigned)c.wave), dim3(256), 0, st, c);
 }
 
