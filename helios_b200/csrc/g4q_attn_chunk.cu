@@ -5,9 +5,9 @@
 //
 // A tile is 256 query rows of a CTA pair (cta_group::2), 128 to a CTA: floor(128 / group) tokens times the query
 // heads of one key head, so every K and V tile serves the whole group. Each CTA fetches half of a K tile's keys
-// and half of a V tile's columns, and the pair's MMAs read both halves: on single CTAs the fetches of 128 rows' K
-// and V (64 bytes per cycle and SM at head_dim 256) outran L2 and took 3000-4000 cycles a tile. The pair walks
-// the 128-key tiles that its rows see, warp-specialised in each CTA:
+// and half of a V tile's columns, and the pair's MMAs read both halves: on single CTAs, which fetch twice as much,
+// one producer's page look-ups and boxes took 2600-4000 cycles a tile where the products are 2048 (head_dim 256).
+// The pair walks the 128-key tiles that its rows see, warp-specialised in each CTA:
 //   warps 0, 6  fill a ring of K and a ring of V stages (up to 32 KB each) by TMA: boxes of one page x 64 elements,
 //               SWIZZLE_128B. A warp issues a box in about 90 cycles, and pages of 16 slots make 16 boxes a stage: one
 //               warp for both took 3200 cycles a tile.
@@ -18,7 +18,13 @@
 //   warps 2-5   the softmax, one query row per thread: S from TMEM, row maximum, 2^(s - m) rounded to bf16 back
 //               over S. The maximum used, m, is only raised when a row exceeds it by more than 2^8: the weights
 //               stay below 256 (bf16 keeps its relative precision), and the output, which would have to be
-//               rescaled in TMEM, is touched in the first few tiles only. Then O / sum to global memory.
+//               rescaled in TMEM, is touched in the first few tiles only. Then O / sum, whole rows at a time, to global memory.
+//
+// Bound by the tensor cores for a long context: 2048 tokens of 16 heads of 512 over 16384 keys take 960-1010 us back
+// to back, 1.15 ms among other work that draws power (1.34 PFLOP/s of products); a key tile takes 3520 cycles, 87 %
+// of them products. 2048 tokens of 16 heads of 256 with a window of 1024 (9 key tiles a row tile): 45 us, the first
+// softmax and the epilogue of each row tile being latency.
+//
 // head_dim 64: a pair would leave each CTA 32 columns of V, less than a swizzle row, and its tiles' bytes are few
 // for the softmax they take: single CTAs (cta_group::1) run the same code.
 // head_dim 512: O would take all of TMEM, so a CTA computes half of the output columns and the scores whole
@@ -26,7 +32,8 @@
 // The row tiles (x key heads x halves) that fill the GPU in whole waves are computed whole, the longest of a causal
 // chunk first. The rest, which would leave SMs idle for a wave (or all of them, for a drafted block or a small chunk
 // over a long context), have their keys cut into as many pieces as there are CTAs for them, 6 key tiles or more
-// each; a join kernel adds the fp32 partials in piece order.
+// each; a join kernel adds the fp32 partials in piece order. The pairs are as many as fit the GPU, and each walks the
+// list back and forth (the first wave's order, then the reverse, so that a long tile is followed by a short one).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -114,8 +121,9 @@ __device__ __forceinline__ TileWork tile_work(const ChunkCall& c, const SeqGeom&
 }
 
 // The index-th piece of work of the launch, or the index-th tile of the last wave (kLast); b < 0: none. One warp.
-// Tiles of the whole waves come first, each one piece; then the rest's first pieces, second pieces and so on. The longest tiles come first: a sequence's last one, and up to 32 sequences by their lengths (more: the
-// batch's last first).
+// Tiles of the whole waves come first, each one piece; then the rest's first pieces, second pieces and so on.
+// The longest tiles come first: a sequence's last one, and up to 32 sequences by their lengths (more: the batch's last
+// first).
 template <int D, bool kLast>
 __device__ __noinline__ Work find_work(const ChunkCall& c, int index, int lane) {
     constexpr int kHalves = ChunkCfg<D>::kHalves;

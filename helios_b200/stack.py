@@ -516,7 +516,7 @@ class DecoderStack:
             qkv = quantized_matmul(rms_norm(res, L["in_norm"], c.eps), L["qkv"])
             q, k, v = (t.unflatten(1, (-1, d)) for t in qkv.split((self.nq, self.nkv, self.nkv), 1))
             q = kv_append(q, k, v, L["cache"], batch, self.rope, L["q_norm"], L["k_norm"], eps=c.eps)
-            # the last partly filled block of a padded step belongs to no sequence: zeros, not what memory held
+            # rows behind the last sequence are left as they are: zeros, not what memory held, for the o matmul
             out = torch.zeros_like(q)
             attn = self.attend(q, L["cache"], batch, scale=self.scale, window=self.window, out=out)
             if keep is not None:
