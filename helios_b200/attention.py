@@ -167,7 +167,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rope
                  k_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """``rope(rms_norm(q) * q_weight)`` and the same for k, in one launch: q [tokens, q_heads, head_dim],
     k [tokens, kv_heads, head_dim] (views of the q|k|v matmul's output qualify), ``positions`` int32 [tokens].
-    fp32 inside, one rounding at the end. The outputs may be the inputs (in place)."""
+    fp32 inside, one rounding at the end. The outputs may be the inputs (in place), else they must not overlap
+    any other rows of the call."""
     dev = rope.device
     return rope._ops.qk_norm_rope(rope.handle.value, rope.head_dim, dev, _raw_stream(dev), q, k, positions, q_weight, k_weight,
                                   eps, q_out, k_out)

@@ -999,6 +999,46 @@ static void check_heads(const G4qHeadRows* t, int64_t head_dim, const char* name
     if (wrong != nullptr) throw Error(G4Q_ERR_INVALID_ARGUMENT, std::string(name) + wrong);
 }
 
+// Whether two tensors of head rows share elements. Exact where their strides are alike (views of one buffer); else two
+// tensors whose spans overlap are taken to share some.
+static bool heads_overlap(const G4qHeadRows& a, const G4qHeadRows& b, int64_t M, int64_t d) {
+    struct Axes {
+        int64_t outer, inner, span, inner_span;      // strides of the two axes, and extents in elements
+    };
+    auto axes = [&](const G4qHeadRows& t) {
+        const int64_t ts = M > 1 ? t.token_stride : 0, hs = t.n_heads > 1 ? t.head_stride : 0;
+        const bool tokens_out = ts >= hs;
+        Axes x;
+        x.outer = std::max(ts, hs), x.inner = std::min(ts, hs);
+        x.inner_span = x.inner * ((tokens_out ? t.n_heads : M) - 1) + d;
+        x.span = x.outer * ((tokens_out ? M : t.n_heads) - 1) + x.inner_span;
+        return x;
+    };
+    const Axes x = axes(a), y = axes(b);
+    const int64_t gap = b.data - a.data;             // both are 16-byte aligned
+    if (gap >= x.span || -gap >= y.span) return false;
+    if (x.outer != y.outer || x.outer < std::max(x.inner_span, y.inner_span)) return true;
+    auto rows_meet = [&](int64_t g) {                // one row of each, b's g elements on
+        if (g >= x.inner_span || -g >= y.inner_span) return false;
+        if (x.inner != y.inner || x.inner < d) return true;
+        const int64_t r = ((g % x.inner) + x.inner) % x.inner;
+        return r < d || x.inner - r < d;
+    };
+    if (x.outer == 0) return rows_meet(gap);
+    const int64_t r = ((gap % x.outer) + x.outer) % x.outer;
+    return rows_meet(r) || rows_meet(r - x.outer);
+}
+
+// An output of the head norms: the input that its rows come from, or memory that no other rows are in.
+static void check_output(const G4qHeadRows* out, const G4qHeadRows* own, std::initializer_list<const G4qHeadRows*> others,
+                         int64_t M, int64_t d, const char* name) {
+    const bool in_place = out->data == own->data && (M == 1 || out->token_stride == own->token_stride) &&
+                          (out->n_heads == 1 || out->head_stride == own->head_stride);
+    bool bad = !in_place && heads_overlap(*out, *own, M, d);
+    for (const G4qHeadRows* t : others) bad = bad || (t != nullptr && heads_overlap(*out, *t, M, d));
+    if (bad) throw Error(G4Q_ERR_INVALID_ARGUMENT, std::string(name) + " overlaps other rows of the call");
+}
+
 static void check_aligned(const uint16_t* w, const char* name) {
     if ((reinterpret_cast<uintptr_t>(w) & 15u) != 0) require_aligned16(w, name);
 }
@@ -1135,7 +1175,9 @@ G4qStatus g4q_qk_norm_rope(const G4qRope* rope, const G4qHeadRows* q, const G4qH
             check_heads(k_out, r->head_dim, "k_out");
             require(k_out->n_heads == k->n_heads, G4Q_ERR_INVALID_ARGUMENT, "k_out must have k's heads");
             c.k_out = k_out->data, c.ko_t = k_out->token_stride, c.ko_h = k_out->head_stride;
+            check_output(k_out, k, {q, q != nullptr ? q_out : nullptr}, M, r->head_dim, "k_out");
         }
+        if (q != nullptr) check_output(q_out, q, {k}, M, r->head_dim, "q_out");
         launch_head_rows(c, r->head_dim, false, reinterpret_cast<cudaStream_t>(stream));
     });
 }
@@ -1154,6 +1196,7 @@ G4qStatus g4q_kv_append(const G4qRope* rope, const G4qHeadRows* q, const G4qHead
         check_heads(v, r->head_dim, "v");
         require(k->n_heads == cache->n_kv_heads && v->n_heads == cache->n_kv_heads, G4Q_ERR_INVALID_ARGUMENT,
                 "k and v must have the cache's heads");
+        if (q != nullptr) check_output(q_out, q, {k, v}, M, r->head_dim, "q_out");
         c.v = v->data, c.v_t = v->token_stride, c.v_h = v->head_stride, c.hv = v->n_heads;
         c.raw_v = (flags & G4Q_APPEND_RAW_VALUES) ? 1 : 0;
         c.k_out = cache->k, c.v_out = cache->v;
@@ -1242,7 +1285,7 @@ G4qStatus g4q_paged_attention(const G4qAttn* attn, const G4qHeadRows* q, int64_t
                 "q and out must have the handle's query heads");
         require(M == 1 || q->token_stride >= a->head_dim, G4Q_ERR_INVALID_ARGUMENT, "q.token_stride must be >= head_dim");
         // several CTAs read a query row, and one may write its result before another has read it
-        require(out->data != q->data, G4Q_ERR_INVALID_ARGUMENT, "out must not be q");
+        require(!heads_overlap(*out, *q, M, a->head_dim), G4Q_ERR_INVALID_ARGUMENT, "out must not be q, nor overlap it");
         AttnCall c = {};
         c.q = q->data, c.q_t = q->token_stride, c.q_h = q->head_stride;
         c.out = out->data, c.o_t = out->token_stride, c.o_h = out->head_stride;

@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     using C = ChunkCfg<D>;
     constexpr int kCtas = C::kCtas;
     extern __shared__ uint8_t smem_raw[];
-        const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_addr(smem_raw));
     const uint32_t s_q = base, s_ring = s_q + C::kQBytes, s_bar = s_ring + C::kStages * C::kStageBytes;
     auto full = [&](int s) { return s_bar + 8u * s; };
@@ -429,289 +429,287 @@ __global__ void __launch_bounds__(kThreads, 1)
     Work next = find(0);
     uint32_t done = 0;     // tiles of work done, and the key tiles of them: the phases of the barriers go on
     uint32_t g = 0;
-    {
-        if (warp == 0 || warp == 6) {
-            // ---------------- producers: Q and K tiles (warp 0), V tiles (warp 6)
-            const int first_stage = warp == 0 ? 0 : C::kKStages, last_stage = warp == 0 ? C::kKStages : C::kStages;
-            int stage = first_stage;
-            uint32_t round = 0, edge_round = 0;
-            const PagedView& pv = c.a.pv;
-            const int page_mask = (1 << pv.page_shift) - 1;
-            const uint32_t box_bytes = (uint32_t)c.box * 128u;
-            const int boxes = kTile / c.box;             // of a tile of keys; box i is lane i's
-            // The page of this lane's box of tile j, looked up two tiles ahead of its use (the look-up takes as long
-            // as half a tile's products).
-            auto look_up = [&](int j) {
-                const int key = w.lo + (j0 + j) * kTile + lane * c.box;
-                int page = pv.n_pages;                    // outside the map: reads zeros
-                if (j < n && lane < boxes && key < w.any_hi) {
-                    page = pv.table[at.b * pv.table_ld + (key >> pv.page_shift)];
-                    if (page < 0 || page >= pv.n_pages) {
-                        record_input_error(pv.err, kErrPage);
-                        page = pv.n_pages;
-                    }
+    if (warp == 0 || warp == 6) {
+        // ---------------- producers: Q and K tiles (warp 0), V tiles (warp 6)
+        const int first_stage = warp == 0 ? 0 : C::kKStages, last_stage = warp == 0 ? C::kKStages : C::kStages;
+        int stage = first_stage;
+        uint32_t round = 0, edge_round = 0;
+        const PagedView& pv = c.a.pv;
+        const int page_mask = (1 << pv.page_shift) - 1;
+        const uint32_t box_bytes = (uint32_t)c.box * 128u;
+        const int boxes = kTile / c.box;             // of a tile of keys; box i is lane i's
+        // The page of this lane's box of tile j, looked up two tiles ahead of its use (the look-up takes as long
+        // as half a tile's products).
+        auto look_up = [&](int j) {
+            const int key = w.lo + (j0 + j) * kTile + lane * c.box;
+            int page = pv.n_pages;                    // outside the map: reads zeros
+            if (j < n && lane < boxes && key < w.any_hi) {
+                page = pv.table[at.b * pv.table_ld + (key >> pv.page_shift)];
+                if (page < 0 || page >= pv.n_pages) {
+                    record_input_error(pv.err, kErrPage);
+                    page = pv.n_pages;
                 }
-                return page;
-            };
-            // Fills the next stage with boxes [b0, b1) of its keys k0.. (`keys` of them, the first one box `first` of
-            // its tile), columns [col0, col0 + 64 * blocks): at most one box a lane. All of it is worked out before the
-            // stage is free: with two or three stages, what happens between its release and the copies is waited for.
-            auto fill = [&](const CUtensorMap* map, bool edge, int pages, int k0, int keys, int first, int b0, int b1, int col0,
-                            int blocks) {
-                const int box = b0 + lane / blocks, cb = lane % blocks;
-                const int page = __shfl_sync(0xFFFFFFFFu, pages, (first + box) & 31);
-                const uint32_t dst = s_ring + stage * C::kStageBytes + cb * (keys * 128) + box * box_bytes;
-                const int slot = (k0 + box * c.box) & page_mask, count = (b1 - b0) * blocks;
-                const uint32_t bar = edge ? edge_full : in_first_cta(full(stage));
-                if (round > 0) bar_wait(empty(stage), (round - 1) & 1, c.err, 80);
-                if (lane == 0) bar_expect_tx_cluster(bar, (uint32_t)count * box_bytes);
-                __syncwarp();
-                if (lane < count) tma_page<kCtas>(dst, map, col0 + cb * 64, slot, h, page, bar);
-            };
-            auto load_k = [&](int j, int pages) {
-                const int k0 = w.lo + (j0 + j) * kTile + rank * C::kKeysHeld;
-                // a box without a key that some row sees is left out: its scores are masked
-                const int nb = max(0, min(C::kKeysHeld / c.box, (w.any_hi - k0 + c.box - 1) / c.box));
-                for (int p = 0; p < C::kKSt; ++p) {
-                    fill(&tm_k, false, pages, k0, C::kKeysHeld, rank * C::kKeysHeld / c.box, 0, nb, p * C::kKCols, C::kKCols / 64);
-                    if (++stage == last_stage) stage = first_stage, ++round;
-                }
-            };
-            auto load_v = [&](int j, int pages) {
-                const int k0 = w.lo + (j0 + j) * kTile, col0 = half * C::kDv + rank * C::kVCols;
-                const int b1 = max(0, min(boxes, (w.any_hi - k0 + c.box - 1) / c.box));
-                if (k0 >= w.any_lo && k0 + kTile <= w.any_hi) {
-                    fill(&tm_v, false, pages, k0, kTile, 0, 0, boxes, col0, C::kVCols / 64);
-                } else {
-                    // Keys that no row of the tile sees hold anything, and a zero weight times NaN is NaN: the stage
-                    // is filled on a barrier of this CTA's own, their rows are zeroed, and it is handed over then.
-                    const int b0 = max(0, w.any_lo - k0) / c.box;
-                    fill(&tm_v, true, pages, k0, kTile, 0, min(b0, b1), b1, col0, C::kVCols / 64);
-                    bar_wait(edge_full, edge_round++ & 1, c.err, 88);
-                    const int lo = min(kTile, max(0, w.any_lo - k0)), hi = min(kTile, max(lo, w.any_hi - k0));
-                    for (int i = lane; i < (lo + kTile - hi) * (C::kVCols / 8); i += 32) {
-                        const int ch = i & 7, x = i >> 3, cb = x % (C::kVCols / 64);
-                        int row = x / (C::kVCols / 64);
-                        if (row >= lo) row += hi - lo;
-                        *reinterpret_cast<uint4*>(gen + (s_ring - base) + stage * C::kStageBytes + cb * (kTile * 128) + row * 128 +
-                                                  ch * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;\n\tfence.acq_rel.cluster;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) bar_expect_tx_cluster(in_first_cta(full(stage)), 0);
-                }
+            }
+            return page;
+        };
+        // Fills the next stage with boxes [b0, b1) of its keys k0.. (`keys` of them, the first one box `first` of
+        // its tile), columns [col0, col0 + 64 * blocks): at most one box a lane. All of it is worked out before the
+        // stage is free: with two or three stages, what happens between its release and the copies is waited for.
+        auto fill = [&](const CUtensorMap* map, bool edge, int pages, int k0, int keys, int first, int b0, int b1, int col0,
+                        int blocks) {
+            const int box = b0 + lane / blocks, cb = lane % blocks;
+            const int page = __shfl_sync(0xFFFFFFFFu, pages, (first + box) & 31);
+            const uint32_t dst = s_ring + stage * C::kStageBytes + cb * (keys * 128) + box * box_bytes;
+            const int slot = (k0 + box * c.box) & page_mask, count = (b1 - b0) * blocks;
+            const uint32_t bar = edge ? edge_full : in_first_cta(full(stage));
+            if (round > 0) bar_wait(empty(stage), (round - 1) & 1, c.err, 80);
+            if (lane == 0) bar_expect_tx_cluster(bar, (uint32_t)count * box_bytes);
+            __syncwarp();
+            if (lane < count) tma_page<kCtas>(dst, map, col0 + cb * 64, slot, h, page, bar);
+        };
+        auto load_k = [&](int j, int pages) {
+            const int k0 = w.lo + (j0 + j) * kTile + rank * C::kKeysHeld;
+            // a box without a key that some row sees is left out: its scores are masked
+            const int nb = max(0, min(C::kKeysHeld / c.box, (w.any_hi - k0 + c.box - 1) / c.box));
+            for (int p = 0; p < C::kKSt; ++p) {
+                fill(&tm_k, false, pages, k0, C::kKeysHeld, rank * C::kKeysHeld / c.box, 0, nb, p * C::kKCols, C::kKCols / 64);
                 if (++stage == last_stage) stage = first_stage, ++round;
+            }
+        };
+        auto load_v = [&](int j, int pages) {
+            const int k0 = w.lo + (j0 + j) * kTile, col0 = half * C::kDv + rank * C::kVCols;
+            const int b1 = max(0, min(boxes, (w.any_hi - k0 + c.box - 1) / c.box));
+            if (k0 >= w.any_lo && k0 + kTile <= w.any_hi) {
+                fill(&tm_v, false, pages, k0, kTile, 0, 0, boxes, col0, C::kVCols / 64);
+            } else {
+                // Keys that no row of the tile sees hold anything, and a zero weight times NaN is NaN: the stage
+                // is filled on a barrier of this CTA's own, their rows are zeroed, and it is handed over then.
+                const int b0 = max(0, w.any_lo - k0) / c.box;
+                fill(&tm_v, true, pages, k0, kTile, 0, min(b0, b1), b1, col0, C::kVCols / 64);
+                bar_wait(edge_full, edge_round++ & 1, c.err, 88);
+                const int lo = min(kTile, max(0, w.any_lo - k0)), hi = min(kTile, max(lo, w.any_hi - k0));
+                for (int i = lane; i < (lo + kTile - hi) * (C::kVCols / 8); i += 32) {
+                    const int ch = i & 7, x = i >> 3, cb = x % (C::kVCols / 64);
+                    int row = x / (C::kVCols / 64);
+                    if (row >= lo) row += hi - lo;
+                    *reinterpret_cast<uint4*>(gen + (s_ring - base) + stage * C::kStageBytes + cb * (kTile * 128) + row * 128 +
+                                              ch * 16) = make_uint4(0, 0, 0, 0);
+                }
+                asm volatile("fence.proxy.async.shared::cta;\n\tfence.acq_rel.cluster;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) bar_expect_tx_cluster(in_first_cta(full(stage)), 0);
+            }
+            if (++stage == last_stage) stage = first_stage, ++round;
+        };
+        for (int r = 0; r * c.clusters < next.count; ++r) {
+            const bool some = begin(next);
+            next = find(r + 1);
+            if (!some) continue;
+            if (warp == 0) {
+                if (done > 0) bar_wait(q_free, (done - 1) & 1, c.err, 89);
+                if (lane == 0) {
+                    const uint32_t qb = in_first_cta(q_full);
+                    bar_expect_tx_cluster(qb, (uint32_t)(c.tokens * c.group) * 128u * (D / 64));
+                    for (int x = 0; x < D / 64; ++x)
+                        tma_rows<kCtas>(s_q + x * (kTile * 128), &tm_q, x * 64, h * c.group, w.g.q0 + t0, qb);
+                }
+                __syncwarp();
+            }
+            int pages = look_up(0), pages1 = look_up(1);
+            for (int j = 0; j < n; ++j) {
+                const int pages2 = look_up(j + 2);
+                if (warp == 0)
+                    load_k(j, pages);
+                else
+                    load_v(j, pages);
+                pages = pages1;
+                pages1 = pages2;
+            }
+            ++done;
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (of the pair's first CTA)
+        if (rank == 0) {
+            int stage = 0, v_stage = C::kKStages;
+            uint32_t round = 0, v_round = 0;
+            auto scores = [&](int j) {
+                for (int p = 0; p < C::kKSt; ++p) {
+                    bar_wait(full(stage), round & 1, c.err, 81);
+                    tc_fence_after();
+                    if (lane == 0) {
+                        const uint32_t q = desc_low(s_q + p * (C::kKCols / 64) * (kTile * 128), 16);
+                        const uint32_t k = desc_low(s_ring + stage * C::kStageBytes, 16);
+                        const uint32_t d = t_s + ((g + j) & 1) * kTile;
+#pragma unroll
+                        for (int kk = 0; kk < C::kKCols / 16; ++kk)
+                            mma_ss<kCtas>(d, q + ((kk >> 2) * (kTile * 128) + (kk & 3) * 32) / 16,
+                                          k + ((kk >> 2) * (C::kKeysHeld * 128) + (kk & 3) * 32) / 16,
+                                          instr_desc(kTile * kCtas, kTile, false), (p | kk) != 0);
+                        mma_commit<kCtas>(empty(stage));
+                    }
+                    __syncwarp();
+                    if (++stage == C::kKStages) stage = 0, ++round;
+                }
+                if (lane == 0) {
+                    mma_commit<kCtas>(s_full((g + j) & 1));
+                    if (j + 1 == n) mma_commit<kCtas>(q_free);     // Q has been read
+                }
+                __syncwarp();
             };
-            for (int r = 0; r * c.clusters < next.count; ++r) {
-                const bool some = begin(next);
-                next = find(r + 1);
-                if (!some) continue;
-                if (warp == 0) {
-                    if (done > 0) bar_wait(q_free, (done - 1) & 1, c.err, 89);
-                    if (lane == 0) {
-                        const uint32_t qb = in_first_cta(q_full);
-                        bar_expect_tx_cluster(qb, (uint32_t)(c.tokens * c.group) * 128u * (D / 64));
-                        for (int x = 0; x < D / 64; ++x)
-                            tma_rows<kCtas>(s_q + x * (kTile * 128), &tm_q, x * 64, h * c.group, w.g.q0 + t0, qb);
-                    }
-                    __syncwarp();
-                }
-                int pages = look_up(0), pages1 = look_up(1);
-                for (int j = 0; j < n; ++j) {
-                    const int pages2 = look_up(j + 2);
-                    if (warp == 0)
-                        load_k(j, pages);
-                    else
-                        load_v(j, pages);
-                    pages = pages1;
-                    pages1 = pages2;
-                }
-                ++done;
-            }
-        } else if (warp == 1) {
-            // ---------------- MMA issuer (of the pair's first CTA)
-            if (rank == 0) {
-                int stage = 0, v_stage = C::kKStages;
-                uint32_t round = 0, v_round = 0;
-                auto scores = [&](int j) {
-                    for (int p = 0; p < C::kKSt; ++p) {
-                        bar_wait(full(stage), round & 1, c.err, 81);
-                        tc_fence_after();
-                        if (lane == 0) {
-                            const uint32_t q = desc_low(s_q + p * (C::kKCols / 64) * (kTile * 128), 16);
-                            const uint32_t k = desc_low(s_ring + stage * C::kStageBytes, 16);
-                            const uint32_t d = t_s + ((g + j) & 1) * kTile;
-#pragma unroll
-                            for (int kk = 0; kk < C::kKCols / 16; ++kk)
-                                mma_ss<kCtas>(d, q + ((kk >> 2) * (kTile * 128) + (kk & 3) * 32) / 16,
-                                              k + ((kk >> 2) * (C::kKeysHeld * 128) + (kk & 3) * 32) / 16,
-                                              instr_desc(kTile * kCtas, kTile, false), (p | kk) != 0);
-                            mma_commit<kCtas>(empty(stage));
-                        }
-                        __syncwarp();
-                        if (++stage == C::kKStages) stage = 0, ++round;
-                    }
-                    if (lane == 0) {
-                        mma_commit<kCtas>(s_full((g + j) & 1));
-                        if (j + 1 == n) mma_commit<kCtas>(q_free);     // Q has been read
-                    }
-                    __syncwarp();
-                };
-                for (int r = 0; r * c.clusters < next.count; ++r) {
-                    if (!begin(next)) {
-                        next = find(r + 1);
-                        continue;
-                    }
-                    bar_wait(q_full, done & 1, c.err, 82);
-                    scores(0);
-                    for (int j = 0; j < n; ++j) {
-                        if (j + 1 < n) scores(j + 1);
-                        const uint32_t b = (g + j) & 1;
-                        bar_wait(p_full(b), ((g + j) >> 1) & 1, c.err, 83);
-                        bar_wait(full(v_stage), v_round & 1, c.err, 84);
-                        tc_fence_after();
-                        if (lane == 0) {
-                            const uint32_t v = desc_low(s_ring + v_stage * C::kStageBytes, kTile * 128);
-#pragma unroll
-                            for (int kk = 0; kk < kTile / 16; ++kk)
-                                mma_ts<kCtas>(t_o, t_s + b * kTile + kk * 8, v + kk * (2048 / 16),
-                                              instr_desc(kTile * kCtas, C::kDv, true), (j | kk) != 0);
-                            mma_commit<kCtas>(empty(v_stage));
-                            mma_commit<kCtas>(o_done(b));
-                        }
-                        __syncwarp();
-                        if (++v_stage == C::kStages) v_stage = C::kKStages, ++v_round;
-                    }
-                    g += n;
-                    ++done;
-                    next = find(r + 1);                                // while the last products run
-                }
-            }
-        } else {
-            // ---------------- softmax, one row per thread
-            const int quarter = warp & 3;
-            const int row_in = quarter * 32 + lane;
-            const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-            const int tok = row_in / c.group;
-            const float scale2 = c.a.scale * kLog2e;
             for (int r = 0; r * c.clusters < next.count; ++r) {
                 if (!begin(next)) {
                     next = find(r + 1);
                     continue;
                 }
-                const bool mine = tok < c.tokens && t0 + tok < w.g.q_len;
-                int vis_lo = 0, vis_hi = 0;
-                if (mine) {
-                    const int pos = w.g.first + t0 + tok;
-                    vis_hi = min(max(pos + 1, 0), w.g.kv_len);
-                    if (c.a.window > 0) vis_lo = max(0, pos - c.a.window + 1);
-                }
-                // keys that every row of this CTA sees (rows beyond the sequence do not matter)
-                const int all_hi = min(max(w.g.first + t0 + 1, 0), w.g.kv_len);
-                const int all_lo = c.a.window > 0 ? max(0, w.g.first + min(t0 + c.tokens, w.g.q_len) - c.a.window) : 0;
-                float m = -INFINITY, l = 0.0f;
+                bar_wait(q_full, done & 1, c.err, 82);
+                scores(0);
                 for (int j = 0; j < n; ++j) {
-                    const int k0 = w.lo + (j0 + j) * kTile;
-                    const uint32_t b = (g + j) & 1, ts = t_s + b * kTile + lanes;
-                    bar_wait(s_full(b), ((g + j) >> 1) & 1, c.err, 85);
+                    if (j + 1 < n) scores(j + 1);
+                    const uint32_t b = (g + j) & 1;
+                    bar_wait(p_full(b), ((g + j) >> 1) & 1, c.err, 83);
+                    bar_wait(full(v_stage), v_round & 1, c.err, 84);
                     tc_fence_after();
-                    uint32_t s[kTile];
+                    if (lane == 0) {
+                        const uint32_t v = desc_low(s_ring + v_stage * C::kStageBytes, kTile * 128);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, s + 32 * i);
-                    tmem_wait_ld(s, kTile);
-                    if (k0 < all_lo || k0 + kTile > all_hi) {
-#pragma unroll
-                        for (int x = 0; x < kTile; x += 32) {
-                            // bit i: key k0 + x + i is seen
-                            const int lo = min(max(vis_lo - k0 - x, 0), 32), hi = min(max(vis_hi - k0 - x, 0), 32);
-                            const uint32_t seen = (hi == 32 ? 0xFFFFFFFFu : (1u << hi) - 1u) & ~(lo == 32 ? 0xFFFFFFFFu : (1u << lo) - 1u);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if ((seen & (1u << i)) == 0) s[x + i] = 0xFF800000u;       // -inf
-                        }
+                        for (int kk = 0; kk < kTile / 16; ++kk)
+                            mma_ts<kCtas>(t_o, t_s + b * kTile + kk * 8, v + kk * (2048 / 16),
+                                          instr_desc(kTile * kCtas, C::kDv, true), (j | kk) != 0);
+                        mma_commit<kCtas>(empty(v_stage));
+                        mma_commit<kCtas>(o_done(b));
                     }
-                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int i = 0; i < kTile; i += 4)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], __uint_as_float(s[i + e]));
-                    const float tile_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
-                    if (__any_sync(0xFFFFFFFFu, tile_max > m + kRaise)) {
-                        const float m_new = fmaxf(m, tile_max);
-                        const float f = fast_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));
-                        if (j > 0) {
-                            bar_wait(o_done(b ^ 1), ((g + j - 1) >> 1) & 1, c.err, 86);
-                            tc_fence_after();
-#pragma unroll 1
-                            for (int x = 0; x < C::kDv; x += 32) {
-                                uint32_t o[32];
-                                tmem_ld32(t_o + lanes + x, o);
-                                tmem_wait_ld(o, 32);
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                                tmem_st32(t_o + lanes + x, o);
-                            }
-                        }
-                        l *= f;
-                        m = m_new;
-                    }
-                    const float ref = m == -INFINITY ? 0.0f : m;           // a row that has seen nothing yet
-                    float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        uint32_t pk[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const float e0 = fast_exp2(fmaf(__uint_as_float(s[64 * x + 2 * i]), scale2, -ref));
-                            const float e1 = fast_exp2(fmaf(__uint_as_float(s[64 * x + 2 * i + 1]), scale2, -ref));
-                            sum[0] += e0;
-                            sum[1] += e1;
-                            pk[i] = pack_bf16(e0, e1);
-                        }
-                        tmem_st32(ts + 32 * x, pk);
-                    }
-                    l += sum[0] + sum[1];
-                    tmem_wait_st();
-                    tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) bar_arrive_cluster(in_first_cta(p_full(b)));
+                    if (++v_stage == C::kStages) v_stage = C::kKStages, ++v_round;
                 }
-                next = find(r + 1);                                    // while the last products run
-                // ---------------- epilogue (before the next work's first weights, so its products do not start yet)
-                bar_wait(o_done((g + n - 1) & 1), ((g + n - 1) >> 1) & 1, c.err, 87);
-                tc_fence_after();
-                const bool last = at.pieces == 1;
-                const float inv = !last ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-                const int64_t row = ((int64_t)at.slot * kCtas + rank) * kTile + row_in;
-                uint16_t* dst = c.a.out + (int64_t)(w.g.q0 + t0 + tok) * c.a.o_t + (int64_t)(h * c.group + row_in % c.group) * c.a.o_h +
-                                half * C::kDv;
-                float* part = c.part_o + row * C::kDv;
-#pragma unroll 1
-                for (int x = 0; x < C::kDv; x += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(t_o + lanes + x, o);
-                    tmem_wait_ld(o, 32);
-                    if (!mine) continue;
-                    if (last) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            uint32_t pk[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                pk[e] = pack_bf16(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
-                            *reinterpret_cast<uint4*>(dst + x + i) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<uint4*>(part + x + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                    }
-                }
-                if (!last) *reinterpret_cast<float2*>(c.part_ml + row * 2) = make_float2(m, l);
-                tc_fence_before();      // the next first weights say that the output has been read
                 g += n;
                 ++done;
+                next = find(r + 1);                                // while the last products run
             }
+        }
+    } else {
+        // ---------------- softmax, one row per thread
+        const int quarter = warp & 3;
+        const int row_in = quarter * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const int tok = row_in / c.group;
+        const float scale2 = c.a.scale * kLog2e;
+        for (int r = 0; r * c.clusters < next.count; ++r) {
+            if (!begin(next)) {
+                next = find(r + 1);
+                continue;
+            }
+            const bool mine = tok < c.tokens && t0 + tok < w.g.q_len;
+            int vis_lo = 0, vis_hi = 0;
+            if (mine) {
+                const int pos = w.g.first + t0 + tok;
+                vis_hi = min(max(pos + 1, 0), w.g.kv_len);
+                if (c.a.window > 0) vis_lo = max(0, pos - c.a.window + 1);
+            }
+            // keys that every row of this CTA sees (rows beyond the sequence do not matter)
+            const int all_hi = min(max(w.g.first + t0 + 1, 0), w.g.kv_len);
+            const int all_lo = c.a.window > 0 ? max(0, w.g.first + min(t0 + c.tokens, w.g.q_len) - c.a.window) : 0;
+            float m = -INFINITY, l = 0.0f;
+            for (int j = 0; j < n; ++j) {
+                const int k0 = w.lo + (j0 + j) * kTile;
+                const uint32_t b = (g + j) & 1, ts = t_s + b * kTile + lanes;
+                bar_wait(s_full(b), ((g + j) >> 1) & 1, c.err, 85);
+                tc_fence_after();
+                uint32_t s[kTile];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, s + 32 * i);
+                tmem_wait_ld(s, kTile);
+                if (k0 < all_lo || k0 + kTile > all_hi) {
+#pragma unroll
+                    for (int x = 0; x < kTile; x += 32) {
+                        // bit i: key k0 + x + i is seen
+                        const int lo = min(max(vis_lo - k0 - x, 0), 32), hi = min(max(vis_hi - k0 - x, 0), 32);
+                        const uint32_t seen = (hi == 32 ? 0xFFFFFFFFu : (1u << hi) - 1u) & ~(lo == 32 ? 0xFFFFFFFFu : (1u << lo) - 1u);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if ((seen & (1u << i)) == 0) s[x + i] = 0xFF800000u;       // -inf
+                    }
+                }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < kTile; i += 4)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], __uint_as_float(s[i + e]));
+                const float tile_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
+                if (__any_sync(0xFFFFFFFFu, tile_max > m + kRaise)) {
+                    const float m_new = fmaxf(m, tile_max);
+                    const float f = fast_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));
+                    if (j > 0) {
+                        bar_wait(o_done(b ^ 1), ((g + j - 1) >> 1) & 1, c.err, 86);
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int x = 0; x < C::kDv; x += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(t_o + lanes + x, o);
+                            tmem_wait_ld(o, 32);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st32(t_o + lanes + x, o);
+                        }
+                    }
+                    l *= f;
+                    m = m_new;
+                }
+                const float ref = m == -INFINITY ? 0.0f : m;           // a row that has seen nothing yet
+                float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float e0 = fast_exp2(fmaf(__uint_as_float(s[64 * x + 2 * i]), scale2, -ref));
+                        const float e1 = fast_exp2(fmaf(__uint_as_float(s[64 * x + 2 * i + 1]), scale2, -ref));
+                        sum[0] += e0;
+                        sum[1] += e1;
+                        pk[i] = pack_bf16(e0, e1);
+                    }
+                    tmem_st32(ts + 32 * x, pk);
+                }
+                l += sum[0] + sum[1];
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive_cluster(in_first_cta(p_full(b)));
+            }
+            next = find(r + 1);                                    // while the last products run
+            // ---------------- epilogue (before the next work's first weights, so its products do not start yet)
+            bar_wait(o_done((g + n - 1) & 1), ((g + n - 1) >> 1) & 1, c.err, 87);
+            tc_fence_after();
+            const bool last = at.pieces == 1;
+            const float inv = !last ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+            const int64_t row = ((int64_t)at.slot * kCtas + rank) * kTile + row_in;
+            uint16_t* dst = c.a.out + (int64_t)(w.g.q0 + t0 + tok) * c.a.o_t + (int64_t)(h * c.group + row_in % c.group) * c.a.o_h +
+                            half * C::kDv;
+            float* part = c.part_o + row * C::kDv;
+#pragma unroll 1
+            for (int x = 0; x < C::kDv; x += 32) {
+                uint32_t o[32];
+                tmem_ld32(t_o + lanes + x, o);
+                tmem_wait_ld(o, 32);
+                if (!mine) continue;
+                if (last) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        uint32_t pk[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            pk[e] = pack_bf16(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
+                        *reinterpret_cast<uint4*>(dst + x + i) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<uint4*>(part + x + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                }
+            }
+            if (!last) *reinterpret_cast<float2*>(c.part_ml + row * 2) = make_float2(m, l);
+            tc_fence_before();      // the next first weights say that the output has been read
+            g += n;
+            ++done;
         }
     }
     // The pair's MMAs read both CTAs' shared memory and signal both: neither leaves before the other is done.

@@ -338,14 +338,15 @@ G4qStatus g4q_rope_free(G4qRope* rope);
 /* q_out = rope(rms_norm(q) * q_weight), k_out = rope(rms_norm(k) * k_weight) for M tokens at `positions`
  * (device int32 [M]), in one launch, fp32 inside with one rounding at the end. Weights: bf16 [head_dim] or
  * NULL (none). q (with q_out) or k (with k_out) may be NULL. An output may be its input (same data and
- * strides); otherwise they must not overlap. */
+ * strides); otherwise it must not overlap any other rows of the call. */
 G4qStatus g4q_qk_norm_rope(const G4qRope* rope, const G4qHeadRows* q, const G4qHeadRows* k, int64_t M,
                            const int32_t* positions, const uint16_t* q_weight, const uint16_t* k_weight, float eps,
                            const G4qHeadRows* q_out, const G4qHeadRows* k_out, void* stream);
 
 /* The same on the new tokens of a paged batch, at their positions in it: the keys are stored in the cache's
  * pages, the values beside them (rms_norm without a weight; with G4Q_APPEND_RAW_VALUES as they are). v may be
- * k (full-attention layers, whose key projection is the value too: :820-822). q (with q_out) may be NULL. */
+ * k (full-attention layers, whose key projection is the value too: :820-822). q (with q_out) may be NULL; q_out
+ * may be q, else it must not overlap q, k or v. */
 #define G4Q_APPEND_RAW_VALUES 0x1u
 G4qStatus g4q_kv_append(const G4qRope* rope, const G4qHeadRows* q, const G4qHeadRows* k, const G4qHeadRows* v, int64_t M,
                         const uint16_t* q_weight, const uint16_t* k_weight, float eps, uint32_t flags,
@@ -353,11 +354,11 @@ G4qStatus g4q_kv_append(const G4qRope* rope, const G4qHeadRows* q, const G4qHead
 
 /* out = softmax(scale * q . k^T) v over the cache, query head h against key head h / (n_q_heads / n_kv_heads);
  * the query at position t sees the keys j <= t, and j > t - window when window > 0. Single tokens, drafted
- * blocks and prompt chunks may be mixed in one call. A row that sees no key is zero. out must not overlap q. What the cache holds at
- * slots that no query of a sequence's step sees does not matter (NaN included); a non-finite value that some
- * query of the step sees may reach the step's other queries of that sequence. The handle owns the scratch of
- * partial results: calls on one handle must not overlap on the GPU (one stream, or events), replays of graphs
- * that captured it included. Allocates nothing. */
+ * blocks and prompt chunks may be mixed in one call. A row that sees no key is zero. out must not overlap q.
+ * What the cache holds at slots that no query of a sequence's step sees does not matter (NaN included); a
+ * non-finite value that some query of the step sees may reach the step's other queries of that sequence. The
+ * handle owns the scratch of partial results: calls on one handle must not overlap on the GPU (one stream, or
+ * events), replays of graphs that captured it included. Allocates nothing. */
 typedef struct G4qAttn G4qAttn;
 G4qStatus g4q_attn_create(int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, G4qAttn** out);
 G4qStatus g4q_paged_attention(const G4qAttn* attn, const G4qHeadRows* q, int64_t M, const G4qPagedCache* cache,

@@ -1,6 +1,9 @@
 """GPU: head norms with rotation, append to a paged cache and attention over it, against 64-bit forms on the CPU.
 Tolerances are the bounds of attn_ref.py."""
 import ctypes
+import pathlib
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -445,6 +448,96 @@ def test_refusals(cuda):
     attend.free()
     with pytest.raises(ValueError, match="freed"):
         attend(q, s.cache, s.batch)
+
+
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_outputs_that_overlap_inputs(cuda, tokens):
+    """Views of one buffer qualify while no element is shared; anything else is refused before a launch."""
+    from helios_b200 import attention as A
+    d, hq, hk = 64, 4, 2
+    rope = A.Rope(d)
+    pos = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    base = randn(tokens, 2 * hq + 2 * hk, d, seed=1)
+    q, k = base[:, :hq].clone(), base[:, hq:hq + hk].clone()
+    want_q, want_k = A.qk_norm_rope(q, k, pos, rope)
+
+    def run(views):
+        buf = base.clone()
+        flat = torch.zeros(tokens * (2 * hq + 2 * hk) * d + 64, dtype=torch.bfloat16, device="cuda")
+        qv, kv, qo, ko = views(buf, flat)
+        qv.copy_(q), kv.copy_(k)
+        got = A.qk_norm_rope(qv, kv, pos, rope, q_out=qo, k_out=ko)
+        assert torch.equal(got[0], want_q) and torch.equal(got[1], want_k)
+
+    # behind each other in a token's row, in place, heads in turn, heads outside of the tokens
+    run(lambda b, f: (b[:, :hq], b[:, hq:hq + hk], b[:, hq + hk:2 * hq + hk], b[:, 2 * hq + hk:]))
+    run(lambda b, f: (b[:, :hq], b[:, hq:hq + hk], b[:, :hq], b[:, hq:hq + hk]))
+    run(lambda b, f: (b[:, 0:2 * hq:2], b[:, 2 * hq:2 * hq + hk], b[:, 1:2 * hq:2], b[:, 2 * hq + hk:]))
+    run(lambda b, f: (f[:tokens * hq * d].view(hq, tokens, d).transpose(0, 1), b[:, :hk],
+                      f[tokens * hq * d:2 * tokens * hq * d].view(hq, tokens, d).transpose(0, 1), b[:, hk:2 * hk]))
+    # a head on, half a head on, the other one's rows, the other output's rows
+    bad = [lambda b, f: (b[:, :hq], b[:, 2 * hq:2 * hq + hk], b[:, 1:hq + 1], b[:, 2 * hq + hk:]),
+           lambda b, f: (f[:tokens * hq * d].view(tokens, hq, d), b[:, :hk],
+                         f[32:tokens * hq * d + 32].view(tokens, hq, d), b[:, hk:2 * hk]),
+           lambda b, f: (b[:, :hq], b[:, hq:hq + hk], b[:, hq:2 * hq], b[:, 2 * hq:2 * hq + hk]),
+           lambda b, f: (b[:, :hq], b[:, hq:hq + hk], b[:, 2 * hk + hq:], b[:, hq + hk + 1:hq + 2 * hk + 1]),
+           lambda b, f: (b[:, :hq], b[:, hq:hq + hk], b[:, :hq], b[:, :hk])]
+    for views in bad:
+        with pytest.raises(ValueError, match="overlaps other rows"):
+            run(views)
+
+    s = Step([tokens], [20], hk, d, 16, 1)
+    attend = A.PagedAttention(hq, hk, d)
+    want = attend(q, s.cache, s.batch)
+    buf = base.clone()
+    buf[:, :hq].copy_(q)
+    assert torch.equal(attend(buf[:, :hq], s.cache, s.batch, out=buf[:, hq:2 * hq]), want)
+    with pytest.raises(ValueError, match="out must not be q"):
+        attend(buf[:, :hq], s.cache, s.batch, out=buf[:, 1:hq + 1])
+    no_device_error()
+
+
+def test_chunk_of_one_query_head_without_a_head_stride(cuda):
+    """The stride of a single head is not used: zero qualifies at the C interface, for a chunk as for few rows."""
+    from helios_b200 import _lib
+    from helios_b200 import attention as A
+    s = Step([100], [130], 1, 64, 16, 2)
+    q, out = randn(100, 1, 64, seed=3), torch.zeros(100, 1, 64, dtype=torch.bfloat16, device="cuda")
+    attend = A.PagedAttention(1, 1, 64)
+    rows = [_lib.G4qHeadRows(t.data_ptr(), 64, 0, 1) for t in (q, out)]
+    _lib.call("g4q_paged_attention", attend.handle, ctypes.byref(rows[0]), 100, ctypes.byref(s.cache.c),
+              ctypes.byref(s.batch._view(16)), 0.125, 0, ctypes.byref(rows[1]), torch.cuda.current_stream().cuda_stream)
+    close(out, *s.reference(q, 0.125, 0))
+
+
+def test_first_calls_inside_a_capture(cuda):
+    """A process whose first calls are captured: nothing of theirs needs a run before."""
+    code = """
+import torch
+from helios_b200 import _lib, attention as A
+torch.manual_seed(0)
+def make(n, kv):
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    return A.PagedBatch(t([0, n]), t([kv]), t([list(range(16))]), max_q=n)
+rope, attend, cache = A.Rope(128), A.PagedAttention(4, 2, 128), A.PagedKVCache.allocate(16, 32, 2, 128)
+cache.k.normal_(), cache.v.normal_()
+q, k, v = (torch.randn(150, h, 128, device="cuda").bfloat16() for h in (4, 2, 2))
+few, many = make(2, 500), make(150, 400)
+def step():
+    return [attend(A.kv_append(q[:n], k[:n], v[:n], cache, b, rope), cache, b) for n, b in ((2, few), (150, many))]
+g = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(g):
+    out = step()
+g.replay()          # appends: from here on the cache holds the same keys before and after a step
+want = step()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, want)) and _lib.device_error() == 0
+"""
+    root = pathlib.Path(__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 def test_step_replays_in_a_cuda_graph_with_new_lengths(cuda):
