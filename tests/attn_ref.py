@@ -9,8 +9,9 @@ of half a step:
   and the hardware sine and cosine 2^-21.2 = 7 u: below 2^-19 = 32 u of |y_i| + |y_j| of the pair.
 * attention: each score is a sum of D exact products in fp32, off by at most D 2^-23 sum|q k|, the sum's
   running value being at most that; the exponential and the running rescaling add 2^-20 relative. A weight is
-  rounded to bf16 (2^-9 to either side), and the sum of the weights takes them rounded, so numerator and
-  denominator are each off by 2^-9 relative at most: 2^-8 of sum(p |v|), plus twice the scores' error.
+  rounded to bf16, p (1 + e) with |e| <= 2^-8. With the sum of the rounded weights below, the output is off by
+  sum(p e (v - o)), at most 2^-8 (sum(p |v|) + |o|); with the sum of the weights as they were (chunks), by
+  sum(p e v), which is less. The scores' error, of numerator and denominator, counts twice in sum(p |v|).
 """
 import torch
 
@@ -86,5 +87,6 @@ def attention(q, k_pages, v_pages, q_offsets, kv_lens, table, scale, window):
             p = p / torch.where(total > 0, total, 1.0)
             o = p @ v[:, kh]
             out[q0:q1, h] = o
-            bound[q0:q1, h] = half_step(o) + (p @ v[:, kh].abs()) * (2.0 ** -8 + 2.0 ** -20 + 2 * s_err) + 2.0 ** -126
+            bound[q0:q1, h] = half_step(o) + (p @ v[:, kh].abs()) * (2.0 ** -8 + 2.0 ** -20 + 2 * s_err) \
+                + 2.0 ** -8 * o.abs() + 2.0 ** -126
     return out, bound

@@ -346,6 +346,43 @@ def test_attention_strided_queries_and_output(cuda):
     close(out, *s.reference(q, 128 ** -0.5, 0))
 
 
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 2], [130, 64]), ([100], [130])])
+def test_offsets_beyond_32_bits(cuda, q_lens, kv_lens):
+    """Pages 2^31 elements apart and token rows 2^25 or 2^30 apart: append and attention of few rows and of a chunk."""
+    from helios_b200 import attention as A
+    d, hk, hq, page, pages = 64, 2, 4, 64, 4
+    n = sum(q_lens)
+    apart = 2 ** 30 if n < 4 else 2 ** 25
+    big = torch.empty(3 * 2 ** 31 + 2 ** 20, dtype=torch.bfloat16, device="cuda")
+    strides = (2 ** 31, page * d, d, 1)
+    kd = big.as_strided((pages, hk, page, d), strides, 0)
+    vd = big.as_strided((pages, hk, page, d), strides, 2 ** 16)
+    q = big.as_strided((n, hq, d), (apart, d, 1), 2 ** 17)
+    k, v = (big.as_strided((n, hk, d), (apart, d, 1), 2 ** 17 + i * 2 ** 12) for i in (1, 2))
+    out = big.as_strided((n, hq, d), (apart, d, 1), 2 ** 17 + 3 * 2 ** 12)
+    s = Step(q_lens, kv_lens, hk, d, page, 51, spare=0)
+    for i in range(s.kc.shape[0]):                     # the cache's pages, from the far end
+        kd[pages - 1 - i], vd[pages - 1 - i] = s.kc[i].cuda(), s.vc[i].cuda()
+    s.t_table.copy_(torch.where(s.table >= 0, pages - 1 - s.table, -1))
+    fresh = [randn(n, h, d, seed=52 + i) for i, h in enumerate((hq, hk, hk))]
+    for to, x in zip((q, k, v), fresh):
+        to.copy_(x)
+    cache, rope = A.PagedKVCache(kd, vd), A.Rope(d)
+    attend = A.PagedAttention(hq, hk, d)
+    A.kv_append(q, k, v, cache, s.batch, rope, q_out=q)
+    attend(q, cache, s.batch, out=out)
+    want_q = A.kv_append(*fresh, s.cache, A.PagedBatch(s.t_off, s.t_kv, s.table.cuda(), max_q=max(q_lens)), rope)
+    assert torch.equal(q, want_q)
+    for b, (m, far) in enumerate(zip(kv_lens, s.t_table.tolist())):
+        for p in range(-(-m // page)):
+            near, held = int(s.table[b, p]), min(page, m - p * page)
+            assert torch.equal(kd[far[p], :, :held], s.cache.k[near, :, :held])
+            assert torch.equal(vd[far[p], :, :held], s.cache.v[near, :, :held])
+    s.kc, s.vc = s.cache.k.cpu(), s.cache.v.cpu()
+    close(out, *s.reference(want_q, d ** -0.5, 0))
+    no_device_error()
+
+
 def test_page_ids_and_lengths_outside_are_reported_and_touch_nothing(cuda):
     from helios_b200 import _lib
     from helios_b200 import attention as A
