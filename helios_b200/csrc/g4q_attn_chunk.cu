@@ -46,7 +46,9 @@ namespace g4q {
 namespace {
 
 constexpr int kTile = 128;             // query rows and keys of a tile
-constexpr int kThreads = 224;
+constexpr int kThreads = 352;
+constexpr int kSoftWarps = 8;          // of the softmax: warps 2..9
+constexpr int kVWarp = 10;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 8.0f;         // how far (log2) a score may exceed the maximum in use
 constexpr uint32_t kTmemCols = 512;
@@ -64,11 +66,12 @@ struct ChunkCfg {
     static constexpr int kVCols = kDv / kCtas;               // V stage: 128 keys x kVCols elements
     static constexpr int kStageBytes = kTile * kVCols * 2;
     static constexpr int kQBytes = kTile * D * 2;
-    static constexpr int kFit = (227 * 1024 - 1024 - 256 - kQBytes) / kStageBytes;
+    static constexpr int kTail = 256 + 2 * 2 * kTile * 4;    // barriers, and the row maxima of two halves and two tiles
+    static constexpr int kFit = (227 * 1024 - kTail - kQBytes) / kStageBytes;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     static constexpr int kVStages = kStages / 2 < 1 ? 1 : (kStages - (kKSt - 1)) / 2;   // of the ring of V tiles
     static constexpr int kKStages = kStages - kVStages;                                 // of the ring of K tiles
-    static constexpr int kSmem = 1024 + kQBytes + kStages * kStageBytes + 256;
+    static constexpr int kSmem = kQBytes + kStages * kStageBytes + kTail;
     static_assert(kKeysHeld / 16 * (kKCols / 64) <= 32 && kTile / 16 * (kVCols / 64) <= 32, "a lane issues one box of a stage");
     static_assert(kKeysHeld * kKCols == kTile * kVCols && kVCols % 64 == 0, "stages hold either operand");
     static_assert(kVStages >= 1 && kKStages >= kKSt, "a tile of each fits");
@@ -83,7 +86,7 @@ struct ChunkCall {
     int box;
     int wave;            // tiles that the GPU computes at once
     int clusters;        // CTAs or CTA pairs of the launch
-    float* part_o;       // [pieces, at most a wave][CTAs of a tile * 128][output columns of a CTA]
+    float* part_o;       // [pieces, at most a wave][CTAs of a tile][output columns of a CTA / 4][128 rows][4]
     float* part_ml;      // [pieces][CTAs of a tile * 128][2]
     int* err;
 };
@@ -265,6 +268,15 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
+// True for one thread of a converged warp. The compiler knows that the code behind it is one thread's, and keeps the
+// operands of the MMAs in uniform registers: with a test of the lane it moved them there before every MMA, 65 to 85
+// cycles each (2048 tokens, 16384 keys of head_dim 512: 970 us against 900).
+__device__ __forceinline__ bool elect() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
 // The address of the same shared-memory object in the first CTA of the cluster.
 __device__ __forceinline__ uint32_t in_first_cta(uint32_t addr) {
     uint32_t r;
@@ -283,9 +295,9 @@ __device__ __forceinline__ void bar_expect_tx_cluster(uint32_t bar, uint32_t byt
     asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
+// The two steps of a barrier of the pair.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* v) {
     asm volatile(
@@ -348,15 +360,34 @@ __device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, i
         tma_load_page(dst, map, x, slot, head, page, bar);
 }
 
+// Four lanes with four 16-byte chunks each, of a row of their own: afterwards lane i has chunk i of all four rows.
+__device__ __forceinline__ void quad_transpose(uint32_t (&ch)[4][4], int lane) {
+#pragma unroll
+    for (int bit = 1; bit < 4; bit <<= 1) {
+        const bool upper = (lane & bit) != 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if ((i & bit) != 0) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, upper ? ch[i][e] : ch[i + bit][e], bit);
+                if (upper)
+                    ch[i][e] = got;
+                else
+                    ch[i + bit][e] = got;
+            }
+        }
+    }
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ ChunkCall c) {
     using C = ChunkCfg<D>;
     constexpr int kCtas = C::kCtas;
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
-    uint8_t* gen = smem_raw + (base - smem_addr(smem_raw));
+    extern __shared__ __align__(1024) uint8_t gen[];     // SWIZZLE_128B repeats every 1024 bytes
+    const uint32_t base = smem_addr(gen);
     const uint32_t s_q = base, s_ring = s_q + C::kQBytes, s_bar = s_ring + C::kStages * C::kStageBytes;
     auto full = [&](int s) { return s_bar + 8u * s; };
     auto empty = [&](int s) { return s_bar + 8u * (C::kStages + s); };
@@ -366,6 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto o_done = [&](int b) { return q_full + 8u + 8u * b; };    // products of the even and the odd tiles
     const uint32_t edge_full = q_full + 24, q_free = q_full + 32;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (s_bar - base) + 8u * (2 * C::kStages + 9));
+    float* s_max = reinterpret_cast<float*>(gen + (s_bar - base) + 256);     // [parity of the tile][half][row]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = blockIdx.x % kCtas;                 // place in the pair
@@ -387,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             bar_init(s_full(b), 1);
-            bar_init(p_full(b), 4 * kCtas);       // every softmax warp of the pair
+            bar_init(p_full(b), kSoftWarps * kCtas);     // every softmax warp of the pair
             bar_init(o_done(b), 1);
         }
         bar_init(q_full, kCtas);
@@ -397,14 +429,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (const CUtensorMap* map : {&tm_q, &tm_k, &tm_v})
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
     }
-    wait_for_predecessor();
-    release_successor();
     tc_fence_before();
     __syncthreads();
-    if constexpr (kCtas == 2) cluster_sync();
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
-    const uint32_t t_o = tmem, t_s = tmem + 256;     // output, two score buffers of 128 columns
+    if constexpr (kCtas == 2) cluster_arrive();
+    wait_for_predecessor();
+    release_successor();
 
     // The work of this cluster: every warp walks the same list, the way back and forth over the clusters, so that who
     // had a long tile in one round has a short one in the next.
@@ -413,6 +442,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     int t0 = 0, j0 = 0, n = 0, h = 0, half = 0;
     auto find = [&](int r) {
         return find_work<D, false>(c, r * c.clusters + ((r & 1) ? c.clusters - 1 - cluster : cluster), lane);
+    };
+    auto find_next = [&](int r, Work now) {         // after `now`, of round r - 1
+        if (r * c.clusters < now.count) return find(r);
+        now.b = -1;
+        return now;
     };
     auto begin = [&](const Work& next) {
         at = next;
@@ -427,10 +461,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
     };
     Work next = find(0);
+    if constexpr (kCtas == 2) cluster_wait();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t t_o = tmem, t_s = tmem + 256;     // output, two score buffers of 128 columns
     uint32_t done = 0;     // tiles of work done, and the key tiles of them: the phases of the barriers go on
     uint32_t g = 0;
-    if (warp == 0 || warp == 6) {
-        // ---------------- producers: Q and K tiles (warp 0), V tiles (warp 6)
+    if (warp == 0 || warp == kVWarp) {
+        // ---------------- producers: Q and K tiles (warp 0), V tiles (kVWarp)
         const int first_stage = warp == 0 ? 0 : C::kKStages, last_stage = warp == 0 ? C::kKStages : C::kStages;
         int stage = first_stage;
         uint32_t round = 0, edge_round = 0;
@@ -503,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         for (int r = 0; r * c.clusters < next.count; ++r) {
             const bool some = begin(next);
-            next = find(r + 1);
+            next = find_next(r + 1, next);
             if (!some) continue;
             if (warp == 0) {
                 if (done > 0) bar_wait(q_free, (done - 1) & 1, c.err, 89);
@@ -536,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int p = 0; p < C::kKSt; ++p) {
                     bar_wait(full(stage), round & 1, c.err, 81);
                     tc_fence_after();
-                    if (lane == 0) {
+                    if (elect()) {
                         const uint32_t q = desc_low(s_q + p * (C::kKCols / 64) * (kTile * 128), 16);
                         const uint32_t k = desc_low(s_ring + stage * C::kStageBytes, 16);
                         const uint32_t d = t_s + ((g + j) & 1) * kTile;
@@ -550,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __syncwarp();
                     if (++stage == C::kKStages) stage = 0, ++round;
                 }
-                if (lane == 0) {
+                if (elect()) {
                     mma_commit<kCtas>(s_full((g + j) & 1));
                     if (j + 1 == n) mma_commit<kCtas>(q_free);     // Q has been read
                 }
@@ -558,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             for (int r = 0; r * c.clusters < next.count; ++r) {
                 if (!begin(next)) {
-                    next = find(r + 1);
+                    next = find_next(r + 1, next);
                     continue;
                 }
                 bar_wait(q_full, done & 1, c.err, 82);
@@ -569,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     bar_wait(p_full(b), ((g + j) >> 1) & 1, c.err, 83);
                     bar_wait(full(v_stage), v_round & 1, c.err, 84);
                     tc_fence_after();
-                    if (lane == 0) {
+                    if (elect()) {
                         const uint32_t v = desc_low(s_ring + v_stage * C::kStageBytes, kTile * 128);
 #pragma unroll
                         for (int kk = 0; kk < kTile / 16; ++kk)
@@ -583,19 +621,37 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 g += n;
                 ++done;
-                next = find(r + 1);                                // while the last products run
+                next = find_next(r + 1, next);                     // while the last products run
             }
         }
     } else {
-        // ---------------- softmax, one row per thread
-        const int quarter = warp & 3;
+        // ---------------- softmax: two threads to a row, in warps w and w + 4, which reach the same TMEM lanes; each
+        // has 64 of a tile's keys and half of the output columns
+        const int quarter = warp & 3, side = (warp - 2) >> 2;
         const int row_in = quarter * 32 + lane;
+        constexpr int kKeys = kTile / 2, kCols = C::kDv / 2;
+        uint32_t swaps = 0;
+        // The other thread's value. Two places in turn: the next write to one comes after the barrier that its reader
+        // has to reach first.
+        auto swap = [&](float v) {
+            float* at = s_max + (swaps++ & 1) * (2 * kTile) + row_in;
+            at[side * kTile] = v;
+            tc_fence_before();
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+            tc_fence_after();
+            return at[(side ^ 1) * kTile];
+        };
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const int tok = row_in / c.group;
         const float scale2 = c.a.scale * kLog2e;
-        for (int r = 0; r * c.clusters < next.count; ++r) {
-            if (!begin(next)) {
-                next = find(r + 1);
+        for (int r = 0;; ++r) {
+            // Both warps take the same steps whatever they have read: lengths that change under a running kernel are an
+            // error, but the barrier between the two has no limit of its own, so they agree on the number first.
+            const int steps = r * c.clusters >= next.count ? -1 : begin(next) ? n : 0;
+            n = min(steps, __float_as_int(swap(__int_as_float(steps))));
+            if (n < 0) break;
+            if (n == 0) {
+                next = find_next(r + 1, next);
                 continue;
             }
             const bool mine = tok < c.tokens && t0 + tok < w.g.q_len;
@@ -610,17 +666,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int all_lo = c.a.window > 0 ? max(0, w.g.first + min(t0 + c.tokens, w.g.q_len) - c.a.window) : 0;
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < n; ++j) {
-                const int k0 = w.lo + (j0 + j) * kTile;
+                const int k0 = w.lo + (j0 + j) * kTile + side * kKeys;
                 const uint32_t b = (g + j) & 1, ts = t_s + b * kTile + lanes;
                 bar_wait(s_full(b), ((g + j) >> 1) & 1, c.err, 85);
                 tc_fence_after();
-                uint32_t s[kTile];
+                uint32_t s[kKeys];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, s + 32 * i);
-                tmem_wait_ld(s, kTile);
-                if (k0 < all_lo || k0 + kTile > all_hi) {
+                for (int i = 0; i < kKeys; i += 32) tmem_ld32(ts + side * kKeys + i, s + i);
+                tmem_wait_ld(s, kKeys);
+                if (k0 < all_lo || k0 + kKeys > all_hi) {
 #pragma unroll
-                    for (int x = 0; x < kTile; x += 32) {
+                    for (int x = 0; x < kKeys; x += 32) {
                         // bit i: key k0 + x + i is seen
                         const int lo = min(max(vis_lo - k0 - x, 0), 32), hi = min(max(vis_hi - k0 - x, 0), 32);
                         const uint32_t seen = (hi == 32 ? 0xFFFFFFFFu : (1u << hi) - 1u) & ~(lo == 32 ? 0xFFFFFFFFu : (1u << lo) - 1u);
@@ -631,10 +687,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < kTile; i += 4)
+                for (int i = 0; i < kKeys; i += 4)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], __uint_as_float(s[i + e]));
-                const float tile_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
+                float tile_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
+                // after this the other thread has read its scores too, over which this one's weights will lie
+                tile_max = fmaxf(tile_max, swap(tile_max));
                 if (__any_sync(0xFFFFFFFFu, tile_max > m + kRaise)) {
                     const float m_new = fmaxf(m, tile_max);
                     const float f = fast_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));
@@ -642,13 +700,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                         bar_wait(o_done(b ^ 1), ((g + j - 1) >> 1) & 1, c.err, 86);
                         tc_fence_after();
 #pragma unroll 1
-                        for (int x = 0; x < C::kDv; x += 32) {
+                        for (int x = 0; x < kCols; x += 32) {
+                            const uint32_t to = t_o + lanes + side * kCols + x;
                             uint32_t o[32];
-                            tmem_ld32(t_o + lanes + x, o);
+                            tmem_ld32(to, o);
                             tmem_wait_ld(o, 32);
 #pragma unroll
                             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tmem_st32(t_o + lanes + x, o);
+                            tmem_st32(to, o);
                         }
                     }
                     l *= f;
@@ -656,57 +715,69 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 const float ref = m == -INFINITY ? 0.0f : m;           // a row that has seen nothing yet
                 float sum[2] = {0.0f, 0.0f};
+                uint32_t pk[32];
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    uint32_t pk[32];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float e0 = fast_exp2(fmaf(__uint_as_float(s[64 * x + 2 * i]), scale2, -ref));
-                        const float e1 = fast_exp2(fmaf(__uint_as_float(s[64 * x + 2 * i + 1]), scale2, -ref));
-                        sum[0] += e0;
-                        sum[1] += e1;
-                        pk[i] = pack_bf16(e0, e1);
-                    }
-                    tmem_st32(ts + 32 * x, pk);
+                for (int i = 0; i < 32; ++i) {
+                    const float e0 = fast_exp2(fmaf(__uint_as_float(s[2 * i]), scale2, -ref));
+                    const float e1 = fast_exp2(fmaf(__uint_as_float(s[2 * i + 1]), scale2, -ref));
+                    sum[0] += e0;
+                    sum[1] += e1;
+                    pk[i] = pack_bf16(e0, e1);
                 }
+                tmem_st32(ts + 32 * side, pk);
                 l += sum[0] + sum[1];
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive_cluster(in_first_cta(p_full(b)));
             }
-            next = find(r + 1);                                    // while the last products run
+            next = find_next(r + 1, next);                         // while the last products run
+            l += swap(l);
             // ---------------- epilogue (before the next work's first weights, so its products do not start yet)
             bar_wait(o_done((g + n - 1) & 1), ((g + n - 1) >> 1) & 1, c.err, 87);
             tc_fence_after();
             const bool last = at.pieces == 1;
-            const float inv = !last ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-            const int64_t row = ((int64_t)at.slot * kCtas + rank) * kTile + row_in;
-            uint16_t* dst = c.a.out + (int64_t)(w.g.q0 + t0 + tok) * c.a.o_t + (int64_t)(h * c.group + row_in % c.group) * c.a.o_h +
-                            half * C::kDv;
-            float* part = c.part_o + row * C::kDv;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            if (last) {
+                // A thread's own row, 16 bytes at a time, would touch 32 lines a store: four lanes exchange the chunks
+                // of their rows, and each store has 64 bytes of eight rows.
+                uint16_t* dst = c.a.out + (int64_t)(w.g.q0 + t0 + tok) * c.a.o_t +
+                                (int64_t)(h * c.group + row_in % c.group) * c.a.o_h + half * C::kDv;
+                uint16_t* dst4[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    dst4[i] = reinterpret_cast<uint16_t*>(
+                                  __shfl_sync(0xFFFFFFFFu, mine ? reinterpret_cast<uintptr_t>(dst) : 0, (lane & ~3) + i));
 #pragma unroll 1
-            for (int x = 0; x < C::kDv; x += 32) {
-                uint32_t o[32];
-                tmem_ld32(t_o + lanes + x, o);
-                tmem_wait_ld(o, 32);
-                if (!mine) continue;
-                if (last) {
+                for (int x = side * kCols; x < (side + 1) * kCols; x += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(t_o + lanes + x, o);
+                    tmem_wait_ld(o, 32);
+                    uint32_t ch[4][4];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        uint32_t pk[4];
+                    for (int i = 0; i < 16; ++i)
+                        ch[i >> 2][i & 3] = pack_bf16(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+                    quad_transpose(ch, lane);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            pk[e] = pack_bf16(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
-                        *reinterpret_cast<uint4*>(dst + x + i) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-                    }
-                } else {
+                    for (int i = 0; i < 4; ++i)
+                        if (dst4[i] != nullptr)
+                            *reinterpret_cast<uint4*>(dst4[i] + x + (lane & 3) * 8) = make_uint4(ch[i][0], ch[i][1], ch[i][2], ch[i][3]);
+                }
+            } else {
+                // partials lie as [4 columns][row], so that a store of 32 rows is contiguous
+                const int64_t cta = (int64_t)at.slot * kCtas + rank;
+                float* part = c.part_o + cta * kTile * C::kDv + row_in * 4;
+#pragma unroll 1
+                for (int x = side * kCols; x < (side + 1) * kCols; x += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(t_o + lanes + x, o);
+                    tmem_wait_ld(o, 32);
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<uint4*>(part + x + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        *reinterpret_cast<uint4*>(part + (x + i) * kTile) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                 }
+                if (side == 0) *reinterpret_cast<float2*>(c.part_ml + (cta * kTile + row_in) * 2) = make_float2(m, l);
             }
-            if (!last) *reinterpret_cast<float2*>(c.part_ml + row * 2) = make_float2(m, l);
             tc_fence_before();      // the next first weights say that the output has been read
             g += n;
             ++done;
@@ -715,7 +786,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The pair's MMAs read both CTAs' shared memory and signal both: neither leaves before the other is done.
     tc_fence_before();
     __syncthreads();
-    if constexpr (kCtas == 2) cluster_sync();
+    if constexpr (kCtas == 2) {
+        cluster_arrive();
+        cluster_wait();
+    }
     if (warp == 1) {
         tc_fence_after();
         if constexpr (kCtas == 2)
@@ -725,53 +799,76 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// Joins the pieces of the last wave's tiles (blockIdx.y), the partials added in piece order: a warp has every eighth
-// of 32 rows.
-constexpr int kJoinRows = 32;
+// Joins the pieces of the last wave's tiles (blockIdx.y), the partials added in piece order. A warp has 32 rows, one a
+// lane, and 16 columns.
+constexpr int kJoinCols = 16, kJoinWarps = 8;
 
 template <int D>
-__global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_constant__ ChunkCall c) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_chunk_join_kernel(const __grid_constant__ ChunkCall c) {
     using C = ChunkCfg<D>;
-    constexpr int kRows = C::kCtas * kTile, kV = C::kDv / 32;         // output columns of a lane
+    constexpr int kGroups = C::kCtas * kTile / 32;                   // of rows
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     wait_for_predecessor();
     release_successor();
     const Work at = find_work<D, true>(c, blockIdx.y, lane);
     if (at.b < 0 || at.pieces == 1) return;
     const TileWork w = tile_work(c, at.g, at.tile);
-    for (int i = 0; i < kJoinRows; i += 8) {
-        const int row = blockIdx.x * kJoinRows + i + warp, r = row % kTile;
-        const int tok = row / kTile * c.tokens + r / c.group;
-        if (r >= c.tokens * c.group || w.t0 + tok >= w.g.q_len) continue;
-        const int64_t row0 = (int64_t)at.slot * kRows + row;
-        float2 ml = make_float2(-INFINITY, 0.0f);
-        if (lane < at.pieces) ml = *reinterpret_cast<const float2*>(c.part_ml + (row0 + lane * kRows) * 2);
-        float top = ml.x;
+    const int unit = blockIdx.x * kJoinWarps + warp, row = unit % kGroups * 32 + lane, col = unit / kGroups * kJoinCols;
+    const int r = row % kTile, tok = row / kTile * c.tokens + r / c.group;
+    if (r >= c.tokens * c.group || w.t0 + tok >= w.g.q_len) return;
+    const int64_t cta = (int64_t)at.slot * C::kCtas + row / kTile;   // of the first piece
+    const float* part = c.part_o + cta * kTile * C::kDv + (col * kTile + r * 4);
+    const float* ml = c.part_ml + (cta * kTile + r) * 2;
+    constexpr int kBatch = 4;
+    float acc[kJoinCols];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        const float f = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
-        float total = f * ml.y;
+    for (int e = 0; e < kJoinCols; ++e) acc[e] = 0.0f;
+    float top = -INFINITY, sum = 0.0f;
+    for (int z0 = 0; z0 < at.pieces; z0 += kBatch) {
+        float2 s[kBatch];
+        float4 v[kBatch][kJoinCols / 4];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
-        const float mine = total == 0.0f ? 0.0f : f / total;
-        float acc[kV];
+        for (int z = 0; z < kBatch; ++z) {
+            s[z] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-        for (int e = 0; e < kV; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-        for (int z = 0; z < at.pieces; ++z) {
-            const float g = __shfl_sync(0xFFFFFFFFu, mine, z);
-            const float* src = c.part_o + (row0 + (int64_t)z * kRows) * C::kDv + lane * kV;
+            for (int e = 0; e < kJoinCols / 4; ++e) v[z][e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (z0 + z < at.pieces) {
+                s[z] = *reinterpret_cast<const float2*>(ml + (int64_t)(z0 + z) * C::kCtas * kTile * 2);
 #pragma unroll
-            for (int e = 0; e < kV; e += 2) {
-                const float2 v = *reinterpret_cast<const float2*>(src + e);
-                acc[e] += g * v.x;
-                acc[e + 1] += g * v.y;
+                for (int e = 0; e < kJoinCols / 4; ++e)
+                    v[z][e] = *reinterpret_cast<const float4*>(part + (int64_t)(z0 + z) * C::kCtas * kTile * C::kDv + e * 4 * kTile);
             }
         }
-        uint16_t* dst = c.a.out + (int64_t)(w.g.q0 + w.t0 + tok) * c.a.o_t + (int64_t)(at.h * c.group + r % c.group) * c.a.o_h +
-                        at.half * C::kDv + lane * kV;
+        float now = top;
 #pragma unroll
-        for (int e = 0; e < kV; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16(acc[e], acc[e + 1]);
+        for (int z = 0; z < kBatch; ++z) now = fmaxf(now, s[z].x);
+        const float ref = now == -INFINITY ? 0.0f : now, back = fast_exp2(top - ref);
+        top = now;
+        sum *= back;
+#pragma unroll
+        for (int e = 0; e < kJoinCols; ++e) acc[e] *= back;
+#pragma unroll
+        for (int z = 0; z < kBatch; ++z) {
+            const float f = fast_exp2(s[z].x - ref);
+            sum += f * s[z].y;
+#pragma unroll
+            for (int e = 0; e < kJoinCols / 4; ++e) {
+                acc[4 * e] += f * v[z][e].x;
+                acc[4 * e + 1] += f * v[z][e].y;
+                acc[4 * e + 2] += f * v[z][e].z;
+                acc[4 * e + 3] += f * v[z][e].w;
+            }
+        }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint16_t* dst = c.a.out + (int64_t)(w.g.q0 + w.t0 + tok) * c.a.o_t + (int64_t)(at.h * c.group + r % c.group) * c.a.o_h +
+                    at.half * C::kDv + col;
+#pragma unroll
+    for (int e = 0; e < kJoinCols; e += 8) {
+        uint32_t pk[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pk[i] = pack_bf16(acc[e + 2 * i] * inv, acc[e + 2 * i + 1] * inv);
+        *reinterpret_cast<uint4*>(dst + e) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
     }
 }
 
@@ -810,8 +907,11 @@ void launch_chunk_dim(const Attn& hd, const AttnCall& a, int few_rows, cudaStrea
     const CUtensorMap tk = paged_map(a, a.k, D, c.box), tv = paged_map(a, a.v, D, c.box);
     launch_dependent<C::kCtas>(attn_chunk_kernel<D>, dim3((unsigned)(c.clusters * C::kCtas)), dim3(kThreads), C::kSmem, st, tq,
                                tk, tv, c);
-    if (pieces > 1)   // else no tile is long enough for two pieces
-        launch_dependent(attn_chunk_join_kernel<D>, dim3(C::kCtas * kTile / kJoinRows, (unsigned)c.wave), dim3(256), 0, st, c);
+    const int cut = (int)std::min<int64_t>(c.wave / 2, tiles * a.hk * C::kHalves);   // a wave holds two pieces of each
+    if (pieces > 1 && cut > 0)   // else no tile is long enough for two pieces
+        launch_dependent(attn_chunk_join_kernel<D>,
+                         dim3(C::kCtas * kTile / 32 * (C::kDv / kJoinCols) / kJoinWarps, (unsigned)cut), dim3(kJoinWarps * 32), 0,
+                         st, c);
 }
 
 }  // namespace
