@@ -49,6 +49,7 @@ constexpr int kTile = 128;             // query rows and keys of a tile
 constexpr int kThreads = 352;
 constexpr int kSoftWarps = 8;          // of the softmax: warps 2..9
 constexpr int kVWarp = 10;
+constexpr int kItems = 4;              // of work, between the warp that finds them and the others
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 8.0f;         // how far (log2) a score may exceed the maximum in use
 constexpr uint32_t kTmemCols = 512;
@@ -66,7 +67,8 @@ struct ChunkCfg {
     static constexpr int kVCols = kDv / kCtas;               // V stage: 128 keys x kVCols elements
     static constexpr int kStageBytes = kTile * kVCols * 2;
     static constexpr int kQBytes = kTile * D * 2;
-    static constexpr int kTail = 256 + 2 * 2 * kTile * 4;    // barriers, and the row maxima of two halves and two tiles
+    // barriers, items of work, and the row maxima of two halves and two tiles
+    static constexpr int kTail = 256 + kItems * 64 + 2 * 2 * kTile * 4;
     static constexpr int kFit = (227 * 1024 - kTail - kQBytes) / kStageBytes;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     static constexpr int kVStages = kStages / 2 < 1 ? 1 : (kStages - (kKSt - 1)) / 2;   // of the ring of V tiles
@@ -83,7 +85,7 @@ struct ChunkCall {
     int few_rows;        // sequences of at most so many rows belong to the other kernel
     int tokens;          // tokens of a CTA's 128 rows: 128 / group
     int tile_tokens;     // tokens of a tile: of all the CTAs that share it
-    int box;
+    int box, box_shift;
     int wave;            // tiles that the GPU computes at once
     int clusters;        // CTAs or CTA pairs of the launch
     float* part_o;       // [pieces, at most a wave][CTAs of a tile][output columns of a CTA / 4][128 rows][4]
@@ -122,6 +124,15 @@ __device__ __forceinline__ TileWork tile_work(const ChunkCall& c, const SeqGeom&
     w.n = max(1, (w.any_hi - w.lo + kTile - 1) / kTile);    // rows that see nothing still become zeros
     return w;
 }
+
+// A piece of work as the warps of a CTA share it.
+struct alignas(16) Item {
+    int q0, q_len, first, kv_len;      // its sequence
+    int b, h, half, t0;                // t0: first token of this CTA's rows
+    int lo, n, any_lo, any_hi;         // first key of the first key tile, their number (0: no more work)
+    int pieces, slot, unused[2];
+};
+static_assert(sizeof(Item) == 64, "items lie in kTail");
 
 // The index-th piece of work of the launch, or the index-th tile of the last wave (kLast); b < 0: none. One warp.
 // Tiles of the whole waves come first, each one piece; then the rest's first pieces, second pieces and so on.
@@ -397,7 +408,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto o_done = [&](int b) { return q_full + 8u + 8u * b; };    // products of the even and the odd tiles
     const uint32_t edge_full = q_full + 24, q_free = q_full + 32;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (s_bar - base) + 8u * (2 * C::kStages + 9));
-    float* s_max = reinterpret_cast<float*>(gen + (s_bar - base) + 256);     // [parity of the tile][half][row]
+    auto work_full = [&](uint32_t i) { return s_bar + 8u * (2 * C::kStages + 10 + i % kItems); };
+    Item* s_item = reinterpret_cast<Item*>(gen + (s_bar - base) + 256);
+    float* s_max = reinterpret_cast<float*>(s_item + kItems);                // [parity of the exchange][half][row]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = blockIdx.x % kCtas;                 // place in the pair
@@ -425,6 +438,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         bar_init(q_full, kCtas);
         bar_init(q_free, 1);
         bar_init(edge_full, 1);
+        for (int i = 0; i < kItems; ++i) {
+            bar_init(work_full(i), 1);
+            s_item[i].n = 0;
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         for (const CUtensorMap* map : {&tm_q, &tm_k, &tm_v})
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
@@ -435,38 +452,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     wait_for_predecessor();
     release_successor();
 
-    // The work of this cluster: every warp walks the same list, the way back and forth over the clusters, so that who
-    // had a long tile in one round has a short one in the next.
-    Work at;
-    TileWork w;
-    int t0 = 0, j0 = 0, n = 0, h = 0, half = 0;
-    auto find = [&](int r) {
-        return find_work<D, false>(c, r * c.clusters + ((r & 1) ? c.clusters - 1 - cluster : cluster), lane);
-    };
-    auto find_next = [&](int r, Work now) {         // after `now`, of round r - 1
-        if (r * c.clusters < now.count) return find(r);
-        now.b = -1;
-        return now;
-    };
-    auto begin = [&](const Work& next) {
-        at = next;
-        if (at.b < 0) return false;
-        w = tile_work(c, at.g, at.tile);
-        t0 = w.t0 + rank * c.tokens;             // this CTA's first token
-        // this piece's key tiles
-        j0 = w.n * at.piece / at.pieces;
-        n = w.n * (at.piece + 1) / at.pieces - j0;
-        h = at.h;
-        half = at.half;
-        return true;
-    };
-    Work next = find(0);
     if constexpr (kCtas == 2) cluster_wait();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const uint32_t t_o = tmem, t_s = tmem + 256;     // output, two score buffers of 128 columns
-    uint32_t done = 0;     // tiles of work done, and the key tiles of them: the phases of the barriers go on
+    uint32_t done = 0;     // items done, and their key tiles: the phases of the barriers go on
     uint32_t g = 0;
+    Item w;                // the one at hand
+    // Warp 0 finds the work: a search takes 2000 to 4000 cycles, which every warp would wait for. It is at most three
+    // items ahead of the others, as Q of an item is only loaded when the scores of the one before are done.
+    auto take = [&] {
+        bar_wait(work_full(done), done / kItems & 1, c.err, 90);
+        w = s_item[done % kItems];
+        return w.n > 0;
+    };
     if (warp == 0 || warp == kVWarp) {
         // ---------------- producers: Q and K tiles (warp 0), V tiles (kVWarp)
         const int first_stage = warp == 0 ? 0 : C::kKStages, last_stage = warp == 0 ? C::kKStages : C::kStages;
@@ -479,10 +478,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         // The page of this lane's box of tile j, looked up two tiles ahead of its use (the look-up takes as long
         // as half a tile's products).
         auto look_up = [&](int j) {
-            const int key = w.lo + (j0 + j) * kTile + lane * c.box;
+            const int key = w.lo + j * kTile + lane * c.box;
             int page = pv.n_pages;                    // outside the map: reads zeros
-            if (j < n && lane < boxes && key < w.any_hi) {
-                page = pv.table[at.b * pv.table_ld + (key >> pv.page_shift)];
+            if (j < w.n && lane < boxes && key < w.any_hi) {
+                page = pv.table[w.b * pv.table_ld + (key >> pv.page_shift)];
                 if (page < 0 || page >= pv.n_pages) {
                     record_input_error(pv.err, kErrPage);
                     page = pv.n_pages;
@@ -503,26 +502,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (round > 0) bar_wait(empty(stage), (round - 1) & 1, c.err, 80);
             if (lane == 0) bar_expect_tx_cluster(bar, (uint32_t)count * box_bytes);
             __syncwarp();
-            if (lane < count) tma_page<kCtas>(dst, map, col0 + cb * 64, slot, h, page, bar);
+            if (lane < count) tma_page<kCtas>(dst, map, col0 + cb * 64, slot, w.h, page, bar);
         };
         auto load_k = [&](int j, int pages) {
-            const int k0 = w.lo + (j0 + j) * kTile + rank * C::kKeysHeld;
+            const int k0 = w.lo + j * kTile + rank * C::kKeysHeld;
             // a box without a key that some row sees is left out: its scores are masked
-            const int nb = max(0, min(C::kKeysHeld / c.box, (w.any_hi - k0 + c.box - 1) / c.box));
+            const int nb = max(0, min(C::kKeysHeld / c.box, (w.any_hi - k0 + c.box - 1) >> c.box_shift));
             for (int p = 0; p < C::kKSt; ++p) {
                 fill(&tm_k, false, pages, k0, C::kKeysHeld, rank * C::kKeysHeld / c.box, 0, nb, p * C::kKCols, C::kKCols / 64);
                 if (++stage == last_stage) stage = first_stage, ++round;
             }
         };
         auto load_v = [&](int j, int pages) {
-            const int k0 = w.lo + (j0 + j) * kTile, col0 = half * C::kDv + rank * C::kVCols;
-            const int b1 = max(0, min(boxes, (w.any_hi - k0 + c.box - 1) / c.box));
+            const int k0 = w.lo + j * kTile, col0 = w.half * C::kDv + rank * C::kVCols;
+            const int b1 = max(0, min(boxes, (w.any_hi - k0 + c.box - 1) >> c.box_shift));
             if (k0 >= w.any_lo && k0 + kTile <= w.any_hi) {
                 fill(&tm_v, false, pages, k0, kTile, 0, 0, boxes, col0, C::kVCols / 64);
             } else {
                 // Keys that no row of the tile sees hold anything, and a zero weight times NaN is NaN: the stage
                 // is filled on a barrier of this CTA's own, their rows are zeroed, and it is handed over then.
-                const int b0 = max(0, w.any_lo - k0) / c.box;
+                const int b0 = max(0, w.any_lo - k0) >> c.box_shift;
                 fill(&tm_v, true, pages, k0, kTile, 0, min(b0, b1), b1, col0, C::kVCols / 64);
                 bar_wait(edge_full, edge_round++ & 1, c.err, 88);
                 const int lo = min(kTile, max(0, w.any_lo - k0)), hi = min(kTile, max(lo, w.any_hi - k0));
@@ -539,31 +538,70 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (++stage == last_stage) stage = first_stage, ++round;
         };
-        for (int r = 0; r * c.clusters < next.count; ++r) {
-            const bool some = begin(next);
-            next = find_next(r + 1, next);
-            if (!some) continue;
-            if (warp == 0) {
+        auto load_v_tiles = [&] {
+            int pages = look_up(0), pages1 = look_up(1);
+            for (int j = 0; j < w.n; ++j) {
+                const int pages2 = look_up(j + 2);
+                load_v(j, pages);
+                pages = pages1;
+                pages1 = pages2;
+            }
+        };
+        if (warp == kVWarp) {
+            for (; take(); ++done) load_v_tiles();
+        } else {
+            // The work of this cluster: the way back and forth over the clusters, so that who had a long tile in one
+            // round has a short one in the next.
+            int r = 0, count = 1;                        // of the list: known after the first search
+            auto find = [&] {
+                Item it = {};
+                for (; it.n == 0 && r * c.clusters < count; ++r) {
+                    const Work at =
+                        find_work<D, false>(c, r * c.clusters + ((r & 1) ? c.clusters - 1 - cluster : cluster), lane);
+                    count = at.count;
+                    if (at.b < 0) continue;
+                    const TileWork t = tile_work(c, at.g, at.tile);
+                    const int j0 = t.n * at.piece / at.pieces;           // this piece's key tiles
+                    it = {at.g.q0, at.g.q_len, at.g.first, at.g.kv_len, at.b, at.h, at.half, t.t0 + rank * c.tokens,
+                          t.lo + j0 * kTile, t.n * (at.piece + 1) / at.pieces - j0, t.any_lo, t.any_hi, at.pieces, at.slot};
+                }
+                return it;
+            };
+            uint32_t made = 0;
+            auto hand_out = [&](const Item& it) {
+                if (lane == 0) {
+                    s_item[made % kItems] = it;
+                    bar_arrive(work_full(made));
+                }
+                __syncwarp();
+                ++made;
+            };
+            w = find();
+            hand_out(w);
+            while (w.n > 0) {
+                int pages = look_up(0), pages1 = look_up(1);
                 if (done > 0) bar_wait(q_free, (done - 1) & 1, c.err, 89);
                 if (lane == 0) {
                     const uint32_t qb = in_first_cta(q_full);
                     bar_expect_tx_cluster(qb, (uint32_t)(c.tokens * c.group) * 128u * (D / 64));
                     for (int x = 0; x < D / 64; ++x)
-                        tma_rows<kCtas>(s_q + x * (kTile * 128), &tm_q, x * 64, h * c.group, w.g.q0 + t0, qb);
+                        tma_rows<kCtas>(s_q + x * (kTile * 128), &tm_q, x * 64, w.h * c.group, w.q0 + w.t0, qb);
                 }
                 __syncwarp();
-            }
-            int pages = look_up(0), pages1 = look_up(1);
-            for (int j = 0; j < n; ++j) {
-                const int pages2 = look_up(j + 2);
-                if (warp == 0)
+                Item next;
+                for (int j = 0; j < w.n; ++j) {
+                    const int pages2 = look_up(j + 2);
                     load_k(j, pages);
-                else
-                    load_v(j, pages);
-                pages = pages1;
-                pages1 = pages2;
+                    pages = pages1;
+                    pages1 = pages2;
+                    if (j == 0) {
+                        next = find();
+                        hand_out(next);
+                    }
+                }
+                w = next;
+                ++done;
             }
-            ++done;
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer (of the pair's first CTA)
@@ -590,15 +628,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (elect()) {
                     mma_commit<kCtas>(s_full((g + j) & 1));
-                    if (j + 1 == n) mma_commit<kCtas>(q_free);     // Q has been read
+                    if (j + 1 == w.n) mma_commit<kCtas>(q_free);   // Q has been read
                 }
                 __syncwarp();
             };
-            for (int r = 0; r * c.clusters < next.count; ++r) {
-                if (!begin(next)) {
-                    next = find_next(r + 1, next);
-                    continue;
-                }
+            while (take()) {
+                const int n = w.n;
                 bar_wait(q_full, done & 1, c.err, 82);
                 scores(0);
                 for (int j = 0; j < n; ++j) {
@@ -621,7 +656,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 g += n;
                 ++done;
-                next = find_next(r + 1, next);                     // while the last products run
             }
         }
     } else {
@@ -644,29 +678,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const int tok = row_in / c.group;
         const float scale2 = c.a.scale * kLog2e;
-        for (int r = 0;; ++r) {
-            // Both warps take the same steps whatever they have read: lengths that change under a running kernel are an
-            // error, but the barrier between the two has no limit of its own, so they agree on the number first.
-            const int steps = r * c.clusters >= next.count ? -1 : begin(next) ? n : 0;
-            n = min(steps, __float_as_int(swap(__int_as_float(steps))));
-            if (n < 0) break;
-            if (n == 0) {
-                next = find_next(r + 1, next);
-                continue;
-            }
-            const bool mine = tok < c.tokens && t0 + tok < w.g.q_len;
+        for (;;) {
+            // Both warps take the same number of steps, whatever they have read (a wait that gave up leaves an old item):
+            // the barrier between the two has no limit of its own.
+            const int steps = take() ? w.n : 0;
+            const int n = min(steps, __float_as_int(swap(__int_as_float(steps))));
+            if (n == 0) break;
+            const bool mine = tok < c.tokens && w.t0 + tok < w.q_len;
             int vis_lo = 0, vis_hi = 0;
             if (mine) {
-                const int pos = w.g.first + t0 + tok;
-                vis_hi = min(max(pos + 1, 0), w.g.kv_len);
+                const int pos = w.first + w.t0 + tok;
+                vis_hi = min(max(pos + 1, 0), w.kv_len);
                 if (c.a.window > 0) vis_lo = max(0, pos - c.a.window + 1);
             }
             // keys that every row of this CTA sees (rows beyond the sequence do not matter)
-            const int all_hi = min(max(w.g.first + t0 + 1, 0), w.g.kv_len);
-            const int all_lo = c.a.window > 0 ? max(0, w.g.first + min(t0 + c.tokens, w.g.q_len) - c.a.window) : 0;
+            const int all_hi = min(max(w.first + w.t0 + 1, 0), w.kv_len);
+            const int all_lo = c.a.window > 0 ? max(0, w.first + min(w.t0 + c.tokens, w.q_len) - c.a.window) : 0;
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < n; ++j) {
-                const int k0 = w.lo + (j0 + j) * kTile + side * kKeys;
+                const int k0 = w.lo + j * kTile + side * kKeys;
                 const uint32_t b = (g + j) & 1, ts = t_s + b * kTile + lanes;
                 bar_wait(s_full(b), ((g + j) >> 1) & 1, c.err, 85);
                 tc_fence_after();
@@ -731,18 +761,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) bar_arrive_cluster(in_first_cta(p_full(b)));
             }
-            next = find_next(r + 1, next);                         // while the last products run
             l += swap(l);
             // ---------------- epilogue (before the next work's first weights, so its products do not start yet)
             bar_wait(o_done((g + n - 1) & 1), ((g + n - 1) >> 1) & 1, c.err, 87);
             tc_fence_after();
-            const bool last = at.pieces == 1;
+            const bool last = w.pieces == 1;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             if (last) {
                 // A thread's own row, 16 bytes at a time, would touch 32 lines a store: four lanes exchange the chunks
                 // of their rows, and each store has 64 bytes of eight rows.
-                uint16_t* dst = c.a.out + (int64_t)(w.g.q0 + t0 + tok) * c.a.o_t +
-                                (int64_t)(h * c.group + row_in % c.group) * c.a.o_h + half * C::kDv;
+                uint16_t* dst = c.a.out + (int64_t)(w.q0 + w.t0 + tok) * c.a.o_t +
+                                (int64_t)(w.h * c.group + row_in % c.group) * c.a.o_h + w.half * C::kDv;
                 uint16_t* dst4[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -765,7 +794,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             } else {
                 // partials lie as [4 columns][row], so that a store of 32 rows is contiguous
-                const int64_t cta = (int64_t)at.slot * kCtas + rank;
+                const int64_t cta = (int64_t)w.slot * kCtas + rank;
                 float* part = c.part_o + cta * kTile * C::kDv + row_in * 4;
 #pragma unroll 1
                 for (int x = side * kCols; x < (side + 1) * kCols; x += 32) {
@@ -889,6 +918,7 @@ void launch_chunk_dim(const Attn& hd, const AttnCall& a, int few_rows, cudaStrea
     c.tokens = kTile / c.group;
     c.tile_tokens = c.tokens * C::kCtas;
     c.box = std::min(1 << a.pv.page_shift, 64);
+    c.box_shift = std::min(a.pv.page_shift, 6);
     c.wave = device_sm_count() / C::kCtas;
     // a sequence has at most one tile that is not full
     const int64_t tiles = std::min<int64_t>((int64_t)a.pv.rows / c.tile_tokens + a.pv.n_seqs,
