@@ -1,5 +1,6 @@
 // g4q_attn.cu -- attention of a few new tokens per sequence over a paged cache (sm_100a): one decoded token
-// each, or a block of drafted ones, up to 64 query rows (tokens x query heads of a key head) per key head.
+// each, or a block of drafted ones, up to 64 query rows (tokens x query heads of a key head) per key head (32 at
+// head_dim 512).
 //
 //   out = softmax(scale * q k^T + mask) v, masked to the positions j <= t (and j > t - window)
 //
@@ -31,7 +32,9 @@
 namespace g4q {
 namespace {
 
-constexpr int kFewRows = 64;         // rows per key head that this kernel takes
+// Rows per key head that this kernel takes. At head_dim 512 the registers end at 32: blocks of 4 tokens x 16 heads of two
+// sequences of 16000 keys take 56 us here with spills, 41 in the chunk kernel (of 2049 and 4000 keys 25.7 and 26.6).
+constexpr int few_rows(int head_dim) { return head_dim == 512 ? 32 : 64; }
 constexpr int kKeys = 64;            // keys per tile
 constexpr int kComputeWarps = 8;
 constexpr int kThreads = (kComputeWarps + 1) * 32;
@@ -669,13 +672,15 @@ void launch_few_rows(const Attn& h, const AttnCall& a, int64_t rows, cudaStream_
         launch_few<D, 1>(h, a, st);
     else if (rows <= 32)
         launch_few<D, 2>(h, a, st);
-    else
+    else if constexpr (few_rows(D) == 64)
         launch_few<D, 4>(h, a, st);
 }
 
 template <int D>
 size_t few_part_rows() {
-    return 2 * std::max({(size_t)few_ctas<D, 1>() * 16, (size_t)few_ctas<D, 2>() * 32, (size_t)few_ctas<D, 4>() * 64});
+    size_t rows = std::max((size_t)few_ctas<D, 1>() * 16, (size_t)few_ctas<D, 2>() * 32);
+    if constexpr (few_rows(D) == 64) rows = std::max(rows, (size_t)few_ctas<D, 4>() * 64);
+    return 2 * rows;
 }
 
 }  // namespace
@@ -740,9 +745,9 @@ void launch_attention(const Attn& h, const AttnCall& a, cudaStream_t st) {
     // (two tokens beside four prompts, head_dim 256: 20.8 us against 8).
     const int group = a.hq / a.hk;
     const int64_t rows = (int64_t)a.pv.max_q * group;
-    if (rows <= kFewRows) return launch_few_any(h, a, rows, st);
-    if ((int64_t)a.pv.n_seqs * a.pv.max_q == a.pv.rows) return launch_chunk(h, a, 0, st);
+    if (rows <= few_rows(h.head_dim)) return launch_few_any(h, a, rows, st);
     const int few = group <= 16 ? 16 : group <= 32 ? 32 : 64;
+    if ((int64_t)a.pv.n_seqs * a.pv.max_q == a.pv.rows || few > few_rows(h.head_dim)) return launch_chunk(h, a, 0, st);
     launch_few_any(h, a, few, st);
     launch_chunk(h, a, few, st);
 }

@@ -54,7 +54,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 8.0f;         // how far (log2) a score may exceed the maximum in use
 constexpr uint32_t kTmemCols = 512;
 constexpr int kMaxSplits = 32;         // pieces of a tile's keys
-constexpr int kMinPiece = 6;           // key tiles of a piece, at least
+// Key tiles of a piece, at least. Where all the work is one wave, pieces always shorten it (300 tokens over 2000 keys:
+// 29.4 us with 6, 28.5 with 3; 12 tokens of two sequences at head_dim 512: 32.7 and 28.0). After a wave of whole tiles
+// more pieces also land behind the long ones (4 prompts beside 2 tokens: 59.7 us with 6, 69.9 with 3).
+constexpr int kMinPiece = 6, kMinPieceAlone = 3;
 
 template <int D>
 struct ChunkCfg {
@@ -88,6 +91,7 @@ struct ChunkCall {
     int box, box_shift;
     int wave;            // tiles that the GPU computes at once
     int clusters;        // CTAs or CTA pairs of the launch
+    int max_pieces;      // of a tile's keys
     float* part_o;       // [pieces, at most a wave][CTAs of a tile][output columns of a CTA / 4][128 rows][4]
     float* part_ml;      // [pieces][CTAs of a tile * 128][2]
     int* err;
@@ -156,7 +160,7 @@ __device__ __noinline__ Work find_work(const ChunkCall& c, int index, int lane) 
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
     const int per_tile = c.a.hk * kHalves, items = total * per_tile;
     const int whole = items / c.wave * c.wave, rest = items - whole;
-    const int cuts = rest > 0 ? min(kMaxSplits, c.wave / rest) : 1;
+    const int cuts = rest > 0 ? min(c.max_pieces, c.wave / rest) : 1;
     w.count = whole + rest * cuts;
     int item = index, piece = 0;
     if (kLast) {
@@ -207,7 +211,8 @@ __device__ __noinline__ Work find_work(const ChunkCall& c, int index, int lane) 
     w.g.kv_len = __shfl_sync(0xFFFFFFFFu, g.kv_len, at);
     w.h = item % per_tile / kHalves;
     w.half = item % kHalves;
-    w.pieces = item < whole ? 1 : max(1, min(cuts, tile_work(c, w.g, w.tile).n / kMinPiece));
+    const int least = whole > 0 ? kMinPiece : kMinPieceAlone;
+    w.pieces = item < whole ? 1 : max(1, min(cuts, tile_work(c, w.g, w.tile).n / least));
     w.piece = piece;
     w.slot = (item - whole) * cuts + piece;
     if (piece >= w.pieces) w.b = -1;
@@ -589,12 +594,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 __syncwarp();
                 Item next;
+                const int ahead = min(w.n, C::kKStages / C::kKSt) - 1;
                 for (int j = 0; j < w.n; ++j) {
                     const int pages2 = look_up(j + 2);
                     load_k(j, pages);
                     pages = pages1;
                     pages1 = pages2;
-                    if (j == 0) {
+                    if (j == ahead) {                    // while these tiles arrive
                         next = find();
                         hand_out(next);
                     }
@@ -925,11 +931,16 @@ void launch_chunk_dim(const Attn& hd, const AttnCall& a, int few_rows, cudaStrea
                                             (int64_t)a.pv.n_seqs * ((a.pv.max_q + c.tile_tokens - 1) / c.tile_tokens));
     if ((tiles * a.hk * C::kHalves + c.wave) * kMaxSplits > 0x7FFFFFFF)
         throw Error(G4Q_ERR_INVALID_ARGUMENT, "too many rows for one call");
-    // as many as run at once, unless there can be less work: a tile has at most kMaxSplits pieces, of kMinPiece key tiles
+    // as many as run at once, unless there can be less work
     int64_t cap = (int64_t)a.pv.max_pages << a.pv.page_shift;
     if (a.window > 0) cap = std::min<int64_t>(cap, (int64_t)a.window + c.tile_tokens + c.box);
-    const int64_t pieces = std::max<int64_t>(1, (cap + kTile - 1) / kTile / kMinPiece);
-    c.clusters = (int)std::min<int64_t>(c.wave, tiles * a.hk * C::kHalves * std::min<int64_t>(pieces, kMaxSplits));
+    const int64_t key_tiles = (cap + kTile - 1) / kTile, items = tiles * a.hk * C::kHalves, rest = items % c.wave;
+    c.max_pieces = (int)std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, key_tiles / kMinPieceAlone));
+    // Sequences of one length: the tiles are known here, and where none will be cut there is nothing to join (an empty
+    // join costs 6 us).
+    const bool known = (int64_t)a.pv.n_seqs * a.pv.max_q == a.pv.rows;
+    if (known && (rest * 2 > c.wave || rest == 0 || (items > c.wave && key_tiles / kMinPiece < 2))) c.max_pieces = 1;
+    c.clusters = (int)std::min<int64_t>(c.wave, items * c.max_pieces);
     c.part_o = hd.part_o;
     c.part_ml = hd.part_ml;
     c.err = device_scratch().err;
@@ -937,8 +948,8 @@ void launch_chunk_dim(const Attn& hd, const AttnCall& a, int few_rows, cudaStrea
     const CUtensorMap tk = paged_map(a, a.k, D, c.box), tv = paged_map(a, a.v, D, c.box);
     launch_dependent<C::kCtas>(attn_chunk_kernel<D>, dim3((unsigned)(c.clusters * C::kCtas)), dim3(kThreads), C::kSmem, st, tq,
                                tk, tv, c);
-    const int cut = (int)std::min<int64_t>(c.wave / 2, tiles * a.hk * C::kHalves);   // a wave holds two pieces of each
-    if (pieces > 1 && cut > 0)   // else no tile is long enough for two pieces
+    const int cut = (int)std::min<int64_t>(c.wave / 2, items);   // a wave holds two pieces of each
+    if (c.max_pieces > 1 && cut > 0)   // else no tile is long enough for two pieces
         launch_dependent(attn_chunk_join_kernel<D>,
                          dim3(C::kCtas * kTile / 32 * (C::kDv / kJoinCols) / kJoinWarps, (unsigned)cut), dim3(kJoinWarps * 32), 0,
                          st, c);
