@@ -82,6 +82,20 @@ struct ChunkCfg {
     static_assert(kVStages >= 1 && kKStages >= kKSt, "a tile of each fits");
 };
 
+// n / d for 0 <= n < 2^31 as a product: with 2^(l-1) < d <= 2^l and mul = floor(2^(31+l) / d) + 1, mul d exceeds
+// 2^(31+l) by e in (0, 2^l], and n e < 2^(31+l) leaves the quotient as it is.
+struct Divisor {
+    uint32_t mul;
+    int shift;
+    explicit Divisor(uint32_t d = 1) {
+        int l = 0;
+        while ((1ull << l) < d) ++l;
+        mul = (uint32_t)((1ull << (31 + l)) / d + 1);
+        shift = 31 + l;
+    }
+    __device__ __forceinline__ int of(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
+};
+
 struct ChunkCall {
     AttnCall a;
     int group;
@@ -92,6 +106,7 @@ struct ChunkCall {
     int wave;            // tiles that the GPU computes at once
     int clusters;        // CTAs or CTA pairs of the launch
     int max_pieces;      // of a tile's keys
+    Divisor by_tile_tokens, by_wave, by_per_tile;    // per_tile: key heads x halves
     float* part_o;       // [pieces, at most a wave][CTAs of a tile][output columns of a CTA / 4][128 rows][4]
     float* part_ml;      // [pieces][CTAs of a tile * 128][2]
     int* err;
@@ -114,7 +129,7 @@ struct TileWork {
 };
 
 __device__ __forceinline__ int tiles_of(const ChunkCall& c, const SeqGeom& g) {
-    return g.q_len * c.group > c.few_rows ? (g.q_len + c.tile_tokens - 1) / c.tile_tokens : 0;
+    return g.q_len * c.group > c.few_rows ? c.by_tile_tokens.of(g.q_len + c.tile_tokens - 1) : 0;
 }
 
 __device__ __forceinline__ TileWork tile_work(const ChunkCall& c, const SeqGeom& g, int tile) {
@@ -156,22 +171,22 @@ __device__ __noinline__ Work find_work(const ChunkCall& c, int index, int lane) 
     SeqGeom g = geom_of(lane);                   // the first 32 sequences stay in registers
     int nt = tiles_of(c, g), total = nt;
     for (int b = lane + 32; b < n_seqs; b += 32) total += tiles_of(c, seq_geom(c.a.pv, b));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
-    const int per_tile = c.a.hk * kHalves, items = total * per_tile;
-    const int whole = items / c.wave * c.wave, rest = items - whole;
-    const int cuts = rest > 0 ? min(c.max_pieces, c.wave / rest) : 1;
+    total = __reduce_add_sync(0xFFFFFFFFu, total);
+    const int per_tile = c.a.hk * kHalves, items = max(0, total * per_tile);
+    const int whole = c.by_wave.of(items) * c.wave, rest = items - whole;
+    const int cuts = rest > 0 && c.max_pieces > 1 ? min(c.max_pieces, c.wave / rest) : 1;
     w.count = whole + rest * cuts;
     int item = index, piece = 0;
     if (kLast) {
         if (index >= rest) return w;
         item = whole + index;
     } else if (index >= whole && rest > 0) {
-        item = whole + (index - whole) % rest;
-        piece = (index - whole) / rest;
+        piece = cuts > 1 ? (index - whole) / rest : 0;
+        item = index - piece * rest;
     }
     if (item >= items || piece >= cuts) return w;
-    int t = item / per_tile, at = 0;
+    int t = c.by_per_tile.of(item), at = 0;
+    const int unit = item - t * per_tile;        // of the row tile's
     if (n_seqs <= 32) {
         int before = 0;                          // tiles of the sequences that come before this lane's
         for (int o = 0; o < n_seqs; ++o) {
@@ -209,10 +224,10 @@ __device__ __noinline__ Work find_work(const ChunkCall& c, int index, int lane) 
     w.g.q_len = __shfl_sync(0xFFFFFFFFu, g.q_len, at);
     w.g.first = __shfl_sync(0xFFFFFFFFu, g.first, at);
     w.g.kv_len = __shfl_sync(0xFFFFFFFFu, g.kv_len, at);
-    w.h = item % per_tile / kHalves;
-    w.half = item % kHalves;
+    w.h = unit / kHalves;
+    w.half = unit % kHalves;
     const int least = whole > 0 ? kMinPiece : kMinPieceAlone;
-    w.pieces = item < whole ? 1 : max(1, min(cuts, tile_work(c, w.g, w.tile).n / least));
+    w.pieces = cuts == 1 || item < whole ? 1 : max(1, min(cuts, tile_work(c, w.g, w.tile).n / least));
     w.piece = piece;
     w.slot = (item - whole) * cuts + piece;
     if (piece >= w.pieces) w.b = -1;
@@ -481,18 +496,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t box_bytes = (uint32_t)c.box * 128u;
         const int boxes = kTile / c.box;             // of a tile of keys; box i is lane i's
         // The page of this lane's box of tile j, looked up two tiles ahead of its use (the look-up takes as long
-        // as half a tile's products).
+        // as half a tile's products) and checked when it is used, so that nothing waits for it before.
+        constexpr int kNoBox = INT32_MIN;
         auto look_up = [&](int j) {
             const int key = w.lo + j * kTile + lane * c.box;
-            int page = pv.n_pages;                    // outside the map: reads zeros
-            if (j < w.n && lane < boxes && key < w.any_hi) {
-                page = pv.table[w.b * pv.table_ld + (key >> pv.page_shift)];
-                if (page < 0 || page >= pv.n_pages) {
-                    record_input_error(pv.err, kErrPage);
-                    page = pv.n_pages;
-                }
-            }
-            return page;
+            return j < w.n && lane < boxes && key < w.any_hi ? pv.table[w.b * pv.table_ld + (key >> pv.page_shift)] : kNoBox;
+        };
+        auto checked = [&](int page) {
+            if (page >= 0 && page < pv.n_pages) return page;
+            if (page != kNoBox) record_input_error(pv.err, kErrPage);
+            return pv.n_pages;                        // outside the map: reads zeros
         };
         // Fills the next stage with boxes [b0, b1) of its keys k0.. (`keys` of them, the first one box `first` of
         // its tile), columns [col0, col0 + 64 * blocks): at most one box a lane. All of it is worked out before the
@@ -509,7 +522,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane < count) tma_page<kCtas>(dst, map, col0 + cb * 64, slot, w.h, page, bar);
         };
-        auto load_k = [&](int j, int pages) {
+        auto load_k = [&](int j, int raw_pages) {
+            const int pages = checked(raw_pages);
             const int k0 = w.lo + j * kTile + rank * C::kKeysHeld;
             // a box without a key that some row sees is left out: its scores are masked
             const int nb = max(0, min(C::kKeysHeld / c.box, (w.any_hi - k0 + c.box - 1) >> c.box_shift));
@@ -518,7 +532,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (++stage == last_stage) stage = first_stage, ++round;
             }
         };
-        auto load_v = [&](int j, int pages) {
+        auto load_v = [&](int j, int raw_pages) {
+            const int pages = checked(raw_pages);
             const int k0 = w.lo + j * kTile, col0 = w.half * C::kDv + rank * C::kVCols;
             const int b1 = max(0, min(boxes, (w.any_hi - k0 + c.box - 1) >> c.box_shift));
             if (k0 >= w.any_lo && k0 + kTile <= w.any_hi) {
@@ -566,9 +581,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     count = at.count;
                     if (at.b < 0) continue;
                     const TileWork t = tile_work(c, at.g, at.tile);
-                    const int j0 = t.n * at.piece / at.pieces;           // this piece's key tiles
+                    int j0 = 0, n = t.n;                                 // this piece's key tiles
+                    if (at.pieces > 1) {
+                        j0 = t.n * at.piece / at.pieces;
+                        n = t.n * (at.piece + 1) / at.pieces - j0;
+                    }
                     it = {at.g.q0, at.g.q_len, at.g.first, at.g.kv_len, at.b, at.h, at.half, t.t0 + rank * c.tokens,
-                          t.lo + j0 * kTile, t.n * (at.piece + 1) / at.pieces - j0, t.any_lo, t.any_hi, at.pieces, at.slot};
+                          t.lo + j0 * kTile, n, t.any_lo, t.any_hi, at.pieces, at.slot};
                 }
                 return it;
             };
@@ -926,6 +945,9 @@ void launch_chunk_dim(const Attn& hd, const AttnCall& a, int few_rows, cudaStrea
     c.box = std::min(1 << a.pv.page_shift, 64);
     c.box_shift = std::min(a.pv.page_shift, 6);
     c.wave = device_sm_count() / C::kCtas;
+    c.by_tile_tokens = Divisor(c.tile_tokens);
+    c.by_wave = Divisor(c.wave);
+    c.by_per_tile = Divisor(a.hk * C::kHalves);
     // a sequence has at most one tile that is not full
     const int64_t tiles = std::min<int64_t>((int64_t)a.pv.rows / c.tile_tokens + a.pv.n_seqs,
                                             (int64_t)a.pv.n_seqs * ((a.pv.max_q + c.tile_tokens - 1) / c.tile_tokens));
