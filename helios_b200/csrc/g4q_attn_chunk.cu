@@ -8,22 +8,24 @@
 // and half of a V tile's columns, and the pair's MMAs read both halves: on single CTAs, which fetch twice as much,
 // one producer's page look-ups and boxes took 2600-4000 cycles a tile where the products are 2048 (head_dim 256).
 // The pair walks the 128-key tiles that its rows see, warp-specialised in each CTA:
-//   warps 0, 6  fill a ring of K and a ring of V stages (up to 32 KB each) by TMA: boxes of one page x 64 elements,
+//   warps 0, 10 fill a ring of K and a ring of V stages (up to 32 KB each) by TMA: boxes of one page x 64 elements,
 //               SWIZZLE_128B. A warp issues a box in about 90 cycles, and pages of 16 slots make 16 boxes a stage: one
-//               warp for both took 3200 cycles a tile.
+//               warp for both took 3200 cycles a tile. Warp 0 also loads Q and finds the work for all warps.
 //   warp 1      of the first CTA: one thread issues the MMAs: S = Q K^T (both operands K-major in shared memory,
 //               M = 256, N = 128) into one of two TMEM buffers, and O += P V (P from TMEM, V as it lies, MN-major)
 //               into up to 256 TMEM columns. S of tile j+1 is computed before P V of tile j, so the tensor cores
 //               have work while the softmax of tile j runs.
-//   warps 2-5   the softmax, one query row per thread: S from TMEM, row maximum, 2^(s - m) rounded to bf16 back
-//               over S. The maximum used, m, is only raised when a row exceeds it by more than 2^8: the weights
-//               stay below 256 (bf16 keeps its relative precision), and the output, which would have to be
-//               rescaled in TMEM, is touched in the first few tiles only. Then O / sum, whole rows at a time, to global memory.
+//   warps 2-9   the softmax, two threads to a row: S from TMEM, row maximum, 2^(s - m) rounded to bf16 back over S.
+//               The maximum used, m, is only raised when a row exceeds it by more than 2^8: the weights stay below
+//               256 (bf16 keeps its relative precision), and the output, which would have to be rescaled in TMEM, is
+//               touched in the first few tiles only. Then O / sum to global memory. With one thread to a row a tile's
+//               softmax was 1550 cycles of one warp per scheduler: 2530 cycles a tile at head_dim 256, now 2050.
 //
-// Bound by the tensor cores for a long context: 2048 tokens of 16 heads of 512 over 16384 keys take 960-1010 us back
-// to back, 1.15 ms among other work that draws power (1.34 PFLOP/s of products); a key tile takes 3520 cycles, 87 %
-// of them products. 2048 tokens of 16 heads of 256 with a window of 1024 (9 key tiles a row tile): 45 us, the first
-// softmax and the epilogue of each row tile being latency.
+// Bound by the tensor cores for a long context: a key tile takes its products' cycles (2050 measured of 2048 at head_dim
+// 256, three times 1024 at 512). 2048 tokens of 16 heads of 512 over 16384 keys: 900 us, at the 1.5 GHz that the power
+// limit leaves (1.7 PFLOP/s of products). 2048 tokens of 16 heads of 256 with a window of 1024, 9 or 10 key tiles a row
+// tile: 36 us at full clock, of which the start (finding the work 2 us, Q and K, the first softmax: 5 us) and each
+// tile's epilogue (2 us) are latency. head_dim 128 and 64: the exponentials, 1024 cycles of a tile, and 1750 a tile.
 //
 // head_dim 64: a pair would leave each CTA 32 columns of V, less than a swizzle row, and its tiles' bytes are few
 // for the softmax they take: single CTAs (cta_group::1) run the same code.
@@ -31,9 +33,9 @@
 // (1.5 times the products of a single pass; a row tile of 64 would halve the tensor cores' rate instead).
 // The row tiles (x key heads x halves) that fill the GPU in whole waves are computed whole, the longest of a causal
 // chunk first. The rest, which would leave SMs idle for a wave (or all of them, for a drafted block or a small chunk
-// over a long context), have their keys cut into as many pieces as there are CTAs for them, 6 key tiles or more
-// each; a join kernel adds the fp32 partials in piece order. The pairs are as many as fit the GPU, and each walks the
-// list back and forth (the first wave's order, then the reverse, so that a long tile is followed by a short one).
+// over a long context), have their keys cut into as many pieces as there are CTAs for them; a join kernel adds the fp32
+// partials in piece order. The pairs are as many as fit the GPU, and each walks the list back and forth (the first
+// wave's order, then the reverse, so that a long tile is followed by a short one).
 #include <cuda_runtime.h>
 
 #include <algorithm>
