@@ -19,7 +19,7 @@
 // columns over the 64 keys. mma.sync is enough here: at 64 rows a tile's products take less time than its bytes.
 //
 // Measured, with the join: 16 tokens over 69,823 keys in all (8 key heads of 256) 95 us, 6.0 TB/s of keys and values;
-// one token over a window of 1024 8.0 us and over 16384 keys of head_dim 512 12.5 us, latencies of a tile or two in
+// one token over a window of 1024 7.5 us and over 16384 keys of head_dim 512 12.4 us, latencies of a tile or two in
 // sequence and of the join.
 #include <cuda_runtime.h>
 
@@ -39,6 +39,17 @@ constexpr int kKeys = 64;            // keys per tile
 constexpr int kComputeWarps = 8;
 constexpr int kThreads = (kComputeWarps + 1) * 32;
 constexpr float kLog2e = 1.4426950408889634f;
+// Few units (sequence x key head) of few tiles, 16 rows at most and head_dim up to 256: a cluster of 8 CTAs has a unit to
+// itself and joins its partials in shared memory; there is no second launch. A CTA may have up to 3 tiles, and one more
+// than an even split over the GPU gives. One token over 300 keys, four sequences: 6.0 us against 8.4; four over a window of
+// 1024: 9.6 and 12.1; blocks of 8, of four sequences: 11.2 and 13.3. One token over a window of 1024 has one tile a CTA in
+// the even split and three here: 9.6 us and 8.7, its keys coming from memory. With more rows or at head_dim 512, where a
+// tile takes longer and one CTA fits an SM, fewer CTAs a unit cost more than the launch (15 tokens of two sequences, window
+// of 1024: 20.7 and 13.7; 1500 keys of head_dim 512, four sequences: 12.7 and 10.1).
+constexpr int kUnitCtas = 8, kUnitTiles = 3;
+template <int D, int MT>
+constexpr bool kUnitClusters = MT == 1 && D <= 256;
+constexpr float kNoTiles = -1.0f;    // in the place of a CTA's sums, which are not negative
 
 template <int D, int MT>
 struct FewCfg {
@@ -58,6 +69,7 @@ struct FewCfg {
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     static constexpr int kSmem = kFixed + kStages * kStageBytes;
     static_assert(kStages >= 2 * kParts && kSmem <= 227 * 1024, "ring does not fit");
+    static_assert(kRows * D * 4 <= kStages * kStageBytes, "a partial takes the ring's place");
 };
 
 struct FewCall {
@@ -180,7 +192,29 @@ __device__ __forceinline__ void ldmatrix4t(uint32_t addr, uint32_t& a, uint32_t&
 
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-template <int D, int MT>
+// Clusters: a unit's tiles belong to the kUnitCtas CTAs of a cluster, whose partials stay in shared memory and are
+// joined there.
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+template <int D, int MT, bool kCluster>
 __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
     attn_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                     const __grid_constant__ FewCall c) {
@@ -213,7 +247,21 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
     wait_for_predecessor();
     release_successor();
     int left;
-    Cursor cur = first_place(c, lane, left);
+    Cursor cur;
+    if constexpr (kCluster) {
+        const int unit = blockIdx.x / kUnitCtas, rank = blockIdx.x % kUnitCtas;
+        cur.b = unit / c.a.hk;
+        cur.h = unit % c.a.hk;
+        cur.w = seq_work(c, cur.b);
+        cur.t = cur.w.nt * rank / kUnitCtas;
+        left = cur.w.nt * (rank + 1) / kUnitCtas - cur.t;
+        if (left == 0 && threadIdx.x < C::kRows) {
+            s_max[threadIdx.x] = -INFINITY;
+            s_sum[threadIdx.x] = kNoTiles;
+        }
+    } else {
+        cur = first_place(c, lane, left);
+    }
     if (left > 0) {
         if (warp == kComputeWarps) {
             // ---------------- producer: K then V of every tile, in ring order
@@ -478,7 +526,12 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
                         if (r >= rows) continue;
                         const float sum = s_sum[r];
                         const int col = warp * (D / kComputeWarps) + 2 * t4;
-                        if (whole) {
+                        if constexpr (kCluster) {
+                            float* dst = reinterpret_cast<float*>(gen) + r * D + col;    // the ring has been read
+#pragma unroll
+                            for (int b = 0; b < kNt; ++b)
+                                *reinterpret_cast<float2*>(dst + 8 * b) = make_float2(o[a][b][2 * half], o[a][b][2 * half + 1]);
+                        } else if (whole) {
                             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // a row that sees nothing is zero
                             const int tok = r / c.group, hd = cur.h * c.group + r % c.group;
                             uint16_t* dst = c.a.out + (int64_t)(g.q0 + tok) * c.a.o_t + (int64_t)hd * c.a.o_h + col;
@@ -501,6 +554,40 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
                 if (left > 0) cur.next_unit(c);
             }
         }
+    }
+    if constexpr (kCluster) {
+        __syncwarp();
+        cluster_sync();      // no CTA leaves before the second one: the others read its shared memory
+        // each CTA joins its share of the unit's rows and columns, four columns a thread, in rank order
+        const SeqGeom g = cur.w.g;
+        const int rank = blockIdx.x % kUnitCtas, rows = cur.w.nt > 0 ? g.q_len * c.group : 0, items = rows * (D / 4);
+        const int end = items * (rank + 1) / kUnitCtas;
+        for (int i = items * rank / kUnitCtas + (int)threadIdx.x; i < end; i += kThreads) {
+            const int r = i / (D / 4), col = i % (D / 4) * 4;
+            float top = -INFINITY, m[kUnitCtas], l[kUnitCtas];
+#pragma unroll
+            for (int k = 0; k < kUnitCtas; ++k) {
+                m[k] = ld_cluster(in_cta(smem_addr(s_max + r), k));
+                l[k] = ld_cluster(in_cta(smem_addr(s_sum + r), k));
+                top = fmaxf(top, m[k]);
+            }
+            const float ref = top == -INFINITY ? 0.0f : top;
+            float sum = 0.0f;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < kUnitCtas; ++k) {
+                if (l[k] == kNoTiles) continue;      // its shared memory may hold anything
+                const float f = fast_exp2(m[k] - ref);
+                const float4 v = ld_cluster4(in_cta(base + (r * D + col) * 4, k));
+                sum += f * l[k];
+                acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+            }
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const int tok = r / c.group, hd = cur.h * c.group + r % c.group;
+            *reinterpret_cast<uint2*>(c.a.out + (int64_t)(g.q0 + tok) * c.a.o_t + (int64_t)hd * c.a.o_h + col) =
+                make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+        }
+        cluster_sync();
     }
 }
 
@@ -633,8 +720,11 @@ void launch_few(const Attn& h, const AttnCall& a, cudaStream_t st) {
     static bool attr_set[64] = {false};
     const int dev = current_device();
     if (!attr_set[dev & 63]) {
-        check_cuda(cudaFuncSetAttribute(attn_few_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
+        check_cuda(cudaFuncSetAttribute(attn_few_kernel<D, MT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
                    "cudaFuncSetAttribute(attn_few)");
+        if constexpr (kUnitClusters<D, MT>)
+            check_cuda(cudaFuncSetAttribute(attn_few_kernel<D, MT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
+                       "cudaFuncSetAttribute(attn_few)");
         attr_set[dev & 63] = true;
     }
     const int page_size = 1 << a.pv.page_shift;
@@ -652,9 +742,18 @@ void launch_few(const Attn& h, const AttnCall& a, cudaStream_t st) {
     if (a.window > 0) cap = std::min<int64_t>(cap, (int64_t)a.window + c.max_rows / c.group + c.box);
     const int64_t per_unit = std::max<int64_t>(1, (cap + kKeys - 1) / kKeys);
     if (per_unit * a.hk * a.pv.n_seqs > 0x7FFFFFFF) throw Error(G4Q_ERR_UNSUPPORTED_CONFIG, "too many key tiles for one call");
-    c.ctas = (int)std::min<int64_t>(few_ctas<D, MT>(), per_unit * a.hk * a.pv.n_seqs);
+    const int64_t units = (int64_t)a.hk * a.pv.n_seqs;
+    c.ctas = (int)std::min<int64_t>(few_ctas<D, MT>(), per_unit * units);
     const CUtensorMap tk = paged_map(a, a.k, D, c.box), tv = paged_map(a, a.v, D, c.box);
-    launch_dependent(attn_few_kernel<D, MT>, dim3((unsigned)c.ctas), dim3(kThreads), C::kSmem, st, tk, tv, c);
+    if constexpr (kUnitClusters<D, MT>) {
+        const int64_t mine = (per_unit + kUnitCtas - 1) / kUnitCtas, even = (per_unit * units + c.ctas - 1) / c.ctas;
+        if (per_unit > 1 && mine <= std::min<int64_t>(kUnitTiles, even + 1) && units * kUnitCtas <= few_ctas<D, MT>()) {
+            launch_dependent<kUnitCtas>(attn_few_kernel<D, MT, true>, dim3((unsigned)(units * kUnitCtas)), dim3(kThreads),
+                                        C::kSmem, st, tk, tv, c);
+            return;
+        }
+    }
+    launch_dependent(attn_few_kernel<D, MT, false>, dim3((unsigned)c.ctas), dim3(kThreads), C::kSmem, st, tk, tv, c);
     if (per_unit > 1) {   // a unit of one tile is never cut
         // Few items with possibly many partials each: a block to an item. Else two warps: the blocks are few then,
         // and a unit has about as many partials as CTAs there are to a unit.

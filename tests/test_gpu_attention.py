@@ -236,6 +236,37 @@ def test_attention_window_one_token(cuda, window):
     check_attention([1, 1, 1], [1, 64, 1333], 4, 2, 256, 16, window)
 
 
+@pytest.mark.parametrize("d,hq,hk", [(64, 12, 4), (128, 32, 8), (256, 16, 8), (256, 1, 1)])
+@pytest.mark.parametrize("q_lens,kv_lens,window", [([1], [65], 0), ([1], [1536], 0), ([1], [1537], 0), ([2, 0, 1], [700, 0, 3], 0),
+                                                   ([1, 3, 1, 2], [5000, 3, 1100, 900], 1024), ([1, 1], [0, 500], 0)])
+def test_attention_few_units_of_few_tiles(cuda, d, hq, hk, q_lens, kv_lens, window):
+    if 0 not in kv_lens or q_lens[kv_lens.index(0)] == 0:
+        check_attention(q_lens, kv_lens, hq, hk, d, 64, window, behind=1)
+        return
+    from helios_b200 import _lib
+    from helios_b200 import attention as A
+    s = Step(q_lens, kv_lens, hk, d, 64, 11)                  # more new tokens than keys: reported, zeros
+    q = randn(s.rows, hq, d, seed=12)
+    out = A.PagedAttention(hq, hk, d)(q, s.cache, s.batch)
+    assert _lib.device_error() == _lib.ERR_LENS
+    close(out, *s.reference(q, d ** -0.5, 0))
+    assert not out[0].any() and out[1].any()
+
+
+def test_a_row_of_nan_scores_is_nan(cuda):
+    """A query that is NaN has no maximum: its row is NaN, the others are not; few units, many, and a chunk."""
+    from helios_b200 import attention as A
+    for q_lens, kv_lens in (([1, 1], [300, 200]), ([1, 1], [5000, 200]), ([100], [300])):
+        s = Step(q_lens, kv_lens, 2, 128, 16, 61)
+        q = randn(s.rows, 4, 128, seed=62)
+        q[1, 2] = NAN
+        out = A.PagedAttention(4, 2, 128)(q, s.cache, s.batch)
+        assert out[1, 2].isnan().all()
+        out[1, 2], q[1, 2] = 0, 0
+        assert not out.isnan().any()
+        no_device_error()
+
+
 @pytest.mark.parametrize("order", ["shd", "layers"])
 def test_attention_cache_orders(cuda, order):
     check_attention([1, 3], [90, 200], 8, 4, 128, 32, 0, order=order)
