@@ -233,6 +233,11 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
     auto full = [&](int s) { return s_bar + 8u * s; };
     auto empty = [&](int s) { return s_bar + 8u * (C::kStages + s); };
 
+    bool gave_up = false;
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+        if (!bar_wait(bar, parity, c.err, code)) gave_up = true;
+    };
+
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == kComputeWarps * 32) {
         for (int s = 0; s < C::kStages; ++s) {
@@ -277,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
                 const int nb = min(boxes, (cur.w.g.kv_len - k0 + c.box - 1) / c.box);
 #pragma unroll 1
                 for (int part = 0; part < 2 * C::kParts; ++part) {
-                    if (round > 0) bar_wait(empty(stage), (round - 1) & 1, c.err, 70);
+                    if (round > 0) wait(empty(stage), (round - 1) & 1, 70);
                     const CUtensorMap* map = part < C::kParts ? &tm_k : &tm_v;
                     const int col0 = (part % C::kParts) * C::kCols;
                     if (lane == 0) bar_expect_tx(full(stage), (uint32_t)max(nb, 0) * box_bytes * (C::kCols / 64));
@@ -363,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
                     uint32_t rd = round;
 #pragma unroll
                     for (int part = 0; part < C::kParts; ++part) {
-                        bar_wait(full(st), rd & 1, c.err, 71);
+                        wait(full(st), rd & 1, 71);
                         const uint32_t kb = s_ring + st * C::kStageBytes + (8 * warp + (lane & 7)) * 128;
 #pragma unroll(MT == 1 ? 8 : 2)
                         for (int kk = 0; kk < C::kCols / 32; ++kk) {
@@ -452,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
                         uint32_t vr = round;
 #pragma unroll
                         for (int part = 0; part < C::kParts; ++part) {
-                            bar_wait(full(vs), vr & 1, c.err, 72);
+                            wait(full(vs), vr & 1, 72);
                             uint8_t* vb = gen + (s_ring - base) + vs * C::kStageBytes;
                             for (int i = threadIdx.x; i < kKeys * (C::kCols / 8); i += 256) {
                                 const int key = (i >> 3) & (kKeys - 1);
@@ -472,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
                         int vs = stage + part;
                         uint32_t vr = round;
                         if (vs >= C::kStages) vs -= C::kStages, ++vr;
-                        bar_wait(full(vs), vr & 1, c.err, 73);
+                        wait(full(vs), vr & 1, 73);
                         const uint32_t vb = s_ring + vs * C::kStageBytes;
 #pragma unroll
                         for (int a = 0; a < MT; ++a) {
@@ -555,6 +560,7 @@ __global__ void __launch_bounds__(kThreads, FewCfg<D, MT>::kTwo ? 2 : 1)
             }
         }
     }
+    if (gave_up) let_copies_land();
     if constexpr (kCluster) {
         __syncwarp();
         cluster_sync();      // no CTA leaves before the second one: the others read its shared memory

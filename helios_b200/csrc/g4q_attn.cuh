@@ -146,9 +146,9 @@ __device__ __forceinline__ void bar_arrive(uint32_t bar) {
 
 constexpr long long kAttnWaitCycles = 4000000000ll;   // ~2 s at 2 GHz
 
-// Bounded wait on an mbarrier phase. A wait that gives up records `code` in the device error word; every
+// Bounded wait on an mbarrier phase; false: it gave up. Such a wait records `code` in the device error word; every
 // other wait on the device then returns at once, so the kernel runs to its end.
-__device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, int* err, int code) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int* err, int code) {
     long long t0 = 0;
     for (uint32_t it = 0;; ++it) {
         uint32_t done;
@@ -159,16 +159,24 @@ __device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, int* err
             : "=r"(done)
             : "r"(bar), "r"(parity)
             : "memory");
-        if (done) return;
+        if (done) return true;
         if (it == 0) {
             t0 = clock64();
         } else if ((it & 255u) == 255u) {
-            if (*reinterpret_cast<volatile int*>(err) != 0) return;
+            if (*reinterpret_cast<volatile int*>(err) != 0) return false;
             if (clock64() - t0 > kAttnWaitCycles) {
                 atomicCAS(err, 0, code);
-                return;
+                return false;
             }
         }
+    }
+}
+
+// What a warp does at its end after a wait that gave up: it keeps the CTA's shared memory for about a millisecond, in
+// which the copies that were issued have long landed.
+__device__ __forceinline__ void let_copies_land() {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) {
     }
 }
 

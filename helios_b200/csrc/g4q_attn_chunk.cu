@@ -434,6 +434,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     Item* s_item = reinterpret_cast<Item*>(gen + (s_bar - base) + 256);
     float* s_max = reinterpret_cast<float*>(s_item + kItems);                // [parity of the exchange][half][row]
 
+    bool gave_up = false;
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+        if (!bar_wait(bar, parity, c.err, code)) gave_up = true;
+    };
+
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = blockIdx.x % kCtas;                 // place in the pair
     const int cluster = blockIdx.x / kCtas;
@@ -484,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Warp 0 finds the work: a search takes 2000 to 4000 cycles, which every warp would wait for. It is at most three
     // items ahead of the others, as Q of an item is only loaded when the scores of the one before are done.
     auto take = [&] {
-        bar_wait(work_full(done), done / kItems & 1, c.err, 90);
+        wait(work_full(done), done / kItems & 1, 90);
         w = s_item[done % kItems];
         return w.n > 0;
     };
@@ -519,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t dst = s_ring + stage * C::kStageBytes + cb * (keys * 128) + box * box_bytes;
             const int slot = (k0 + box * c.box) & page_mask, count = (b1 - b0) * blocks;
             const uint32_t bar = edge ? edge_full : in_first_cta(full(stage));
-            if (round > 0) bar_wait(empty(stage), (round - 1) & 1, c.err, 80);
+            if (round > 0) wait(empty(stage), (round - 1) & 1, 80);
             if (lane == 0) bar_expect_tx_cluster(bar, (uint32_t)count * box_bytes);
             __syncwarp();
             if (lane < count) tma_page<kCtas>(dst, map, col0 + cb * 64, slot, w.h, page, bar);
@@ -545,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // is filled on a barrier of this CTA's own, their rows are zeroed, and it is handed over then.
                 const int b0 = max(0, w.any_lo - k0) >> c.box_shift;
                 fill(&tm_v, true, pages, k0, kTile, 0, min(b0, b1), b1, col0, C::kVCols / 64);
-                bar_wait(edge_full, edge_round++ & 1, c.err, 88);
+                wait(edge_full, edge_round++ & 1, 88);
                 const int lo = min(kTile, max(0, w.any_lo - k0)), hi = min(kTile, max(lo, w.any_hi - k0));
                 for (int i = lane; i < (lo + kTile - hi) * (C::kVCols / 8); i += 32) {
                     const int ch = i & 7, x = i >> 3, cb = x % (C::kVCols / 64);
@@ -606,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             hand_out(w);
             while (w.n > 0) {
                 int pages = look_up(0), pages1 = look_up(1);
-                if (done > 0) bar_wait(q_free, (done - 1) & 1, c.err, 89);
+                if (done > 0) wait(q_free, (done - 1) & 1, 89);
                 if (lane == 0) {
                     const uint32_t qb = in_first_cta(q_full);
                     bar_expect_tx_cluster(qb, (uint32_t)(c.tokens * c.group) * 128u * (D / 64));
@@ -637,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t round = 0, v_round = 0;
             auto scores = [&](int j) {
                 for (int p = 0; p < C::kKSt; ++p) {
-                    bar_wait(full(stage), round & 1, c.err, 81);
+                    wait(full(stage), round & 1, 81);
                     tc_fence_after();
                     if (elect()) {
                         const uint32_t q = desc_low(s_q + p * (C::kKCols / 64) * (kTile * 128), 16);
@@ -661,13 +666,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             while (take()) {
                 const int n = w.n;
-                bar_wait(q_full, done & 1, c.err, 82);
+                wait(q_full, done & 1, 82);
                 scores(0);
                 for (int j = 0; j < n; ++j) {
                     if (j + 1 < n) scores(j + 1);
                     const uint32_t b = (g + j) & 1;
-                    bar_wait(p_full(b), ((g + j) >> 1) & 1, c.err, 83);
-                    bar_wait(full(v_stage), v_round & 1, c.err, 84);
+                    wait(p_full(b), ((g + j) >> 1) & 1, 83);
+                    wait(full(v_stage), v_round & 1, 84);
                     tc_fence_after();
                     if (elect()) {
                         const uint32_t v = desc_low(s_ring + v_stage * C::kStageBytes, kTile * 128);
@@ -725,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < n; ++j) {
                 const int k0 = w.lo + j * kTile + side * kKeys;
                 const uint32_t b = (g + j) & 1, ts = t_s + b * kTile + lanes;
-                bar_wait(s_full(b), ((g + j) >> 1) & 1, c.err, 85);
+                wait(s_full(b), ((g + j) >> 1) & 1, 85);
                 tc_fence_after();
                 uint32_t s[kKeys];
 #pragma unroll
@@ -754,7 +759,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float m_new = fmaxf(m, tile_max);
                     const float f = fast_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));
                     if (j > 0) {
-                        bar_wait(o_done(b ^ 1), ((g + j - 1) >> 1) & 1, c.err, 86);
+                        wait(o_done(b ^ 1), ((g + j - 1) >> 1) & 1, 86);
                         tc_fence_after();
 #pragma unroll 1
                         for (int x = 0; x < kCols; x += 32) {
@@ -790,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             l += swap(l);
             // ---------------- epilogue (before the next work's first weights, so its products do not start yet)
-            bar_wait(o_done((g + n - 1) & 1), ((g + n - 1) >> 1) & 1, c.err, 87);
+            wait(o_done((g + n - 1) & 1), ((g + n - 1) >> 1) & 1, 87);
             tc_fence_after();
             const bool last = w.pieces == 1;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -839,6 +844,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++done;
         }
     }
+    if (gave_up) let_copies_land();
     // The pair's MMAs read both CTAs' shared memory and signal both: neither leaves before the other is done.
     tc_fence_before();
     __syncthreads();
