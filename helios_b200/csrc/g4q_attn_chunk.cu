@@ -755,7 +755,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float tile_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
                 // after this the other thread has read its scores too, over which this one's weights will lie
                 tile_max = fmaxf(tile_max, swap(tile_max));
-                if (__any_sync(0xFFFFFFFFu, tile_max > m + kRaise)) {
+                // rows of no token hold anything: they have no say, or the others' last bits would depend on it
+                if (__any_sync(0xFFFFFFFFu, mine && tile_max > m + kRaise)) {
                     const float m_new = fmaxf(m, tile_max);
                     const float f = fast_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));
                     if (j > 0) {

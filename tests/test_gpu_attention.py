@@ -330,6 +330,24 @@ def test_attention_chunk_split_over_a_long_context(cuda):
     check_attention([16, 16], [3000, 17], 16, 1, 512, 64, 0)
 
 
+@pytest.mark.parametrize("d,hq,hk", [(64, 12, 4), (128, 12, 4), (256, 6, 2), (512, 3, 1)])
+def test_attention_chunk_same_bits_whatever_ran_before(cuda, d, hq, hk):
+    """Three heads a group: 42 tokens of a tile leave two spare rows, which hold what the call before left in shared
+    memory. Large queries of four heads a group are that call."""
+    from helios_b200 import attention as A
+    s = Step([300, 77], [900, 400], hk, d, 32, 71)
+    q = randn(s.rows, hq, d, seed=72)
+    attend, other = A.PagedAttention(hq, hk, d), A.PagedAttention(4 * hk, hk, d)
+    want = None
+    for i in range(12):
+        large = randn(s.rows, 4 * hk, d, seed=80 + i, std=4.0 ** (i % 4))
+        other(large, s.cache, s.batch, scale=1.0)
+        got = attend(q, s.cache, s.batch, scale=1.0)
+        want = got if want is None else want
+        assert torch.equal(got, want), i
+    no_device_error()
+
+
 def test_attention_chunk_peaked_scores(cuda):
     check_attention([150], [500], 16, 1, 512, 64, 0, scale=1.0)
 
