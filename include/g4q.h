@@ -495,8 +495,8 @@ G4qStatus g4q_comm_free(G4qComm* comm);
  * per-device error word and the kernel runs to its end (its results are then invalid). This
  * reads the word for the current device (synchronising it) and optionally clears it; it also
  * reports (and clears) code 50 of g4q_lm_head_argmax_noalloc and the codes 60-62 of a paged batch
- * (G4qPagedBatch), and allocates nothing. No
- * reference counterpart: the reference's MLX graph has no device-side waits. */
+ * (G4qPagedBatch), and allocates nothing. Codes 70-73 and 80-90 are waits of g4q_paged_attention. No reference
+ * counterpart: the reference's MLX graph has no device-side waits. */
 G4qStatus g4q_device_error(int32_t* code, int32_t reset);
 
 /* ---- seeded synthetic data (no reference counterpart: benchmark / test inputs) ---------------
