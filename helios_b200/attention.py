@@ -89,7 +89,8 @@ class PagedKVCache:
     """One layer's keys and values in pages: ``k`` and ``v`` bf16 [pages, kv_heads, page_size, head_dim]
     CUDA tensors of equal strides (page_size a power of two, 16 or more). Any stride order qualifies while
     head_dim is contiguous, so ``t.transpose(1, 2)`` of a [pages, page_size, kv_heads, head_dim] tensor does,
-    and so does one layer's slice of a tensor that holds them all. The tensors stay the caller's."""
+    and so does one layer's slice of a tensor that holds them all. The tensors stay the caller's. Elements that ``k``
+    and ``v``, or two of a tensor's slots, share can be read; :func:`kv_append` refuses them."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
         for t, name in ((k, "k"), (v, "v")):

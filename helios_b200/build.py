@@ -23,7 +23,7 @@ OBJDIR = PKG / "_build"
 SOURCES = ["g4q_api.cu", "g4q_layout.cu", "g4q_gemv.cu", "g4q_gemv2.cu", "g4q_gemm.cu", "g4q_decode.cu",
            "g4q_generic.cu", "g4q_comm.cu", "g4q_lora.cu", "g4q_mlp.cu", "g4q_rope.cu",
            "g4q_attn.cu", "g4q_attn_chunk.cu"]
-HEADERS = ["g4q_common.cuh", "g4q_internal.h", "g4q_attn.cuh"]
+HEADERS = ["g4q_common.cuh", "g4q_internal.h", "g4q_overlap.h", "g4q_attn.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

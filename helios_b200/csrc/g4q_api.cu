@@ -17,6 +17,7 @@
 #include "g4q.h"
 #include "g4q_attn.cuh"
 #include "g4q_internal.h"
+#include "g4q_overlap.h"
 
 namespace g4q {
 
@@ -1190,6 +1191,8 @@ G4qStatus g4q_kv_append(const G4qRope* rope, const G4qHeadRows* q, const G4qHead
         require((flags & ~G4Q_APPEND_RAW_VALUES) == 0, G4Q_ERR_INVALID_ARGUMENT, "unknown flag bits");
         const PagedView pv = checked_batch(cache, batch, M);
         require(cache->head_dim == r->head_dim, G4Q_ERR_INVALID_ARGUMENT, "the cache's head_dim is not the rope's");
+        // warps store a slot's key and value, and the slots of a step, in no order
+        if (const char* wrong = shared_slots(*cache)) throw Error(G4Q_ERR_INVALID_ARGUMENT, wrong);
         if (M == 0) return;
         require(k != nullptr && v != nullptr, G4Q_ERR_INVALID_ARGUMENT, "k and v must be non-null");
         HeadRowsCall c = head_rows_call(*r, q, q_out, k, M, q_weight, k_weight, eps);

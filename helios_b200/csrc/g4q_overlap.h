@@ -1,0 +1,80 @@
+// g4q_overlap.h -- whether the strided tensors of a call share elements: host arithmetic on addresses and strides.
+#pragma once
+
+#include <cstdint>
+#include <utility>
+
+#include "g4q.h"
+
+namespace g4q {
+
+// Rows of d contiguous elements on up to three axes, the longest stride first (axes of one row are left out).
+struct Lattice {
+    using Wide = __int128;           // a caller's strides times counts may pass 64 bits
+    int64_t stride[3], count[3], d;
+    int axes = 0;
+
+    void add(int64_t s, int64_t n) {
+        if (n <= 1) return;
+        int i = axes++;
+        for (; i > 0 && stride[i - 1] < s; --i) stride[i] = stride[i - 1], count[i] = count[i - 1];
+        stride[i] = s, count[i] = n;
+    }
+
+    // From the first row's first element to the last one's end, of the axes from `axis` on.
+    Wide span(int axis = 0) const {
+        Wide e = d;
+        for (; axis < axes; ++axis) e += (Wide)stride[axis] * (count[axis] - 1);
+        return e;
+    }
+
+    // No step of an axis is shorter than what lies inside of it, so no two rows share an element.
+    bool nested() const {
+        for (int i = 0; i < axes; ++i)
+            if (stride[i] < span(i + 1)) return false;
+        return true;
+    }
+
+    // Whether the same lattice, its first row `gap` elements on, shares an element with this one. Where the axes are nested
+    // this is exact: the steps i between a row of each leave |gap - sum(i stride)| < d, and an axis has at most three
+    // candidates for its i. Else lattices whose spans overlap are taken to share some.
+    bool meets_shifted(Wide gap) const {
+        if (gap >= span() || -gap >= span()) return false;
+        return !nested() || differ_by(gap, 0);
+    }
+
+private:
+    static Wide floor_div(Wide a, int64_t b) { return a >= 0 ? a / b : -((-a + b - 1) / b); }
+
+    bool differ_by(Wide gap, int axis) const {
+        if (axis == axes) return gap < d && -gap < d;
+        const int64_t s = stride[axis];
+        const Wide reach = span(axis + 1), most = count[axis] - 1;   // |gap - i s| < reach
+        Wide lo = -floor_div(reach - 1 - gap, s), hi = floor_div(gap + reach - 1, s);
+        if (lo < -most) lo = -most;
+        if (hi > most) hi = most;
+        for (Wide i = lo; i <= hi; ++i)
+            if (differ_by(gap - i * s, axis + 1)) return true;
+        return false;
+    }
+};
+
+// The slots of a cache's k (or v), one row a head.
+inline Lattice cache_lattice(const G4qPagedCache& c) {
+    Lattice l;
+    l.d = c.head_dim;
+    l.add(c.page_stride, c.n_pages);
+    l.add(c.head_stride, c.n_kv_heads);
+    l.add(c.slot_stride, c.page_size);
+    return l;
+}
+
+// What an append to the cache would write from several warps at once; null where every slot of k and v is its own.
+inline const char* shared_slots(const G4qPagedCache& c) {
+    const Lattice l = cache_lattice(c);
+    if (!l.nested()) return "cache: pages, heads and slots must not overlap";
+    if (l.meets_shifted(c.v - c.k)) return "cache: k and v share elements";
+    return nullptr;
+}
+
+}  // namespace g4q

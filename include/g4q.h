@@ -345,8 +345,9 @@ G4qStatus g4q_qk_norm_rope(const G4qRope* rope, const G4qHeadRows* q, const G4qH
 
 /* The same on the new tokens of a paged batch, at their positions in it: the keys are stored in the cache's
  * pages, the values beside them (rms_norm without a weight; with G4Q_APPEND_RAW_VALUES as they are). v may be
- * k (full-attention layers, whose key projection is the value too: :820-822). q (with q_out) may be NULL; q_out
- * may be q, else it must not overlap q, k or v. */
+ * k (full-attention layers, whose key projection is the value too: :820-822), but what is stored of the two differs:
+ * caches whose k and v, or pages, heads and slots, share elements are refused (they may be read by g4q_paged_attention).
+ * q (with q_out) may be NULL; q_out may be q, else it must not overlap q, k or v. */
 #define G4Q_APPEND_RAW_VALUES 0x1u
 G4qStatus g4q_kv_append(const G4qRope* rope, const G4qHeadRows* q, const G4qHeadRows* k, const G4qHeadRows* v, int64_t M,
                         const uint16_t* q_weight, const uint16_t* k_weight, float eps, uint32_t flags,

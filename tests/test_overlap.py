@@ -1,0 +1,102 @@
+"""The host arithmetic that tells whether a call's tensors share elements (csrc/g4q_overlap.h), compiled with the host
+compiler, against sets of elements."""
+import itertools
+import random
+import subprocess
+
+import pytest
+
+from conftest import ROOT
+
+D = 8
+
+PROGRAM = r"""
+#include <cstdio>
+#include "g4q_overlap.h"
+int main() {
+    G4qPagedCache c;
+    long long k, v, n, ps, hs, ss;
+    while (std::scanf("%lld %lld %lld %d %d %lld %lld %lld", &k, &v, &n, &c.page_size, &c.n_kv_heads, &ps, &hs, &ss) == 8) {
+        c.k = (uint16_t*)0 + k, c.v = (uint16_t*)0 + v;
+        c.n_pages = n, c.head_dim = 8;
+        c.page_stride = ps, c.head_stride = hs, c.slot_stride = ss;
+        const char* wrong = g4q::shared_slots(c);
+        std::printf("%d %s\n", (int)g4q::cache_lattice(c).nested(), wrong ? wrong : "-");
+    }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def answers(tmp_path_factory):
+    """For cases (k, v, pages, page_size, heads, page_stride, head_stride, slot_stride): (nested, what is wrong)."""
+    at = tmp_path_factory.mktemp("overlap")
+    (at / "main.cpp").write_text(PROGRAM)
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover", "-I",
+                    str(ROOT / "include"), "-I", str(ROOT / "helios_b200" / "csrc"), str(at / "main.cpp"), "-o", str(at / "main")],
+                   check=True)
+
+    def ask(cases):
+        text = "\n".join(" ".join(map(str, c)) for c in cases)
+        out = subprocess.run([str(at / "main")], input=text, check=True, capture_output=True, text=True).stdout.splitlines()
+        assert len(out) == len(cases)
+        return [(line[0] == "1", line[2:]) for line in out]
+
+    return ask
+
+
+def rows(base, counts, strides):
+    return [base + sum(i * s for i, s in zip(at, strides)) for at in itertools.product(*(range(n) for n in counts))]
+
+
+def elements(starts):
+    return [e for r in starts for e in range(r, r + D)]
+
+
+def test_caches_against_sets_of_elements(answers):
+    """Layouts of all orders with gaps, single axes and shared elements: the refusals are those of the sets, except that
+    axes which interleave without sharing are refused too."""
+    rng = random.Random(1)
+    cases = []
+    for _ in range(6000):
+        counts = [rng.choice([1, 2, 3]) for _ in range(3)]
+        strides = [0, 0, 0]
+        inner = D
+        for axis in rng.sample(range(3), 3):
+            strides[axis] = inner + rng.choice([0, 0, 8, 24]) if rng.random() < 0.9 else 8 * rng.randrange(1, 9)
+            inner = max(inner, strides[axis] * counts[axis])
+        k = 4096
+        cases.append((k, k + 8 * rng.randrange(-24, 25), counts[0], counts[2], counts[1], strides[0], strides[1], strides[2]))
+    wrong = {"nested": 0, "shared": 0}
+    for (k, v, pages, slots, heads, ps, hs, ss), (nested, text) in zip(cases, answers(cases)):
+        ke, ve = (elements(rows(b, (pages, heads, slots), (ps, hs, ss))) for b in (k, v))
+        if nested:
+            assert len(set(ke)) == len(ke)
+            assert (text != "-") == bool(set(ke) & set(ve)), (k, v, pages, slots, heads, ps, hs, ss)
+            wrong["shared"] += text == "cache: k and v share elements"
+        else:
+            assert text == "cache: pages, heads and slots must not overlap"
+            wrong["nested"] += 1
+        if len(set(ke)) < len(ke) or set(ke) & set(ve):
+            assert text != "-"
+    assert min(wrong.values()) > 200 and sum(wrong.values()) < 5000
+
+
+def test_usual_caches_qualify(answers):
+    page, heads, pages, d = 16, 2, 4, D
+    block = page * heads * d
+    usual = [(0, pages * block, pages, page, heads, block, page * d, d),                       # two tensors behind each other
+             (0, pages * block, pages, page, heads, block, d, heads * d),                      # slots before heads
+             (0, block, pages, page, heads, 2 * block, page * d, d),                           # k and v of a page in turn
+             (0, d, pages, page, heads, 2 * block, 2 * page * d, 2 * d),                       # k and v of a slot in turn
+             (3 * block, 3 * pages * block + 3 * block, pages, page, heads, 3 * block, page * d, d),   # one layer of three
+             (0, 2 ** 40, 2 ** 31 - 2, 65536, 65535, 2 ** 38 - 8, d * 65536, d)]               # far beyond any memory
+    got = answers(usual)
+    assert [text for _, text in got[:5]] == ["-"] * 5
+    assert got[5][1] != "-"
+
+
+def test_one_tensor_for_keys_and_values(answers):
+    """The key projection is the value too in some layers, but what is stored of it is not."""
+    assert answers([(64, 64, 3, 16, 1, 128, 128, 8), (64, 64 + 8, 3, 16, 1, 128, 128, 8)]) == \
+        [(True, "cache: k and v share elements")] * 2
