@@ -182,7 +182,7 @@ def kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cache
     pages, values normalized (without a weight; ``norm_values=False`` stores them as they are) beside them,
     and the queries, treated like the keys with ``q_weight``, returned (None for q None). One launch. ``v``
     may be ``k``. Sequences may share pages of a common prefix, but no two may append to one slot. Rows that
-    belong to no sequence are left as they were (in ``q_out`` too)."""
+    belong to no sequence are left as they were (in ``q_out`` too). No tensor may overlap the cache."""
     dev = rope.device
     _same_device(dev, cache, batch)
     return rope._ops.kv_append(rope.handle.value, rope.head_dim, dev, _raw_stream(dev), q, k, v, cache.c_addr,
@@ -215,7 +215,7 @@ class PagedAttention:
         the query at position t sees the keys j <= t, and j > t - window when window > 0. ``scale`` defaults
         to ``head_dim ** -0.5``. Single tokens, drafted blocks and prompt chunks may be mixed. A row that sees
         no key is zero; rows that belong to no sequence are left as they were (in ``out``, which must not overlap
-        q)."""
+        q or the cache)."""
         dev = self.device
         _same_device(dev, cache, batch)
         return self._ops.paged_attention(self.handle.value, self.head_dim, dev, _raw_stream(dev), q, cache.c_addr,

@@ -1040,6 +1040,11 @@ static void check_output(const G4qHeadRows* out, const G4qHeadRows* own, std::in
     if (bad) throw Error(G4Q_ERR_INVALID_ARGUMENT, std::string(name) + " overlaps other rows of the call");
 }
 
+// Rows that a call reads or writes while the cache's pages are written, or writes while they are read.
+static void check_outside(const G4qHeadRows* t, int64_t M, const G4qPagedCache& c, const Lattice& l, const char* name) {
+    if (meets_cache(*t, M, c, l)) throw Error(G4Q_ERR_INVALID_ARGUMENT, std::string(name) + " overlaps the cache");
+}
+
 static void check_aligned(const uint16_t* w, const char* name) {
     if ((reinterpret_cast<uintptr_t>(w) & 15u) != 0) require_aligned16(w, name);
 }
@@ -1199,7 +1204,14 @@ G4qStatus g4q_kv_append(const G4qRope* rope, const G4qHeadRows* q, const G4qHead
         check_heads(v, r->head_dim, "v");
         require(k->n_heads == cache->n_kv_heads && v->n_heads == cache->n_kv_heads, G4Q_ERR_INVALID_ARGUMENT,
                 "k and v must have the cache's heads");
-        if (q != nullptr) check_output(q_out, q, {k, v}, M, r->head_dim, "q_out");
+        const Lattice slots = cache_lattice(*cache);
+        check_outside(k, M, *cache, slots, "k");
+        check_outside(v, M, *cache, slots, "v");
+        if (q != nullptr) {
+            check_output(q_out, q, {k, v}, M, r->head_dim, "q_out");
+            check_outside(q, M, *cache, slots, "q");
+            check_outside(q_out, M, *cache, slots, "q_out");
+        }
         c.v = v->data, c.v_t = v->token_stride, c.v_h = v->head_stride, c.hv = v->n_heads;
         c.raw_v = (flags & G4Q_APPEND_RAW_VALUES) ? 1 : 0;
         c.k_out = cache->k, c.v_out = cache->v;
@@ -1289,6 +1301,7 @@ G4qStatus g4q_paged_attention(const G4qAttn* attn, const G4qHeadRows* q, int64_t
         require(M == 1 || q->token_stride >= a->head_dim, G4Q_ERR_INVALID_ARGUMENT, "q.token_stride must be >= head_dim");
         // several CTAs read a query row, and one may write its result before another has read it
         require(!heads_overlap(*out, *q, M, a->head_dim), G4Q_ERR_INVALID_ARGUMENT, "out must not be q, nor overlap it");
+        check_outside(out, M, *cache, cache_lattice(*cache), "out");
         AttnCall c = {};
         c.q = q->data, c.q_t = q->token_stride, c.q_h = q->head_stride;
         c.out = out->data, c.o_t = out->token_stride, c.o_h = out->head_stride;

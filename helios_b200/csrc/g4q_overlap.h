@@ -43,6 +43,12 @@ struct Lattice {
         return !nested() || differ_by(gap, 0);
     }
 
+    // Whether d elements from `gap` elements behind the first row's first one on lie in some row too; exact likewise.
+    bool meets_row(Wide gap) const {
+        if (gap >= span() || -gap >= d) return false;
+        return !nested() || holds(gap, 0);
+    }
+
 private:
     static Wide floor_div(Wide a, int64_t b) { return a >= 0 ? a / b : -((-a + b - 1) / b); }
 
@@ -55,6 +61,17 @@ private:
         if (hi > most) hi = most;
         for (Wide i = lo; i <= hi; ++i)
             if (differ_by(gap - i * s, axis + 1)) return true;
+        return false;
+    }
+
+    bool holds(Wide gap, int axis) const {
+        if (axis == axes) return gap < d && -gap < d;
+        const int64_t s = stride[axis];
+        Wide lo = -floor_div(span(axis + 1) - 1 - gap, s), hi = floor_div(gap + d - 1, s);   // -d < gap - i s < the inner span
+        if (lo < 0) lo = 0;
+        if (hi > count[axis] - 1) hi = count[axis] - 1;
+        for (Wide i = lo; i <= hi; ++i)
+            if (holds(gap - i * s, axis + 1)) return true;
         return false;
     }
 };
@@ -75,6 +92,22 @@ inline const char* shared_slots(const G4qPagedCache& c) {
     if (!l.nested()) return "cache: pages, heads and slots must not overlap";
     if (l.meets_shifted(c.v - c.k)) return "cache: k and v share elements";
     return nullptr;
+}
+
+// Whether M tokens of head rows share elements with the cache's slots. Only rows between the ends of k or v are looked at one
+// by one: those of a buffer that holds both.
+inline bool meets_cache(const G4qHeadRows& r, int64_t M, const G4qPagedCache& c, const Lattice& l) {
+    const Lattice::Wide last = (Lattice::Wide)r.token_stride * (M - 1) + (Lattice::Wide)r.head_stride * (r.n_heads - 1);
+    for (const uint16_t* base : {c.k, c.v}) {
+        const Lattice::Wide gap = r.data - base;
+        if (gap >= l.span() || gap + last + l.d <= 0) continue;
+        if (!l.nested()) return true;
+        const int64_t tokens = r.token_stride == 0 ? 1 : M, heads = r.n_heads;
+        for (int64_t t = 0; t < tokens; ++t)
+            for (int64_t h = 0; h < heads; ++h)
+                if (l.meets_row(gap + (Lattice::Wide)t * r.token_stride + (Lattice::Wide)h * r.head_stride)) return true;
+    }
+    return false;
 }
 
 }  // namespace g4q

@@ -347,7 +347,7 @@ G4qStatus g4q_qk_norm_rope(const G4qRope* rope, const G4qHeadRows* q, const G4qH
  * pages, the values beside them (rms_norm without a weight; with G4Q_APPEND_RAW_VALUES as they are). v may be
  * k (full-attention layers, whose key projection is the value too: :820-822), but what is stored of the two differs:
  * caches whose k and v, or pages, heads and slots, share elements are refused (they may be read by g4q_paged_attention).
- * q (with q_out) may be NULL; q_out may be q, else it must not overlap q, k or v. */
+ * q (with q_out) may be NULL; q_out may be q, else it must not overlap q, k or v. None of the four may overlap the cache. */
 #define G4Q_APPEND_RAW_VALUES 0x1u
 G4qStatus g4q_kv_append(const G4qRope* rope, const G4qHeadRows* q, const G4qHeadRows* k, const G4qHeadRows* v, int64_t M,
                         const uint16_t* q_weight, const uint16_t* k_weight, float eps, uint32_t flags,
@@ -355,7 +355,8 @@ G4qStatus g4q_kv_append(const G4qRope* rope, const G4qHeadRows* q, const G4qHead
 
 /* out = softmax(scale * q . k^T) v over the cache, query head h against key head h / (n_q_heads / n_kv_heads);
  * the query at position t sees the keys j <= t, and j > t - window when window > 0. Single tokens, drafted
- * blocks and prompt chunks may be mixed in one call. A row that sees no key is zero. out must not overlap q.
+ * blocks and prompt chunks may be mixed in one call. A row that sees no key is zero. out must not overlap q
+ * or the cache.
  * What the cache holds at slots that no query of a sequence's step sees does not matter (NaN included); a
  * non-finite value that some query of the step sees may reach the step's other queries of that sequence. The
  * handle owns the scratch of partial results: calls on one handle must not overlap on the GPU (one stream, or

@@ -56,3 +56,43 @@ def test_append_refuses_caches_whose_slots_share_elements(cuda):
         assert stored[1].any() and stored[2].any()
         want = want or stored
         assert all(torch.equal(a, b) for a, b in zip(stored, want))
+
+
+def test_rows_in_the_cache_are_refused(cuda):
+    """Inputs and outputs of the append, and the attention's output, that share elements with the pages; between the pages of
+    a buffer that holds both they qualify."""
+    from helios_b200 import attention as A
+    d, page, pages, hk, hq = 64, 16, 3, 2, 4
+    block = hk * page * d
+    flat = bf16(pages * 4 * block, seed=1)
+    shape = pages, hk, page, d
+    kc, vc = (flat.as_strided(shape, (4 * block, page * d, d, 1), i * block) for i in range(2))
+    cache, batch, rope = A.PagedKVCache(kc, vc), one_sequence(2, 20, page), A.Rope(d)
+    q, k, v = bf16(2, hq, d, seed=2), bf16(2, hk, d, seed=3), bf16(2, hk, d, seed=4)
+    attend = A.PagedAttention(hq, hk, d)
+    before = flat.clone()
+
+    def rows(heads, start, token=None):
+        return flat.as_strided((2, heads, d), (token or heads * d, d, 1), start)
+
+    for start in (0, block - hq * d, block, 4 * block + 8, 2 * block - d):       # in k, over its end, in v, later pages
+        for bad in ({"q": rows(hq, start)}, {"k": rows(hk, start)}, {"v": rows(hk, start)}, {"q_out": rows(hq, start)}):
+            args = {"q": q, "k": k, "v": v, **bad}
+            with pytest.raises(ValueError, match="overlaps"):
+                A.kv_append(args["q"], args["k"], args["v"], cache, batch, rope, q_out=args.get("q_out"))
+        with pytest.raises(ValueError, match="out overlaps the cache"):
+            attend(q, cache, batch, out=rows(hq, start))
+    torch.cuda.synchronize()
+    assert torch.equal(flat, before)
+    # tokens of a row each behind a page's values, and heads of queries that are read only anywhere
+    free = rows(hq, 2 * block, 4 * block), rows(hk, 3 * block, 4 * block), rows(hk, 3 * block + hk * d, 4 * block)
+    for to, x in zip(free, (q, k, v)):
+        to.copy_(x)
+    want_cache = A.PagedKVCache(kc.clone(), vc.clone())
+    want = A.kv_append(q, k, v, want_cache, batch, rope)
+    assert torch.equal(A.kv_append(*free, cache, batch, rope, q_out=free[0]), want)
+    assert torch.equal(cache.k, want_cache.k) and torch.equal(cache.v, want_cache.v)
+    want = attend(want, want_cache, batch)
+    assert torch.equal(attend(free[0], cache, batch, out=rows(hq, 2 * block + hq * d, 4 * block)), want)
+    inside = rows(hq, 0)
+    assert torch.equal(attend(inside, cache, batch), attend(inside.clone(), cache, batch))

@@ -13,14 +13,20 @@ D = 8
 PROGRAM = r"""
 #include <cstdio>
 #include "g4q_overlap.h"
-int main() {
+int main(int argc, char**) {
     G4qPagedCache c;
-    long long k, v, n, ps, hs, ss;
+    long long k, v, n, ps, hs, ss, at, m, ts, rs;
+    G4qHeadRows r;
     while (std::scanf("%lld %lld %lld %d %d %lld %lld %lld", &k, &v, &n, &c.page_size, &c.n_kv_heads, &ps, &hs, &ss) == 8) {
         c.k = (uint16_t*)0 + k, c.v = (uint16_t*)0 + v;
         c.n_pages = n, c.head_dim = 8;
         c.page_stride = ps, c.head_stride = hs, c.slot_stride = ss;
         const char* wrong = g4q::shared_slots(c);
+        if (argc > 1) {      // and rows: meets the cache or not
+            if (std::scanf("%lld %lld %d %lld %lld", &at, &m, &r.n_heads, &ts, &rs) != 5) return 1;
+            r.data = (uint16_t*)0 + at, r.token_stride = ts, r.head_stride = rs;
+            wrong = g4q::meets_cache(r, m, c, g4q::cache_lattice(c)) ? "meets" : nullptr;
+        }
         std::printf("%d %s\n", (int)g4q::cache_lattice(c).nested(), wrong ? wrong : "-");
     }
 }
@@ -29,16 +35,17 @@ int main() {
 
 @pytest.fixture(scope="module")
 def answers(tmp_path_factory):
-    """For cases (k, v, pages, page_size, heads, page_stride, head_stride, slot_stride): (nested, what is wrong)."""
+    """For cases (k, v, pages, page_size, heads, page_stride, head_stride, slot_stride): (nested, what is wrong). With rows,
+    the cases go on with (data, tokens, heads, token_stride, head_stride): (nested, "meets" or "-")."""
     at = tmp_path_factory.mktemp("overlap")
     (at / "main.cpp").write_text(PROGRAM)
     subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover", "-I",
                     str(ROOT / "include"), "-I", str(ROOT / "helios_b200" / "csrc"), str(at / "main.cpp"), "-o", str(at / "main")],
                    check=True)
 
-    def ask(cases):
+    def ask(cases, rows=False):
         text = "\n".join(" ".join(map(str, c)) for c in cases)
-        out = subprocess.run([str(at / "main")], input=text, check=True, capture_output=True, text=True).stdout.splitlines()
+        out = subprocess.run([str(at / "main")] + ["rows"] * rows, input=text, check=True, capture_output=True, text=True).stdout.splitlines()
         assert len(out) == len(cases)
         return [(line[0] == "1", line[2:]) for line in out]
 
@@ -100,3 +107,28 @@ def test_one_tensor_for_keys_and_values(answers):
     """The key projection is the value too in some layers, but what is stored of it is not."""
     assert answers([(64, 64, 3, 16, 1, 128, 128, 8), (64, 64 + 8, 3, 16, 1, 128, 128, 8)]) == \
         [(True, "cache: k and v share elements")] * 2
+
+
+def test_rows_against_sets_of_elements(answers):
+    """Rows before, in, between and behind the slots of a cache. Exact where the cache's axes are nested; else nothing that
+    is shared is missed."""
+    rng = random.Random(2)
+    cases = []
+    for _ in range(6000):
+        counts = [rng.choice([1, 2, 3]) for _ in range(3)]
+        strides = [0, 0, 0]
+        inner = D
+        for axis in rng.sample(range(3), 3):
+            strides[axis] = inner + rng.choice([0, 8, 24, 64]) if rng.random() < 0.95 else 8 * rng.randrange(1, 9)
+            inner = max(inner, strides[axis] * counts[axis])
+        k, m, heads = 4096, rng.choice([1, 2, 4]), rng.choice([1, 2])
+        cases.append((k, k + 8 * rng.randrange(-24, 25), counts[0], counts[2], counts[1], strides[0], strides[1], strides[2],
+                      k + 8 * rng.randrange(-40, 80), m, heads, 8 * rng.randrange(0, 9), 8 * rng.randrange(1, 9)))
+    seen = {False: 0, True: 0}
+    for case, (nested, text) in zip(cases, answers(cases, rows=True)):
+        k, v, pages, slots, heads, ps, hs, ss, at, m, row_heads, ts, rs = case
+        held = set(elements(rows(k, (pages, heads, slots), (ps, hs, ss)) + rows(v, (pages, heads, slots), (ps, hs, ss))))
+        meets = bool(held & set(elements(rows(at, (m, row_heads), (ts, rs)))))
+        assert text == ("meets" if meets else "-") if nested else meets <= (text == "meets"), case
+        seen[meets] += nested
+    assert min(seen.values()) > 1000
