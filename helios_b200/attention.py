@@ -117,6 +117,10 @@ class PagedKVCache:
         return cls(torch.zeros(shape, dtype=torch.bfloat16, device=dev), torch.zeros(shape, dtype=torch.bfloat16, device=dev))
 
 
+def _field(name: str) -> property:
+    return property(lambda self: getattr(self, "_" + name), lambda self, value: self._set(**{name: value}))
+
+
 class PagedBatch:
     """The sequences of one step. int32 CUDA tensors, read on the device when the kernels run (a captured
     graph replays with what they hold then; change them in place): ``q_offsets`` [n + 1], sequence b's new
@@ -125,32 +129,47 @@ class PagedBatch:
     at least the longest sequence's new tokens. ``max_kv``: at least the longest kv_len where the caller
     knows it below the table's capacity; the table is then taken to end there.
 
-    Contents that do not fit are refused on the device without touching other memory, and reported by
+    The five may be assigned later too (a wider table, a larger ``max_q``): from the next call on that holds; a
+    captured graph stays with what it captured, tensors that have to live as long. Another number of sequences is
+    another batch. Contents that do not fit are refused on the device without touching other memory, and reported by
     ``_lib.device_error()`` as ERR_PAGE, ERR_TABLE or ERR_LENS."""
+
+    _FIELDS = ("q_offsets", "kv_lens", "block_table", "max_q", "max_kv")
+    q_offsets, kv_lens, block_table, max_q, max_kv = map(_field, _FIELDS)
 
     def __init__(self, q_offsets: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor, *, max_q: int,
                  max_kv: Optional[int] = None):
-        self.q_offsets = _int32(q_offsets, 1, "q_offsets")
-        self.kv_lens = _int32(kv_lens, 1, "kv_lens")
-        self.block_table = _int32(block_table, 2, "block_table")
+        self._set(q_offsets=q_offsets, kv_lens=kv_lens, block_table=block_table, max_q=max_q, max_kv=max_kv)
+
+    def _set(self, **fields) -> None:
+        """Take the fields if they fit together with the others; the views for the kernels are made anew."""
+        f = {**{n: getattr(self, "_" + n, None) for n in self._FIELDS}, **fields}
+        q_offsets, kv_lens = _int32(f["q_offsets"], 1, "q_offsets"), _int32(f["kv_lens"], 1, "kv_lens")
+        block_table, max_q, max_kv = _int32(f["block_table"], 2, "block_table"), f["max_q"], f["max_kv"]
         n = kv_lens.shape[0]
         if n < 1 or q_offsets.shape[0] != n + 1 or block_table.shape[0] != n:
             raise ValueError(f"q_offsets must hold {n + 1} and block_table {n} rows for {n} sequences (at least one)")
-        self.device = kv_lens.get_device()
-        if q_offsets.get_device() != self.device or block_table.get_device() != self.device:
+        device = kv_lens.get_device()
+        if q_offsets.get_device() != device or block_table.get_device() != device:
             raise ValueError("q_offsets, kv_lens and block_table must be on one device")
         if not 1 <= max_q < 2 ** 31 or (max_kv is not None and max_kv < 1):
             raise ValueError("max_q and max_kv must be >= 1 (and max_q below 2^31)")
-        self.max_q, self.max_kv = max_q, max_kv
+        self.device = device
+        for name in self._FIELDS:
+            setattr(self, "_" + name, f[name])
         self._views = {}
 
     def view(self, page_size: int) -> int:
-        """Address of the C view for a cache of this page size."""
+        """Address of the C view for a cache of this page size; valid until a field is assigned."""
+        return self._held(page_size)[0]
+
+    def _held(self, page_size: int) -> Tuple[int, _lib.G4qPagedBatch]:
+        """The C view's address, and the view, which a call keeps while it runs."""
         v = self._views.get(page_size)
         if v is None:
             c = self._view(page_size)
             v = self._views[page_size] = (ctypes.addressof(c), c)
-        return v[0]
+        return v
 
     def _view(self, page_size: int) -> _lib.G4qPagedBatch:
         t = self.block_table
@@ -185,8 +204,9 @@ def kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cache
     belong to no sequence are left as they were (in ``q_out`` too). No tensor may overlap the cache."""
     dev = rope.device
     _same_device(dev, cache, batch)
+    view = batch._held(cache.page_size)
     return rope._ops.kv_append(rope.handle.value, rope.head_dim, dev, _raw_stream(dev), q, k, v, cache.c_addr,
-                               batch.view(cache.page_size), q_weight, k_weight, eps,
+                               view[0], q_weight, k_weight, eps,
                                0 if norm_values else _lib.APPEND_RAW_VALUES, q_out)
 
 
@@ -218,8 +238,9 @@ class PagedAttention:
         q or the cache)."""
         dev = self.device
         _same_device(dev, cache, batch)
+        view = batch._held(cache.page_size)
         return self._ops.paged_attention(self.handle.value, self.head_dim, dev, _raw_stream(dev), q, cache.c_addr,
-                                         batch.view(cache.page_size), self.head_dim ** -0.5 if scale is None else scale, window,
+                                         view[0], self.head_dim ** -0.5 if scale is None else scale, window,
                                          out)
 
     def free(self) -> None:

@@ -96,3 +96,16 @@ def test_rows_in_the_cache_are_refused(cuda):
     assert torch.equal(attend(free[0], cache, batch, out=rows(hq, 2 * block + hq * d, 4 * block)), want)
     inside = rows(hq, 0)
     assert torch.equal(attend(inside, cache, batch), attend(inside.clone(), cache, batch))
+
+
+def test_fields_assigned_after_the_first_call(cuda):
+    """A batch whose max_q and table grow between two steps."""
+    from helios_b200 import _lib
+    from helios_b200 import attention as A
+    cache = A.PagedKVCache(bf16(8, 2, 16, 64, seed=1), bf16(8, 2, 16, 64, seed=2))
+    attend, q = A.PagedAttention(4, 2, 64), bf16(5, 4, 64, seed=3)
+    batch = one_sequence(1, 16, 16)
+    attend(q[:1], cache, batch)
+    batch.q_offsets, batch.kv_lens, batch.block_table, batch.max_q = int32([0, 5]), int32([100]), int32([list(range(7))]), 5
+    assert torch.equal(attend(q, cache, batch), attend(q, cache, one_sequence(5, 100, 16)))
+    assert _lib.device_error() == 0
