@@ -87,10 +87,10 @@ class Rope:
 
 class PagedKVCache:
     """One layer's keys and values in pages: ``k`` and ``v`` bf16 [pages, kv_heads, page_size, head_dim]
-    CUDA tensors of equal strides (page_size a power of two, 16 or more). Any stride order qualifies while
-    head_dim is contiguous, so ``t.transpose(1, 2)`` of a [pages, page_size, kv_heads, head_dim] tensor does,
-    and so does one layer's slice of a tensor that holds them all. The tensors stay the caller's. Elements that ``k``
-    and ``v``, or two of a tensor's slots, share can be read; :func:`kv_append` refuses them."""
+    CUDA tensors of equal strides (page_size a power of two, 16 or more). Any stride order qualifies while head_dim is
+    contiguous, so ``t.transpose(1, 2)`` of a [pages, page_size, kv_heads, head_dim] tensor does, and so does one
+    layer's slice of a tensor that holds them all. The tensors stay the caller's; other ones are another cache.
+    Elements that ``k`` and ``v``, or two of a tensor's slots, share can be read; :func:`kv_append` refuses them."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
         for t, name in ((k, "k"), (v, "v")):
@@ -108,6 +108,11 @@ class PagedKVCache:
         self.c = _lib.G4qPagedCache(k.data_ptr(), v.data_ptr(), self.n_pages, self.page_size, self.n_kv_heads, d,
                                     max(sp, d) if self.n_pages == 1 else sp, max(sh, d) if self.n_kv_heads == 1 else sh, ss)
         self.c_addr = ctypes.addressof(self.c)
+
+    def __setattr__(self, name, value):
+        if "c_addr" in self.__dict__ and name in self.__dict__:    # the structure for the kernels would not follow
+            raise AttributeError(f"a PagedKVCache stays as it was made ({name} assigned): make another one")
+        super().__setattr__(name, value)
 
     @classmethod
     def allocate(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int) -> "PagedKVCache":

@@ -55,3 +55,19 @@ def test_a_call_keeps_the_view_that_it_was_given(batch):
     address, view = batch._held(16)
     batch.max_q = 11
     assert _lib.G4qPagedBatch.from_address(address).max_q == 4 and view.max_q == 4 and held(batch).max_q == 11
+
+
+class Lent(torch.Tensor):
+    """A CPU tensor that passes for a CUDA one, for the addresses and strides."""
+    is_cuda = True
+
+
+def test_a_cache_stays_as_it_was_made():
+    k, v, other = (torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16).as_subclass(Lent) for _ in range(3))
+    cache = A.PagedKVCache(k, v)
+    for name, value in (("k", other), ("v", other), ("page_size", 32), ("n_pages", 8), ("c", None)):
+        with pytest.raises(AttributeError, match="make another one"):
+            setattr(cache, name, value)
+    cache.layer = 3          # a caller's own
+    assert cache.k is k and cache.v is v and (cache.page_size, cache.n_pages) == (16, 4)
+    assert _lib.G4qPagedCache.from_address(cache.c_addr).k == k.data_ptr()
