@@ -1,5 +1,5 @@
-"""Builds libg4q.so (the C-ABI kernel library) in-tree with nvcc for sm_100a, and _g4q_torch.so (the Python
-side of the attention calls, a CPython module over torch's headers) with the host compiler.
+"""Builds libg4q.so (the C-ABI kernel library) in-tree with nvcc for sm_100a, and, where torch can be imported,
+_g4q_torch.so (the Python side of the attention calls, a CPython module over torch's headers) with the host compiler.
 
 ``python -m helios_b200.build`` or ``helios_b200.build.build()``. The shared library lands
 next to this file so it travels with the source tree; no JIT cache is involved.
@@ -46,11 +46,10 @@ def _stale(target: Path, deps) -> bool:
     return any(Path(d).stat().st_mtime > t for d in deps)
 
 
-def _torch_command() -> list:
+def _torch_command(torch) -> list:
     """The host compiler's command for _g4q_torch.so."""
     import sysconfig
 
-    import torch
     root = Path(torch.__file__).resolve().parent
     inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"],
            INCLUDE]
@@ -60,7 +59,8 @@ def _torch_command() -> list:
 
 
 def build(verbose: bool = False, force: bool = False) -> Path:
-    """Compile every .cu under csrc/ for sm_100a, link libg4q.so and build _g4q_torch.so. Returns libg4q.so's path."""
+    """Compile every .cu under csrc/ for sm_100a and link libg4q.so, whose path is returned; build _g4q_torch.so beside it
+    where torch can be imported (the C ABI needs none of it)."""
     OBJDIR.mkdir(exist_ok=True)
     nvcc = _nvcc()
     common_deps = [CSRC / h for h in HEADERS] + [INCLUDE / "g4q.h"]
@@ -70,8 +70,13 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         objs.append(obj)
         if force or _stale(obj, [CSRC / src] + common_deps):
             cmds.append([nvcc, *NVCC_FLAGS, "-I", str(INCLUDE), "-I", str(CSRC), "-c", str(CSRC / src), "-o", str(obj)])
+    module_cmd = None
     if force or _stale(TORCH_LIB, [TORCH_SRC, INCLUDE / "g4q.h"]):
-        cmds.append(_torch_command())
+        try:
+            import torch
+            module_cmd = _torch_command(torch)
+        except ImportError as e:
+            print(f"{TORCH_LIB.name} is not built, torch cannot be imported: {e}", file=sys.stderr, flush=True)
     # translation units compile independently: one nvcc per source, a few at a time
     from concurrent.futures import ThreadPoolExecutor
 
@@ -81,13 +86,13 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         subprocess.run(cmd, check=True)
 
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+        module = ex.submit(compile_one, module_cmd) if module_cmd else None
         list(ex.map(compile_one, cmds))
-    if force or _stale(LIB, objs):
-        cmd = [nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", str(LIB), *map(str, objs),
-               "-lcudart", "-Xlinker", "-z,defs"]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        subprocess.run(cmd, check=True)
+        if force or _stale(LIB, objs):
+            compile_one([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", str(LIB), *map(str, objs),
+                         "-lcudart", "-Xlinker", "-z,defs"])
+        if module is not None:
+            module.result()      # the library is complete, whatever became of the module
     return LIB
 
 
