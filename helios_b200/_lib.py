@@ -6,6 +6,8 @@ raises ``G4qUnavailable`` instead of computing anything another way.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
+import sysconfig
 import threading
 from pathlib import Path
 
@@ -217,15 +219,24 @@ def raise_status(status: int, name: str) -> None:
 _torch_ops = None
 
 
+def torch_module_path(torch_version: str) -> Path:
+    """Where the CPython module of the attention calls lies. It is bound to the C++ ABI of one torch and to one Python,
+    so its name has both, and what another one's build left is not loaded."""
+    return PKG / f"_g4q_torch-{torch_version}{sysconfig.get_config_var('EXT_SUFFIX')}"
+
+
 def torch_ops():
-    """The CPython module of the attention calls (_g4q_torch.so), bound to the loaded libg4q.so."""
+    """The CPython module of the attention calls (_g4q_torch), bound to the loaded libg4q.so."""
     global _torch_ops
     if _torch_ops is None:
-        lib = load()
+        import torch
+        lib, path = load(), torch_module_path(torch.__version__)
         try:
-            from . import _g4q_torch as ops
+            spec = importlib.util.spec_from_file_location(f"{__package__}._g4q_torch", path)
+            ops = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(ops)
         except ImportError as e:
-            raise G4qUnavailable(f"_g4q_torch.so is missing or cannot load ({e}): build it with "
+            raise G4qUnavailable(f"{path.name} is missing or cannot load ({e}): build it with "
                                  "`python -m helios_b200.build`") from e
         entry = [ctypes.cast(getattr(lib, n), ctypes.c_void_p).value
                  for n in ("g4q_qk_norm_rope", "g4q_kv_append", "g4q_paged_attention")]

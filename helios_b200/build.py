@@ -1,5 +1,5 @@
 """Builds libg4q.so (the C-ABI kernel library) in-tree with nvcc for sm_100a, and, where torch can be imported,
-_g4q_torch.so (the Python side of the attention calls, a CPython module over torch's headers) with the host compiler.
+_g4q_torch (the Python side of the attention calls, a CPython module over torch's headers) with the host compiler.
 
 ``python -m helios_b200.build`` or ``helios_b200.build.build()``. The shared library lands
 next to this file so it travels with the source tree; no JIT cache is involved.
@@ -11,13 +11,14 @@ import subprocess
 import sys
 from pathlib import Path
 
+from . import _lib
+
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libg4q.so"
 TORCH_SRC = CSRC / "g4q_torch.cpp"
-TORCH_LIB = PKG / "_g4q_torch.so"
 OBJDIR = PKG / "_build"
 
 SOURCES = ["g4q_api.cu", "g4q_layout.cu", "g4q_gemv.cu", "g4q_gemv2.cu", "g4q_gemm.cu", "g4q_decode.cu",
@@ -46,8 +47,8 @@ def _stale(target: Path, deps) -> bool:
     return any(Path(d).stat().st_mtime > t for d in deps)
 
 
-def _torch_command(torch) -> list:
-    """The host compiler's command for _g4q_torch.so."""
+def _torch_command(torch, target: Path) -> list:
+    """The host compiler's command for _g4q_torch."""
     import sysconfig
 
     root = Path(torch.__file__).resolve().parent
@@ -55,11 +56,11 @@ def _torch_command(torch) -> list:
            INCLUDE]
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{i}" for i in inc), str(TORCH_SRC),
-            "-o", str(TORCH_LIB), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+            "-o", str(target), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
 
 
 def build(verbose: bool = False, force: bool = False) -> Path:
-    """Compile every .cu under csrc/ for sm_100a and link libg4q.so, whose path is returned; build _g4q_torch.so beside it
+    """Compile every .cu under csrc/ for sm_100a and link libg4q.so, whose path is returned; build _g4q_torch beside it
     where torch can be imported (the C ABI needs none of it)."""
     OBJDIR.mkdir(exist_ok=True)
     nvcc = _nvcc()
@@ -71,12 +72,13 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         if force or _stale(obj, [CSRC / src] + common_deps):
             cmds.append([nvcc, *NVCC_FLAGS, "-I", str(INCLUDE), "-I", str(CSRC), "-c", str(CSRC / src), "-o", str(obj)])
     module_cmd = None
-    if force or _stale(TORCH_LIB, [TORCH_SRC, INCLUDE / "g4q.h"]):
-        try:
-            import torch
-            module_cmd = _torch_command(torch)
-        except ImportError as e:
-            print(f"{TORCH_LIB.name} is not built, torch cannot be imported: {e}", file=sys.stderr, flush=True)
+    try:
+        import torch
+        target = _lib.torch_module_path(torch.__version__)
+        if force or _stale(target, [TORCH_SRC, INCLUDE / "g4q.h"]):
+            module_cmd = _torch_command(torch, target)
+    except ImportError as e:
+        print(f"_g4q_torch is not built, torch cannot be imported: {e}", file=sys.stderr, flush=True)
     # translation units compile independently: one nvcc per source, a few at a time
     from concurrent.futures import ThreadPoolExecutor
 

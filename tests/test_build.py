@@ -43,3 +43,23 @@ def test_the_library_is_linked_before_a_module_that_fails_is_reported(ran, monke
 def test_the_module_is_built_where_torch_is(ran):
     B.build(force=True)
     assert len(module_commands(ran)) == 1
+
+
+def test_another_torch_has_a_module_of_its_own(ran, monkeypatch):
+    """The module is bound to the ABI of one torch and one Python: after an upgrade it is neither loaded nor up to date."""
+    import sysconfig
+
+    import torch
+
+    from helios_b200 import _lib
+    B.build()
+    path = _lib.torch_module_path(torch.__version__)
+    assert not module_commands(ran) and path.exists() and _lib.torch_ops()       # this one's is there
+    assert path.name.endswith(sysconfig.get_config_var("EXT_SUFFIX"))
+    monkeypatch.setattr(torch, "__version__", "99.1")
+    monkeypatch.setattr(_lib, "_torch_ops", None)
+    with pytest.raises(_lib.G4qUnavailable, match="99.1.*helios_b200.build"):
+        _lib.torch_ops()
+    B.build()
+    (cmd,) = module_commands(ran)
+    assert cmd[cmd.index("-o") + 1] == str(_lib.torch_module_path("99.1")) != str(path)
