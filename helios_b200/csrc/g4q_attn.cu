@@ -821,8 +821,8 @@ CUtensorMap paged_map(const AttnCall& a, const uint16_t* base, int D, int box) {
 CUtensorMap rows_map(const uint16_t* base, int64_t token_stride, int64_t head_stride, int heads, int rows, int D, int box_heads,
                      int box_tokens) {
     const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows};
-    // the stride of a single head is never used, but has to be a legal one
-    const cuuint64_t strides[2] = {(cuuint64_t)(heads == 1 ? D : head_stride) * 2, (cuuint64_t)token_stride * 2};
+    // the stride of a single head, or of a single token, is never used, but has to be a legal one (16 bytes to 2^40)
+    const cuuint64_t strides[2] = {(cuuint64_t)(heads == 1 ? D : head_stride) * 2, (cuuint64_t)(rows == 1 ? D : token_stride) * 2};
     const cuuint32_t shape[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
     return bf16_map(3, base, dims, strides, shape);
 }

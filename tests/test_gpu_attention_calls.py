@@ -109,3 +109,15 @@ def test_fields_assigned_after_the_first_call(cuda):
     batch.q_offsets, batch.kv_lens, batch.block_table, batch.max_q = int32([0, 5]), int32([100]), int32([list(range(7))]), 5
     assert torch.equal(attend(q, cache, batch), attend(q, cache, one_sequence(5, 100, 16)))
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("hq,hk,d", [(40, 1, 512), (64, 1, 512), (16, 1, 512), (16, 8, 256)])
+def test_the_stride_of_a_single_token_is_not_used(cuda, hq, hk, d):
+    """More than 32 query heads a key head at head_dim 512 take the chunk kernel with one token too."""
+    from helios_b200 import attention as A
+    cache = A.PagedKVCache(bf16(5, hk, 16, d, seed=1), bf16(5, hk, 16, d, seed=2))
+    batch, attend = one_sequence(1, 70, 16), A.PagedAttention(hq, hk, d)
+    q = bf16(1, hq, d, seed=3)
+    want = attend(q, cache, batch)
+    for stride in (0, 8, 2 ** 41):
+        assert torch.equal(attend(q.as_strided((1, hq, d), (stride, d, 1)), cache, batch), want)
