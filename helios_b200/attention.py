@@ -31,7 +31,7 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _int32(t: torch.Tensor, dims: int, name: str) -> torch.Tensor:
-    if t.dtype is not torch.int32 or not t.is_cuda or t.dim() != dims or (t.numel() and t.stride(-1) != 1):
+    if t.dtype is not torch.int32 or not t.is_cuda or t.dim() != dims or (t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1):
         raise ValueError(f"{name} must be a {dims}-D int32 CUDA tensor with contiguous rows")
     return t
 

@@ -71,3 +71,18 @@ def test_a_cache_stays_as_it_was_made():
     cache.layer = 3          # a caller's own
     assert cache.k is k and cache.v is v and (cache.page_size, cache.n_pages) == (16, 4)
     assert _lib.G4qPagedCache.from_address(cache.c_addr).k == k.data_ptr()
+
+
+def test_the_stride_of_a_single_entry_is_not_used():
+    """The length of one sequence out of a column, a table of one page out of a wider one."""
+    def lent(*shape):
+        return torch.zeros(*shape, dtype=torch.int32).as_subclass(Lent)
+
+    off, column, wide = lent(2), lent(5, 3), lent(1, 12)
+    batch = A.PagedBatch(off, column[2:3, 1], wide[:, ::12], max_q=1)
+    c = held(batch)
+    assert c.kv_lens == column.data_ptr() + 7 * 4 and (c.block_table, c.max_pages) == (wide.data_ptr(), 1)
+    assert c.table_stride >= c.max_pages
+    for bad in ((lent(4)[::2], column[2:3, 1], wide), (off, column[:, 1], lent(5, 3)), (off, column[2:3, 1], wide[:, ::2])):
+        with pytest.raises(ValueError, match="contiguous rows"):
+            A.PagedBatch(*bad, max_q=1)
