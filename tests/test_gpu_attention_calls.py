@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from test_gpu_attention import Step, no_device_error, randn
+
 pytestmark = pytest.mark.gpu
 
 
@@ -121,3 +123,26 @@ def test_the_stride_of_a_single_token_is_not_used(cuda, hq, hk, d):
     want = attend(q, cache, batch)
     for stride in (0, 8, 2 ** 41):
         assert torch.equal(attend(q.as_strided((1, hq, d), (stride, d, 1)), cache, batch), want)
+
+
+def test_two_handles_on_two_streams(cuda):
+    """Calls of one token, drafted blocks and chunks of two layers' layouts, each on a stream of its own."""
+    from helios_b200 import attention as A
+    work = []
+    for hq, hk, d, seed in ((16, 8, 256, 41), (16, 1, 512, 43)):
+        attend = A.PagedAttention(hq, hk, d)
+        for q_lens, kv_lens in (([1], [900]), ([8, 8], [300, 2000]), ([200, 1], [900, 400]), ([700], [1500])):
+            s = Step(q_lens, kv_lens, hk, d, 32, seed)
+            q = randn(s.rows, hq, d, seed=seed + 1)
+            work.append((attend, q, s, attend(q, s.cache, s.batch)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(10):
+        for i in range(4):
+            for stream, (attend, q, s, want) in zip(streams, (work[i], work[4 + (i + 1) % 4])):
+                with torch.cuda.stream(stream):
+                    got.append((attend(q, s.cache, s.batch), want))
+    torch.cuda.synchronize()
+    no_device_error()
+    assert all(torch.equal(a, b) for a, b in got)
