@@ -1030,11 +1030,17 @@ static bool heads_overlap(const G4qHeadRows& a, const G4qHeadRows& b, int64_t M,
     return rows_meet(r) || rows_meet(r - x.outer);
 }
 
+// An output, each of whose rows some warp writes in its own time.
+static void check_apart(const G4qHeadRows* out, int64_t M, int64_t d, const char* name) {
+    if (!rows_apart(*out, M, d)) throw Error(G4Q_ERR_INVALID_ARGUMENT, std::string(name) + ": its rows overlap");
+}
+
 // An output of the head norms: the input that its rows come from, or memory that no other rows are in.
 static void check_output(const G4qHeadRows* out, const G4qHeadRows* own, std::initializer_list<const G4qHeadRows*> others,
                          int64_t M, int64_t d, const char* name) {
     const bool in_place = out->data == own->data && (M == 1 || out->token_stride == own->token_stride) &&
                           (out->n_heads == 1 || out->head_stride == own->head_stride);
+    check_apart(out, M, d, name);
     bool bad = !in_place && heads_overlap(*out, *own, M, d);
     for (const G4qHeadRows* t : others) bad = bad || (t != nullptr && heads_overlap(*out, *t, M, d));
     if (bad) throw Error(G4Q_ERR_INVALID_ARGUMENT, std::string(name) + " overlaps other rows of the call");
@@ -1301,6 +1307,7 @@ G4qStatus g4q_paged_attention(const G4qAttn* attn, const G4qHeadRows* q, int64_t
         require(M == 1 || q->token_stride >= a->head_dim, G4Q_ERR_INVALID_ARGUMENT, "q.token_stride must be >= head_dim");
         // several CTAs read a query row, and one may write its result before another has read it
         require(!heads_overlap(*out, *q, M, a->head_dim), G4Q_ERR_INVALID_ARGUMENT, "out must not be q, nor overlap it");
+        check_apart(out, M, a->head_dim, "out");
         check_outside(out, M, *cache, cache_lattice(*cache), "out");
         AttnCall c = {};
         c.q = q->data, c.q_t = q->token_stride, c.q_h = q->head_stride;

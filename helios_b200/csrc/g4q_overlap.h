@@ -76,6 +76,30 @@ private:
     }
 };
 
+// M tokens of head rows.
+inline Lattice rows_lattice(const G4qHeadRows& r, int64_t M, int64_t d) {
+    Lattice l;
+    l.d = d;
+    l.add(r.token_stride, M);
+    l.add(r.head_stride, r.n_heads);
+    return l;
+}
+
+// Whether no two of the rows share an element. Tokens and heads that interleave without sharing one qualify: of the steps
+// of the longer stride only those within the other axis' reach matter, which are no more than it has rows.
+inline bool rows_apart(const G4qHeadRows& r, int64_t M, int64_t d) {
+    const Lattice l = rows_lattice(r, M, d);
+    if (l.nested()) return true;
+    if (l.stride[l.axes - 1] < d) return false;
+    const int64_t s = l.stride[1];                   // two axes, or the last would have been nested
+    for (int64_t i = 1; i < l.count[0] && (Lattice::Wide)i * l.stride[0] < l.span(1); ++i) {
+        const int64_t rest = (int64_t)((Lattice::Wide)i * l.stride[0] % s);
+        const bool next = (Lattice::Wide)i * l.stride[0] - rest < (Lattice::Wide)s * (l.count[1] - 1);
+        if (rest < d || (next && s - rest < d)) return false;
+    }
+    return true;
+}
+
 // The slots of a cache's k (or v), one row a head.
 inline Lattice cache_lattice(const G4qPagedCache& c) {
     Lattice l;

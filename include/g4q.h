@@ -283,7 +283,8 @@ G4qStatus g4q_rms_norm_residual(const uint16_t* x, int64_t ldx, const uint16_t* 
  * sliding-window mask. head_dim is 64, 128, 256 or 512; activations and cache are bf16.
  *
  * Head rows: M tokens of n_heads heads of head_dim elements, element strides per token and per head
- * (multiples of 8, data 16-byte aligned; [M, heads, head_dim] views of a q|k|v matmul's output qualify). */
+ * (multiples of 8, data 16-byte aligned; [M, heads, head_dim] views of a q|k|v matmul's output qualify). The rows of
+ * an output must not overlap one another. */
 typedef struct G4qHeadRows {
     uint16_t* data;
     int64_t token_stride;

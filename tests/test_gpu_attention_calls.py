@@ -100,6 +100,34 @@ def test_rows_in_the_cache_are_refused(cuda):
     assert torch.equal(attend(inside, cache, batch), attend(inside.clone(), cache, batch))
 
 
+def test_outputs_whose_rows_overlap_are_refused(cuda):
+    """A token's second head in the place of the next token's first one: two warps would write the row."""
+    from helios_b200 import attention as A
+    d, hq, hk = 64, 4, 2
+    cache = A.PagedKVCache(bf16(3, hk, 16, d, seed=1), bf16(3, hk, 16, d, seed=2))
+    batch, rope, attend = one_sequence(3, 40, 16), A.Rope(d), A.PagedAttention(hq, hk, d)
+    q, k, v = bf16(3, hq, d, seed=3), bf16(3, hk, d, seed=4), bf16(3, hk, d, seed=5)
+    pos = int32([0, 1, 2])
+    buf = torch.zeros(64 * d, dtype=torch.bfloat16, device="cuda")
+    before = cache.k.clone()
+
+    def rows(heads, token, head):
+        return buf.as_strided((3, heads, d), (token, head, 1), 0)
+
+    for token, head in ((d, d), (2 * d, d), (d, 2 * d), (3 * d, d + 8)):
+        for call in (lambda: attend(q, cache, batch, out=rows(hq, token, head)),
+                     lambda: A.kv_append(q, k, v, cache, batch, rope, q_out=rows(hq, token, head)),
+                     lambda: A.qk_norm_rope(q, k, pos, rope, q_out=rows(hq, token, head)),
+                     lambda: A.qk_norm_rope(k, q, pos, rope, k_out=rows(hq, token, head))):
+            with pytest.raises(ValueError, match="its rows overlap"):
+                call()
+    torch.cuda.synchronize()
+    assert torch.equal(cache.k, before) and not buf.any()
+    want = attend(q, cache, batch)
+    for token, head in ((hq * d, d), (d, 3 * d), (d, 3 * d + 8), (2 * d, 7 * d)):     # rows of tokens, of heads
+        assert torch.equal(attend(q, cache, batch, out=rows(hq, token, head)), want)
+
+
 def test_fields_assigned_after_the_first_call(cuda):
     """A batch whose max_q and table grow between two steps."""
     from helios_b200 import _lib

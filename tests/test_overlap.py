@@ -12,17 +12,23 @@ D = 8
 
 PROGRAM = r"""
 #include <cstdio>
+#include <string>
 #include "g4q_overlap.h"
-int main(int argc, char**) {
+int main(int argc, char** argv) {
     G4qPagedCache c;
     long long k, v, n, ps, hs, ss, at, m, ts, rs;
     G4qHeadRows r;
+    const std::string mode = argc > 1 ? argv[1] : "";
+    while (mode == "apart" && std::scanf("%lld %d %lld %lld", &m, &r.n_heads, &ts, &rs) == 4) {
+        r.token_stride = ts, r.head_stride = rs;
+        std::printf("%d\n", (int)g4q::rows_apart(r, m, 8));
+    }
     while (std::scanf("%lld %lld %lld %d %d %lld %lld %lld", &k, &v, &n, &c.page_size, &c.n_kv_heads, &ps, &hs, &ss) == 8) {
         c.k = (uint16_t*)0 + k, c.v = (uint16_t*)0 + v;
         c.n_pages = n, c.head_dim = 8;
         c.page_stride = ps, c.head_stride = hs, c.slot_stride = ss;
         const char* wrong = g4q::shared_slots(c);
-        if (argc > 1) {      // and rows: meets the cache or not
+        if (mode == "rows") {      // and rows: meets the cache or not
             if (std::scanf("%lld %lld %d %lld %lld", &at, &m, &r.n_heads, &ts, &rs) != 5) return 1;
             r.data = (uint16_t*)0 + at, r.token_stride = ts, r.head_stride = rs;
             wrong = g4q::meets_cache(r, m, c, g4q::cache_lattice(c)) ? "meets" : nullptr;
@@ -35,17 +41,18 @@ int main(int argc, char**) {
 
 @pytest.fixture(scope="module")
 def answers(tmp_path_factory):
-    """For cases (k, v, pages, page_size, heads, page_stride, head_stride, slot_stride): (nested, what is wrong). With rows,
-    the cases go on with (data, tokens, heads, token_stride, head_stride): (nested, "meets" or "-")."""
+    """Runs the program on cases, numbers each: (k, v, pages, page_size, heads, page_stride, head_stride, slot_stride) gives
+    (nested, what is wrong). Mode "rows": the cases go on with (data, tokens, heads, token_stride, head_stride), and give
+    (nested, "meets" or "-"). Mode "apart": (tokens, heads, token_stride, head_stride) gives (apart, "")."""
     at = tmp_path_factory.mktemp("overlap")
     (at / "main.cpp").write_text(PROGRAM)
     subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover", "-I",
                     str(ROOT / "include"), "-I", str(ROOT / "helios_b200" / "csrc"), str(at / "main.cpp"), "-o", str(at / "main")],
                    check=True)
 
-    def ask(cases, rows=False):
+    def ask(cases, mode=""):
         text = "\n".join(" ".join(map(str, c)) for c in cases)
-        out = subprocess.run([str(at / "main")] + ["rows"] * rows, input=text, check=True, capture_output=True, text=True).stdout.splitlines()
+        out = subprocess.run([str(at / "main"), mode], input=text, check=True, capture_output=True, text=True).stdout.splitlines()
         assert len(out) == len(cases)
         return [(line[0] == "1", line[2:]) for line in out]
 
@@ -125,10 +132,22 @@ def test_rows_against_sets_of_elements(answers):
         cases.append((k, k + 8 * rng.randrange(-24, 25), counts[0], counts[2], counts[1], strides[0], strides[1], strides[2],
                       k + 8 * rng.randrange(-40, 80), m, heads, 8 * rng.randrange(0, 9), 8 * rng.randrange(1, 9)))
     seen = {False: 0, True: 0}
-    for case, (nested, text) in zip(cases, answers(cases, rows=True)):
+    for case, (nested, text) in zip(cases, answers(cases, "rows")):
         k, v, pages, slots, heads, ps, hs, ss, at, m, row_heads, ts, rs = case
         held = set(elements(rows(k, (pages, heads, slots), (ps, hs, ss)) + rows(v, (pages, heads, slots), (ps, hs, ss))))
         meets = bool(held & set(elements(rows(at, (m, row_heads), (ts, rs)))))
         assert text == ("meets" if meets else "-") if nested else meets <= (text == "meets"), case
         seen[meets] += nested
     assert min(seen.values()) > 1000
+
+
+def test_rows_of_an_output_against_sets_of_elements(answers):
+    rng = random.Random(3)
+    cases = [(rng.randrange(1, 6), rng.randrange(1, 6), 8 * rng.randrange(0, 9), 8 * rng.randrange(0, 9)) for _ in range(5000)]
+    for (m, heads, ts, hs), (apart, _) in zip(cases, answers(cases, "apart")):
+        held = elements(rows(0, (m, heads), (ts, hs)))
+        assert apart == (len(set(held)) == len(held)), (m, heads, ts, hs)
+    many = 2 ** 20          # the fourth: heads 24 = 16 + 8 on lie in the gaps between the tokens' rows
+    assert [a for a, _ in answers([(many, 16, 128, 8), (many, 16, 8, 8 * many), (many, 16, 8, 8), (many, 2, 16, 8 * 3),
+                                   (many, 1, 0, 0), (1, 16, 0, 8), (many, many, 2 ** 40, 2 ** 41)], "apart")] == \
+        [True, True, False, True, False, True, False]
