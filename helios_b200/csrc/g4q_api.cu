@@ -1000,36 +1000,6 @@ static void check_heads(const G4qHeadRows* t, int64_t head_dim, const char* name
     if (wrong != nullptr) throw Error(G4Q_ERR_INVALID_ARGUMENT, std::string(name) + wrong);
 }
 
-// Whether two tensors of head rows share elements. Exact where their strides are alike (views of one buffer); else two
-// tensors whose spans overlap are taken to share some.
-static bool heads_overlap(const G4qHeadRows& a, const G4qHeadRows& b, int64_t M, int64_t d) {
-    struct Axes {
-        int64_t outer, inner, span, inner_span;      // strides of the two axes, and extents in elements
-    };
-    auto axes = [&](const G4qHeadRows& t) {
-        const int64_t ts = M > 1 ? t.token_stride : 0, hs = t.n_heads > 1 ? t.head_stride : 0;
-        const bool tokens_out = ts >= hs;
-        Axes x;
-        x.outer = std::max(ts, hs), x.inner = std::min(ts, hs);
-        x.inner_span = x.inner * ((tokens_out ? t.n_heads : M) - 1) + d;
-        x.span = x.outer * ((tokens_out ? M : t.n_heads) - 1) + x.inner_span;
-        return x;
-    };
-    const Axes x = axes(a), y = axes(b);
-    const int64_t gap = b.data - a.data;             // both are 16-byte aligned
-    if (gap >= x.span || -gap >= y.span) return false;
-    if (x.outer != y.outer || x.outer < std::max(x.inner_span, y.inner_span)) return true;
-    auto rows_meet = [&](int64_t g) {                // one row of each, b's g elements on
-        if (g >= x.inner_span || -g >= y.inner_span) return false;
-        if (x.inner != y.inner || x.inner < d) return true;
-        const int64_t r = ((g % x.inner) + x.inner) % x.inner;
-        return r < d || x.inner - r < d;
-    };
-    if (x.outer == 0) return rows_meet(gap);
-    const int64_t r = ((gap % x.outer) + x.outer) % x.outer;
-    return rows_meet(r) || rows_meet(r - x.outer);
-}
-
 // An output, each of whose rows some warp writes in its own time.
 static void check_apart(const G4qHeadRows* out, int64_t M, int64_t d, const char* name) {
     if (!rows_apart(*out, M, d)) throw Error(G4Q_ERR_INVALID_ARGUMENT, std::string(name) + ": its rows overlap");
@@ -1041,8 +1011,8 @@ static void check_output(const G4qHeadRows* out, const G4qHeadRows* own, std::in
     const bool in_place = out->data == own->data && (M == 1 || out->token_stride == own->token_stride) &&
                           (out->n_heads == 1 || out->head_stride == own->head_stride);
     check_apart(out, M, d, name);
-    bool bad = !in_place && heads_overlap(*out, *own, M, d);
-    for (const G4qHeadRows* t : others) bad = bad || (t != nullptr && heads_overlap(*out, *t, M, d));
+    bool bad = !in_place && rows_meet(*out, *own, M, d);
+    for (const G4qHeadRows* t : others) bad = bad || (t != nullptr && rows_meet(*out, *t, M, d));
     if (bad) throw Error(G4Q_ERR_INVALID_ARGUMENT, std::string(name) + " overlaps other rows of the call");
 }
 
@@ -1306,7 +1276,7 @@ G4qStatus g4q_paged_attention(const G4qAttn* attn, const G4qHeadRows* q, int64_t
                 "q and out must have the handle's query heads");
         require(M == 1 || q->token_stride >= a->head_dim, G4Q_ERR_INVALID_ARGUMENT, "q.token_stride must be >= head_dim");
         // several CTAs read a query row, and one may write its result before another has read it
-        require(!heads_overlap(*out, *q, M, a->head_dim), G4Q_ERR_INVALID_ARGUMENT, "out must not be q, nor overlap it");
+        require(!rows_meet(*out, *q, M, a->head_dim), G4Q_ERR_INVALID_ARGUMENT, "out must not be q, nor overlap it");
         check_apart(out, M, a->head_dim, "out");
         check_outside(out, M, *cache, cache_lattice(*cache), "out");
         AttnCall c = {};

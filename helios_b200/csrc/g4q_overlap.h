@@ -1,8 +1,8 @@
 // g4q_overlap.h -- whether the strided tensors of a call share elements: host arithmetic on addresses and strides.
 #pragma once
 
+#include <algorithm>
 #include <cstdint>
-#include <utility>
 
 #include "g4q.h"
 
@@ -98,6 +98,51 @@ inline bool rows_apart(const G4qHeadRows& r, int64_t M, int64_t d) {
         if (rest < d || (next && s - rest < d)) return false;
     }
     return true;
+}
+
+// Whether two tensors of M tokens of head rows may share elements, from the strides alone. Where these are alike (views of one
+// buffer) the places of the rows tell, else tensors whose spans overlap may.
+inline bool rows_may_meet(const G4qHeadRows& a, const G4qHeadRows& b, int64_t M, int64_t d) {
+    struct Axes {
+        int64_t outer, inner, span, inner_span;      // strides of the two axes, and extents in elements
+    };
+    auto axes = [&](const G4qHeadRows& t) {
+        const int64_t ts = M > 1 ? t.token_stride : 0, hs = t.n_heads > 1 ? t.head_stride : 0;
+        const bool tokens_out = ts >= hs;
+        Axes x;
+        x.outer = std::max(ts, hs), x.inner = std::min(ts, hs);
+        x.inner_span = x.inner * ((tokens_out ? t.n_heads : M) - 1) + d;
+        x.span = x.outer * ((tokens_out ? M : t.n_heads) - 1) + x.inner_span;
+        return x;
+    };
+    const Axes x = axes(a), y = axes(b);
+    const int64_t gap = b.data - a.data;             // both are 16-byte aligned
+    if (gap >= x.span || -gap >= y.span) return false;
+    if (x.outer != y.outer || x.outer < std::max(x.inner_span, y.inner_span)) return true;
+    auto inner_meet = [&](int64_t g) {               // one row of each, b's g elements on
+        if (g >= x.inner_span || -g >= y.inner_span) return false;
+        if (x.inner != y.inner || x.inner < d) return true;
+        const int64_t r = ((g % x.inner) + x.inner) % x.inner;
+        return r < d || x.inner - r < d;
+    };
+    if (x.outer == 0) return inner_meet(gap);
+    const int64_t r = ((gap % x.outer) + x.outer) % x.outer;
+    return inner_meet(r) || inner_meet(r - x.outer);
+}
+
+// Whether they do: where they may, the rows are looked at one by one before a call is refused. Exact unless both tensors have
+// rows that interleave.
+inline bool rows_meet(const G4qHeadRows& a, const G4qHeadRows& b, int64_t M, int64_t d) {
+    if (!rows_may_meet(a, b, M, d)) return false;
+    const Lattice la = rows_lattice(a, M, d), lb = rows_lattice(b, M, d);
+    if (!la.nested() && !lb.nested()) return true;
+    const G4qHeadRows &walk = lb.nested() ? a : b, &at = lb.nested() ? b : a;
+    const Lattice& l = lb.nested() ? lb : la;
+    const int64_t tokens = walk.token_stride == 0 ? 1 : M;
+    for (int64_t t = 0; t < tokens; ++t)
+        for (int64_t h = 0; h < walk.n_heads; ++h)
+            if (l.meets_row(walk.data - at.data + (Lattice::Wide)t * walk.token_stride + (Lattice::Wide)h * walk.head_stride)) return true;
+    return false;
 }
 
 // The slots of a cache's k (or v), one row a head.

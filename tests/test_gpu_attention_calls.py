@@ -128,6 +128,28 @@ def test_outputs_whose_rows_overlap_are_refused(cuda):
         assert torch.equal(attend(q, cache, batch, out=rows(hq, token, head)), want)
 
 
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_outputs_between_other_rows_qualify(cuda, tokens):
+    """Rows of different strides whose ends overlap while no element is shared: the keys between two heads of the queries'
+    output, a token's outputs behind its inputs in rows of other lengths."""
+    from helios_b200 import attention as A
+    d, hq, hk = 64, 4, 1
+    rope, pos = A.Rope(d), torch.arange(tokens, dtype=torch.int32, device="cuda")
+    q, k = bf16(tokens, hq, d, seed=1), bf16(tokens, hk, d, seed=2)
+    want = A.qk_norm_rope(q, k, pos, rope)
+    buf = torch.zeros(tokens, 16, d, dtype=torch.bfloat16, device="cuda")
+    k_in = buf[:, 1:2]
+    k_in.copy_(k)
+    got = A.qk_norm_rope(q, k_in, pos, rope, q_out=buf[:, 0:8:2], k_out=buf[:, 3:4])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    flat = torch.zeros(128 * d, dtype=torch.bfloat16, device="cuda")          # even places in, odd ones out
+    q_in, q_out = flat.as_strided((tokens, hq, d), (16 * d, 2 * d, 1)), flat.as_strided((tokens, hq, d), (32 * d, 4 * d, 1), d)
+    q_in.copy_(q)
+    assert torch.equal(A.qk_norm_rope(q_in, k, pos, rope, q_out=q_out)[0], want[0])
+    with pytest.raises(ValueError, match="overlaps other rows"):
+        A.qk_norm_rope(flat.as_strided((tokens, hq, d), (16 * d, 3 * d, 1)), k, pos, rope, q_out=q_out)
+
+
 def test_fields_assigned_after_the_first_call(cuda):
     """A batch whose max_q and table grow between two steps."""
     from helios_b200 import _lib

@@ -17,13 +17,19 @@ PROGRAM = r"""
 int main(int argc, char** argv) {
     G4qPagedCache c;
     long long k, v, n, ps, hs, ss, at, m, ts, rs;
-    G4qHeadRows r;
+    G4qHeadRows r, o;
     const std::string mode = argc > 1 ? argv[1] : "";
     while (mode == "apart" && std::scanf("%lld %d %lld %lld", &m, &r.n_heads, &ts, &rs) == 4) {
         r.token_stride = ts, r.head_stride = rs;
         std::printf("%d\n", (int)g4q::rows_apart(r, m, 8));
     }
-    while (std::scanf("%lld %lld %lld %d %d %lld %lld %lld", &k, &v, &n, &c.page_size, &c.n_kv_heads, &ps, &hs, &ss) == 8) {
+    while (mode == "pair" && std::scanf("%lld %lld %d %lld %lld %lld %d %lld %lld", &m, &k, &r.n_heads, &ts, &rs, &v, &o.n_heads,
+                                        &ps, &hs) == 9) {
+        r.data = (uint16_t*)0 + k, r.token_stride = ts, r.head_stride = rs;
+        o.data = (uint16_t*)0 + v, o.token_stride = ps, o.head_stride = hs;
+        std::printf("%d\n", (int)g4q::rows_meet(r, o, m, 8));
+    }
+    while (mode != "pair" && mode != "apart" && std::scanf("%lld %lld %lld %d %d %lld %lld %lld", &k, &v, &n, &c.page_size, &c.n_kv_heads, &ps, &hs, &ss) == 8) {
         c.k = (uint16_t*)0 + k, c.v = (uint16_t*)0 + v;
         c.n_pages = n, c.head_dim = 8;
         c.page_stride = ps, c.head_stride = hs, c.slot_stride = ss;
@@ -43,7 +49,8 @@ int main(int argc, char** argv) {
 def answers(tmp_path_factory):
     """Runs the program on cases, numbers each: (k, v, pages, page_size, heads, page_stride, head_stride, slot_stride) gives
     (nested, what is wrong). Mode "rows": the cases go on with (data, tokens, heads, token_stride, head_stride), and give
-    (nested, "meets" or "-"). Mode "apart": (tokens, heads, token_stride, head_stride) gives (apart, "")."""
+    (nested, "meets" or "-"). Mode "apart": (tokens, heads, token_stride, head_stride) gives (apart, "").
+    Mode "pair": (tokens, data, heads, token_stride, head_stride, data, heads, token_stride, head_stride) gives (meet, "")."""
     at = tmp_path_factory.mktemp("overlap")
     (at / "main.cpp").write_text(PROGRAM)
     subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover", "-I",
@@ -151,3 +158,33 @@ def test_rows_of_an_output_against_sets_of_elements(answers):
     assert [a for a, _ in answers([(many, 16, 128, 8), (many, 16, 8, 8 * many), (many, 16, 8, 8), (many, 2, 16, 8 * 3),
                                    (many, 1, 0, 0), (1, 16, 0, 8), (many, many, 2 ** 40, 2 ** 41)], "apart")] == \
         [True, True, False, True, False, True, False]
+
+
+def test_two_tensors_of_rows_against_sets_of_elements(answers):
+    """Exact where one of the two has no rows that overlap; else nothing that is shared is missed."""
+    rng = random.Random(4)
+    cases = []
+    for _ in range(20000):
+        m, at = rng.randrange(1, 5), 4096
+        strides = []
+        for _ in range(2):
+            heads, inner = rng.randrange(1, 5), 8 * rng.choice([1, 1, 2, 3])
+            tokens_out = rng.random() < 0.6
+            outer = inner * (heads if tokens_out else m) + 8 * rng.randrange(-1, 7)
+            strides.append((heads, outer, inner) if tokens_out else (heads, inner, outer))
+        if rng.random() < 0.5:
+            strides[1] = (strides[1][0], *strides[0][1:])
+        cases.append((m, at, *strides[0], at + 8 * rng.randrange(-30, 31), *strides[1]))
+    seen = [0, 0, 0]
+    for case, (meet, _) in zip(cases, answers(cases, "pair")):
+        m, a, na, ta, ha, b, nb, tb, hb = case
+        ea, eb = elements(rows(a, (m, na), (ta, ha))), elements(rows(b, (m, nb), (tb, hb)))
+        real = bool(set(ea) & set(eb))
+        assert meet or not real, case
+        if len(set(ea)) < len(ea) and len(set(eb)) < len(eb):
+            continue
+        interleaved = min(len(set(ea)), len(set(eb))) and (max(ea) > min(eb) and max(eb) > min(ea)) and not real
+        seen[0 if real else 2 if interleaved else 1] += 1
+        nested = [t >= h * (n - 1) + D or h >= t * (m - 1) + D or n == 1 or m == 1 for n, t, h in ((na, ta, ha), (nb, tb, hb))]
+        assert meet == real or not any(nested), case
+    assert min(seen) > 1000, seen
