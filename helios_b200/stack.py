@@ -529,6 +529,8 @@ class DecoderStack:
             res = rms_norm_residual(down, L["post_ffn"], res, L["scalar"], c.eps)
         if rows is None:
             return None, res
+        if rows.numel() == 0:      # a chunk in the middle of every prompt
+            return torch.empty(0, dtype=torch.int64, device=h.device), res
         last = rms_norm(res[rows], self.final_norm, c.eps)
         keys = [lm_head_argmax(x, self.lm, softcap=c.softcap, row_offset=self.v_rows[0])[2] for x in last.split(16)]
         return torch.cat(keys), res

@@ -60,3 +60,25 @@ def test_decoder_stack_forward_after_the_attention(cuda):
         assert (top - mine <= 4 * 2.0 ** -8 * top.abs()).all()
         assert len(set(tokens)) > 1
     st.free()
+
+
+def test_decoder_stack_forward_without_rows_or_tokens(cuda):
+    """A step that wants no token (a chunk in the middle of a prompt), and one without new tokens."""
+    from helios_b200 import attention as A
+    from helios_b200.quantized import synth_normal
+    from helios_b200.stack import DecoderStack, StackConfig
+    st = DecoderStack(StackConfig(layers=2, hidden=512, q_out=256, kv_out=128, inter=1024, vocab=2048))
+    st.attach_attention(8, 16, head_dim=64, window=0)
+    int32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    h = synth_normal(7, (40, 512))
+    batch = A.PagedBatch(int32([0, 40]), int32([40]), int32([[3, 1, 2]]), max_q=40)
+    keys, res = st.forward(h, batch, rows=torch.empty(0, dtype=torch.int64, device="cuda"))
+    none, again = st.forward(h, batch)
+    assert keys.shape == (0,) and keys.dtype is torch.int64 and none is None and torch.equal(res, again)
+    before = [L["cache"].k.clone() for L in st.layers]
+    batch.q_offsets = int32([0, 0])
+    keys, res = st.forward(h[:0], batch, rows=torch.empty(0, dtype=torch.int64, device="cuda"))
+    assert keys.shape == (0,) and res.shape == (0, 512)
+    assert all(torch.equal(a, L["cache"].k) for a, L in zip(before, st.layers))
+    no_device_error()
+    st.free()
