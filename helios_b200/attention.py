@@ -205,7 +205,7 @@ def kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cache
     """The new tokens of a step, at their positions: keys normalized, weighted and rotated into the cache's
     pages, values normalized (without a weight; ``norm_values=False`` stores them as they are) beside them,
     and the queries, treated like the keys with ``q_weight``, returned (None for q None). One launch. ``v``
-    may be ``k``. Sequences may share pages of a common prefix, but no two may append to one slot. Rows that
+    may be ``k``. Sequences may share pages of a common prefix, but no two new tokens may go to one slot. Rows that
     belong to no sequence are left as they were (in ``q_out`` too). No tensor may overlap the cache."""
     dev = rope.device
     _same_device(dev, cache, batch)

@@ -1,6 +1,6 @@
 // g4q_attn.cu -- attention of a few new tokens per sequence over a paged cache (sm_100a): one decoded token
 // each, or a block of drafted ones, up to 64 query rows (tokens x query heads of a key head) per key head (32 at
-// head_dim 512).
+// head_dim 512; in a step that has longer sequences too 16, or the rows of one token).
 //
 //   out = softmax(scale * q k^T + mask) v, masked to the positions j <= t (and j > t - window)
 //
@@ -18,9 +18,9 @@
 // to 16); the running softmax is in fp32 over 16-key slices per thread; for the output, warp w takes head_dim/8
 // columns over the 64 keys. mma.sync is enough here: at 64 rows a tile's products take less time than its bytes.
 //
-// Measured, with the join: 16 tokens over 69,823 keys in all (8 key heads of 256) 95 us, 6.0 TB/s of keys and values;
-// one token over a window of 1024 7.5 us and over 16384 keys of head_dim 512 12.4 us, latencies of a tile or two in
-// sequence and of the join.
+// Measured, with the join, a call with new inputs (in brackets: with the same ones in a graph): 16 tokens over 69,823 keys
+// in all (8 key heads of 256) 98 us (96), 5.8 TB/s of keys and values; one token over a window of 1024 8.7 us (8.0) and
+// over 16384 keys of head_dim 512 16.1 us (12.4), latencies of a tile or two in sequence and of the join.
 #include <cuda_runtime.h>
 
 #include <algorithm>

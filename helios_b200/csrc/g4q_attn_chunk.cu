@@ -1,5 +1,6 @@
-// g4q_attn_chunk.cu -- attention of a prompt's chunk (more than 64 query rows per key head) over a paged
-// cache, on the 5th-generation tensor cores (sm_100a).
+// g4q_attn_chunk.cu -- attention of a prompt's chunk over a paged cache, on the 5th-generation tensor cores (sm_100a): the
+// sequences of more query rows per key head than the kernel of few rows takes, which are 64 (32 at head_dim 512), and in a
+// step that mixes both 16 (or the rows of one token, where those are more).
 //
 //   out = softmax(scale * q k^T + mask) v, masked to the positions j <= t (and j > t - window)
 //
@@ -22,10 +23,11 @@
 //               softmax was 1550 cycles of one warp per scheduler: 2530 cycles a tile at head_dim 256, now 2050.
 //
 // Bound by the tensor cores for a long context: a key tile takes its products' cycles (2050 measured of 2048 at head_dim
-// 256, three times 1024 at 512). 2048 tokens of 16 heads of 512 over 16384 keys: 900 us, at the 1.5 GHz that the power
-// limit leaves (1.7 PFLOP/s of products). 2048 tokens of 16 heads of 256 with a window of 1024, 9 or 10 key tiles a row
-// tile: 36 us at full clock, of which the start (finding the work 2 us, Q and K, the first softmax: 5 us) and each
-// tile's epilogue (2 us) are latency. head_dim 128 and 64: the exponentials, 1024 cycles of a tile, and 1750 a tile.
+// 256, three times 1024 at 512). 2048 tokens of 16 heads of 512 over 16384 keys: 1040 us a call, at the 1.4 GHz that the
+// power limit leaves (1.49 PFLOP/s of products; the first ten calls from idle take 910 us each, 1.70). 2048 tokens of 16
+// heads of 256 with a window of 1024, 9 or 10 key tiles a row tile: 43 us a call with new inputs, 39 with the same ones at
+// 1.8 GHz, of which the start (finding the work 2 us, Q and K, the first softmax: 5 us) and each tile's epilogue (2 us) are
+// latency. head_dim 128 and 64: the exponentials, 1024 cycles of a tile, and 1750 a tile.
 //
 // head_dim 64: a pair would leave each CTA 32 columns of V, less than a swizzle row, and its tiles' bytes are few
 // for the softmax they take: single CTAs (cta_group::1) run the same code.
@@ -303,7 +305,7 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
 
 // True for one thread of a converged warp. The compiler knows that the code behind it is one thread's, and keeps the
 // operands of the MMAs in uniform registers: with a test of the lane it moved them there before every MMA, 65 to 85
-// cycles each (2048 tokens, 16384 keys of head_dim 512: 970 us against 900).
+// cycles each (2048 tokens, 16384 keys of head_dim 512, ten calls from idle: 970 us against 900).
 __device__ __forceinline__ bool elect() {
     uint32_t one;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));

@@ -486,8 +486,9 @@ class DecoderStack:
     def attach_attention(self, n_pages: int, page_size: int = 64, *, head_dim: int = 256, window: int = 1024,
                          scale: Optional[float] = None, base: float = 10000.0, rotary_dim: Optional[int] = None) -> None:
         """Give every layer a paged key/value cache of ``n_pages`` pages and seeded query and key norm weights,
-        for :meth:`forward`. ``window``: of the sliding-window layers (0: none); ``scale``: of the scores
-        (default ``head_dim ** -0.5``)."""
+        for :meth:`forward`. All layers have the same head layout, rotation and window (0: none), with a value projection
+        of their own; layers that differ (a full-attention layer whose key is the value too) call the operators of
+        ``helios_b200.attention`` one by one. ``scale``: of the scores (default ``head_dim ** -0.5``)."""
         if self.size != 1:
             raise ValueError("attention in the stack runs on one GPU")
         if self.nq % head_dim or self.nkv % head_dim:

@@ -311,7 +311,7 @@ typedef struct G4qPagedCache {
  * what they hold then): sequence b owns the rows [q_offsets[b], q_offsets[b+1]) of the step's M new tokens,
  * which are the last ones of its kv_lens[b] tokens (the new ones included); its position j is in page
  * block_table[b * table_stride + j / page_size] at slot j % page_size. Sequences may share pages (a common
- * prefix), but no two may append to one slot. Table entries of pages without a token
+ * prefix), but no two new tokens may go to one slot. Table entries of pages without a token
  * to read or write are not looked at. max_q: at least the longest q_offsets[b+1] - q_offsets[b]. Rows before
  * q_offsets[0] or behind q_offsets[n_seqs] belong to no sequence and are left as they were. What the arrays
  * hold is checked on the device: nothing outside of the cache, the table or the rows is touched, and
